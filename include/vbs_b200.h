@@ -257,6 +257,159 @@ VBS_API int vbs_cu_attention_static(const float *q, const uint16_t *kc, const ui
                                     uint32_t n_kv_heads, uint32_t head_dim, float scale, uint32_t batch,
                                     uint64_t kv_batch_stride, void *stream);
 
+/* ---- a cache whose slots are not positions (no reference counterpart) ----
+ * vbs_cu_attention and the decoders keep position t in slot t. Verifying a
+ * tree of drafted tokens, serving padded prompts, positions with several
+ * axes, and evicting positions from a cache all break that rule: these
+ * entry points take slots and positions apart. They share one description
+ * of a cache. Device pointers throughout, fp32 activations, fp16 cache; the
+ * work is queued on `stream` of the current device and no call allocates or
+ * synchronizes, so every one can be captured into a graph. Values that are
+ * read on the device (lengths, slots, lists) cannot be refused by the call:
+ * a bad one sets the device error word, which the next synchronising call
+ * of the library reports, and the rows it concerns are left as they were. */
+
+/* One cache for n_seqs sequences. Within a sequence: [layer][position]
+ * [kv head][head_dim] (the engine's order), or with head_major
+ * [layer][kv head][position][head_dim]. Sequence s starts seq_stride * s
+ * elements in. head_dim a multiple of 8, at most 256; k and v 16-byte
+ * aligned, seq_stride a multiple of 8. */
+typedef struct {
+    uint16_t *k, *v;
+    uint32_t n_layers, max_ctx, n_kv_heads, head_dim, n_seqs;
+    uint32_t head_major;
+    uint64_t seq_stride;
+} vbs_cu_kv_t;
+
+/* Rotary positions: what vbs_cu_rope_init fills and vbs_cu_rope_store takes.
+ * Pair p of a head turns by turn[p] * position[axis[p]] full circles, in
+ * units of 2^-64: the product wraps modulo one circle, so far positions
+ * lose nothing. */
+typedef struct {
+    uint32_t head_dim, rot_dim, n_axes, halves;
+    uint64_t turn[128];
+    uint8_t axis[128];
+} vbs_cu_rope_t;
+
+/* Host only. Pair p < rot_dim / 2 has the angle position * theta^(-2p /
+ * rot_dim) / freq_factors[p] (freq_factors: host array, NULL: 1); dims from
+ * rot_dim on are not turned. A pair is dims (2p, 2p + 1), as in the
+ * engine's ROTARY primitive (src/vbs_host_math.h:38-51), or with halves
+ * (p, p + rot_dim / 2). n_axes 1..4 positions per token (time, height,
+ * width, ...): sections[a] pairs belong to axis a (host array, their sum
+ * rot_dim / 2; NULL with one axis), one axis after the other, or with
+ * interleaved in turn: pair p goes to axis p % n_axes while that axis has
+ * pairs left, and to axis 0 after that. head_dim and rot_dim multiples of
+ * 8, rot_dim <= head_dim <= 256. 0, or -1 with the error latched. */
+VBS_API int vbs_cu_rope_init(vbs_cu_rope_t *r, uint32_t head_dim, uint32_t rot_dim, uint32_t halves, float theta,
+                             const float *freq_factors, uint32_t n_axes, const uint32_t *sections, uint32_t interleaved);
+
+/* For n_tokens tokens: q_out = the query heads turned to the token's
+ * position; the key heads, turned, and the value heads go into slot[i] of
+ * sequence seq[i] (NULL: sequence 0) of `layer` as fp16, rounded as the
+ * engine's CACHE primitive does. pos: [n_tokens][n_axes], any int32. q rows
+ * of q_stride floats (0: n_q_heads * head_dim), k and v rows of kv_stride
+ * floats (0: n_kv_heads * head_dim); q_out rows have no gaps and q_out may
+ * be q when q has none either. n_q_heads 0 (q and q_out NULL) only stores;
+ * k and v NULL only turns the queries (kv, slot and seq are not used and
+ * may be NULL). slot -1 stores nothing for that token. Slots of one call are
+ * distinct; given twice, the slot holds a mix of the two tokens. Pointers
+ * 16-byte aligned, strides multiples of 4. */
+VBS_API int vbs_cu_rope_store(const vbs_cu_rope_t *r, const vbs_cu_kv_t *kv, uint32_t layer, const float *q,
+                              uint64_t q_stride, float *q_out, uint32_t n_q_heads, const float *k, const float *v,
+                              uint64_t kv_stride, uint32_t n_tokens, const int32_t *pos, const int32_t *seq,
+                              const int32_t *slot, void *stream);
+
+/* Attention of new tokens (a tree or chain of drafts, a prompt's chunk, one
+ * decoded token) over a cache. Sequence s has n_ctx[s] slots of context, 0..,
+ * and its n_tok[s] new tokens' keys and values are in the slots behind them.
+ * Token i of sequence s has its query heads at q[s][i] and its result at
+ * out[s][i] ([n_seqs][n_tokens][n_q_heads][head_dim]; rows from n_tok[s] on
+ * are left as they were).
+ *  - It sees every slot of the context, and new token j when bit j % 32 of
+ *    mask[s][i][j / 32] is set (mask NULL: j <= i). A row that sees nothing
+ *    gets zeros. What a row does not see does not reach it, whatever it
+ *    holds.
+ *  - Score: x = scale * q . k; softcap > 0: softcap * tanh(x / softcap);
+ *    slopes: + slopes[head] * (key position - query position).
+ *  - window > 0: only keys with query position - key position < window.
+ *  - Positions (used by slopes and window): q_pos[s][i], NULL: n_ctx[s] + i;
+ *    k_pos[s][slot] ([s][kv head][slot] with k_pos_per_head), rows of max_ctx,
+ *    for every slot below n_ctx[s] + n_tok[s], a negative one marking a slot
+ *    that nobody sees (padding, a hole); NULL: the slot's number for the
+ *    context and q_pos for the new tokens. Without k_pos a window also
+ *    saves reading what it leaves out.
+ *  - weights_out: [n_seqs][kv head][max_ctx], the attention weights of every
+ *    slot below n_ctx + n_tok, summed over the tokens and the query heads of
+ *    its KV head, added to weights_in (NULL: 0; may be weights_out itself);
+ *    slots from there on are left as they were.
+ * n_q_heads is a multiple of the cache's n_kv_heads, at most 256 of them per
+ * KV head; n_tokens at most 4096. ctx_limit: an upper
+ * bound of n_ctx + n_tok over the sequences, known on the host; it sizes the
+ * split of long contexts and the workspace, n_ctx and n_tok are read on the
+ * device. Sums and softmax are fp32; fp32 queries and weights enter the
+ * tensor cores as two fp16 halves each (exact to about 2^-22). */
+typedef struct {
+    uint32_t n_q_heads, n_tokens;
+    float scale, softcap;
+    uint32_t window, ctx_limit;
+    const float *slopes;        /* [n_q_heads] */
+    const int32_t *n_ctx;       /* [n_seqs] */
+    const int32_t *n_tok;       /* [n_seqs]; NULL: n_tokens each */
+    const uint32_t *mask;       /* [n_seqs][n_tokens][(n_tokens + 31) / 32] */
+    const int32_t *q_pos;       /* [n_seqs][n_tokens] */
+    const int32_t *k_pos;
+    uint32_t k_pos_per_head;
+    const float *weights_in;
+    float *weights_out;
+} vbs_cu_tree_t;
+
+/* Workspace of the call below, in bytes (a multiple of 256, at least 256);
+ * 0 with the error latched for a bad description. The caller owns the
+ * workspace: two calls that can overlap in time (other streams, captured
+ * graphs) take one each. Nothing in it is kept between calls. */
+VBS_API size_t vbs_cu_tree_workspace(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t);
+VBS_API int vbs_cu_attention_tree(const vbs_cu_kv_t *kv, uint32_t layer, const vbs_cu_tree_t *t, const float *q, float *out,
+                                  void *work, size_t work_bytes, void *stream);
+
+/* Which slots an eviction keeps: for every list [layer][seq][kv head] of
+ * n[seq] scores (rows of `stride` floats; n <= n_limit <= stride), the first
+ * `first` slots, the last `recent`, and of those between the ones with the
+ * highest scores, `keep` in all. idx[list][keep] receives them in ascending
+ * order, -1 behind them; count[seq] = min(n, keep). Of equal scores the lower
+ * slot is kept; a NaN counts as the lowest score, -0 as 0. first + recent <=
+ * keep; n_limit at most 393216. */
+VBS_API int vbs_cu_cache_select(const float *scores, uint64_t stride, uint32_t n_layers, uint32_t n_seqs, uint32_t n_kv_heads,
+                                const int32_t *n, uint32_t n_limit, uint32_t keep, uint32_t first, uint32_t recent,
+                                int32_t *idx, int32_t *count, void *stream);
+
+/* Row moves: for every layer, sequence s and KV head, the rows of list
+ * idx + layer * layer_stride + s * seq_stride + head * head_stride (elements;
+ * 0: shared), entries i < count[s] <= n_max: slot src_base[s] + idx[i] of src
+ * to slot dst_base[s] + i of dst (bases NULL: 0). Serves an eviction
+ * (vbs_cu_cache_select's lists) and the accepted branch of a draft tree
+ * (src_base = dst_base = n_ctx, one list per sequence).
+ *  - src and dst have the same layers, sequences, heads and head_dim; order
+ *    and max_ctx may differ. They are the same cache, or do not overlap.
+ *  - In the same cache the lists ascend and no row moves up (src_base +
+ *    idx[i] >= dst_base + i); a list that breaks this moves nothing and
+ *    sets the device error word.
+ *  - weights and positions ([layer][seq][kv head][max_ctx], as
+ *    vbs_cu_attention_tree takes them layer by layer) move along with
+ *    their rows when given. */
+typedef struct {
+    uint32_t n_max;
+    const int32_t *idx;
+    uint64_t layer_stride, seq_stride, head_stride;
+    const int32_t *count;       /* [n_seqs] */
+    const int32_t *src_base, *dst_base;   /* [n_seqs] */
+    const float *weights_src;
+    float *weights_dst;
+    const int32_t *pos_src;
+    int32_t *pos_dst;
+} vbs_cu_gather_t;
+VBS_API int vbs_cu_cache_gather(const vbs_cu_kv_t *src, const vbs_cu_kv_t *dst, const vbs_cu_gather_t *g, void *stream);
+
 /* Seeded synthetic weights: the [rows x cols] tile at (row0, col0) of a
  * tensor with full_cols columns, element (r, c) drawn from the Irwin-Hall
  * (n = 4) normal approximation of stream `seed` at index r*full_cols + c,

@@ -131,6 +131,35 @@ class ModelDesc(C.Structure):
     ]
 
 
+class KvDesc(C.Structure):
+    """vbs_cu_kv_t: an fp16 cache of n_seqs sequences (device pointers)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("n_layers", C.c_uint32), ("max_ctx", C.c_uint32),
+                ("n_kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("n_seqs", C.c_uint32), ("head_major", C.c_uint32),
+                ("seq_stride", C.c_uint64)]
+
+
+class RopeDesc(C.Structure):
+    """vbs_cu_rope_t: filled by rope_plan()."""
+    _fields_ = [("head_dim", C.c_uint32), ("rot_dim", C.c_uint32), ("n_axes", C.c_uint32), ("halves", C.c_uint32),
+                ("turn", C.c_uint64 * 128), ("axis", C.c_uint8 * 128)]
+
+
+class TreeDesc(C.Structure):
+    """vbs_cu_tree_t: one attention call of new tokens over a cache."""
+    _fields_ = [("n_q_heads", C.c_uint32), ("n_tokens", C.c_uint32), ("scale", C.c_float), ("softcap", C.c_float),
+                ("window", C.c_uint32), ("ctx_limit", C.c_uint32), ("slopes", C.c_void_p), ("n_ctx", C.c_void_p),
+                ("n_tok", C.c_void_p), ("mask", C.c_void_p), ("q_pos", C.c_void_p), ("k_pos", C.c_void_p),
+                ("k_pos_per_head", C.c_uint32), ("weights_in", C.c_void_p), ("weights_out", C.c_void_p)]
+
+
+class GatherDesc(C.Structure):
+    """vbs_cu_gather_t: the lists of a row move."""
+    _fields_ = [("n_max", C.c_uint32), ("idx", C.c_void_p), ("layer_stride", C.c_uint64), ("seq_stride", C.c_uint64),
+                ("head_stride", C.c_uint64), ("count", C.c_void_p), ("src_base", C.c_void_p), ("dst_base", C.c_void_p),
+                ("weights_src", C.c_void_p), ("weights_dst", C.c_void_p), ("pos_src", C.c_void_p),
+                ("pos_dst", C.c_void_p)]
+
+
 _LIB = None
 
 
@@ -165,6 +194,13 @@ def lib() -> C.CDLL:
         "vbs_cu_ffn_gate_up": (i32, [i32, vp, vp, vp, vp, f32, vp, u32, u32, vp]),
         "vbs_cu_attention": (i32, [vp, vp, vp, vp, u32, u32, u32, u32, u32, u32, f32, u32, u64, vp]),
         "vbs_cu_attention_static": (i32, [vp, vp, vp, vp, u32, u32, u32, u32, u32, u32, f32, u32, u64, vp]),
+        "vbs_cu_rope_init": (i32, [C.POINTER(RopeDesc), u32, u32, u32, f32, vp, u32, vp, u32]),
+        "vbs_cu_rope_store": (i32, [C.POINTER(RopeDesc), C.POINTER(KvDesc), u32, vp, u64, vp, u32, vp, vp, u64, u32, vp, vp,
+                                    vp, vp]),
+        "vbs_cu_tree_workspace": (sz, [C.POINTER(KvDesc), C.POINTER(TreeDesc)]),
+        "vbs_cu_attention_tree": (i32, [C.POINTER(KvDesc), u32, C.POINTER(TreeDesc), vp, vp, vp, sz, vp]),
+        "vbs_cu_cache_select": (i32, [vp, u64, u32, u32, u32, vp, u32, u32, u32, u32, vp, vp, vp]),
+        "vbs_cu_cache_gather": (i32, [C.POINTER(KvDesc), C.POINTER(KvDesc), C.POINTER(GatherDesc), vp]),
         "vbs_cu_synth": (i32, [i32, vp, u64, u64, u64, u64, u64, u64, f32, vp]),
         "vbs_cu_upload_file": (i32, [C.c_char_p, sz, vp, vp, vp, u32, u64]),
         "vbs_cu_decoder_create": (vp, [C.POINTER(ModelDesc), u32, u32, C.c_char_p, sz]),
@@ -251,6 +287,54 @@ def attention_static(q, kc, vc, out, seq_len, layer, max_ctx, nqh, nkh, hd, scal
     and no device allocation (see include/vbs_b200.h for its limit)."""
     check(lib().vbs_cu_attention_static(q, kc, vc, out, seq_len, layer, max_ctx, nqh, nkh, hd, scale, batch,
                                         kv_batch_stride, stream or None), "vbs_cu_attention_static")
+
+
+def rope_plan(head_dim, rot_dim=0, theta=10000.0, halves=False, freq_factors=None, sections=None,
+              interleaved=False) -> RopeDesc:
+    """vbs_cu_rope_init: the turns of a head's pairs. rot_dim 0: the whole
+    head; sections: pairs per position axis (None: one axis). Host only."""
+    rot = rot_dim or head_dim
+    if freq_factors is not None and len(freq_factors) != rot // 2:
+        raise ValueError(f"{len(freq_factors)} frequency factors for {rot // 2} pairs")
+    fac = (C.c_float * len(freq_factors))(*freq_factors) if freq_factors is not None else None
+    sec = (C.c_uint32 * len(sections))(*sections) if sections is not None else None
+    r = RopeDesc()
+    check(lib().vbs_cu_rope_init(C.byref(r), head_dim, rot, int(halves), theta, fac, len(sections) if sections is not None
+                                 else 1, sec, int(interleaved)), "vbs_cu_rope_init")
+    return r
+
+
+def rope_store(rope, kv, layer, q, q_out, n_q_heads, k, v, n_tokens, pos, slot, seq=0, q_stride=0, kv_stride=0, stream=0):
+    """vbs_cu_rope_store: turn q and k to their positions, store k and v."""
+    check(lib().vbs_cu_rope_store(C.byref(rope), C.byref(kv) if kv is not None else None, layer, q or None, q_stride,
+                                  q_out or None, n_q_heads, k or None, v or None, kv_stride, n_tokens, pos, seq or None,
+                                  slot or None, stream or None), "vbs_cu_rope_store")
+
+
+def tree_workspace(kv, tree) -> int:
+    """Bytes of workspace that attention_tree needs for this description."""
+    n = int(lib().vbs_cu_tree_workspace(C.byref(kv), C.byref(tree)))
+    if not n:
+        raise VbsError(f"vbs_cu_tree_workspace: {last_error()}")
+    return n
+
+
+def attention_tree(kv, layer, tree, q, out, work, work_bytes, stream=0):
+    """vbs_cu_attention_tree: new tokens (drafts in a tree or chain, a chunk,
+    one token) over a cache, into `out`; see include/vbs_b200.h."""
+    check(lib().vbs_cu_attention_tree(C.byref(kv), layer, C.byref(tree), q, out, work, work_bytes, stream or None),
+          "vbs_cu_attention_tree")
+
+
+def cache_select(scores, stride, n_layers, n_seqs, n_kv_heads, n, n_limit, keep, first, recent, idx, count, stream=0):
+    """vbs_cu_cache_select: the slots an eviction keeps, ascending."""
+    check(lib().vbs_cu_cache_select(scores, stride, n_layers, n_seqs, n_kv_heads, n, n_limit, keep, first, recent, idx, count,
+                                    stream or None), "vbs_cu_cache_select")
+
+
+def cache_gather(src, dst, gather, stream=0):
+    """vbs_cu_cache_gather: listed rows of `src` to consecutive rows of `dst`."""
+    check(lib().vbs_cu_cache_gather(C.byref(src), C.byref(dst), C.byref(gather), stream or None), "vbs_cu_cache_gather")
 
 
 def synth(type_id, dst_ptr, rows, cols, seed, scale, row0=0, col0=0, full_cols=None, stream=0) -> None:

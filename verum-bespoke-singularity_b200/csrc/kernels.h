@@ -333,6 +333,12 @@ cudaError_t strict_add_launch(float *x, const float *t, uint32_t n, cudaStream_t
 cudaError_t synth_launch(int type, uint8_t *dst, uint64_t rows, uint64_t cols, uint64_t row0, uint64_t col0,
                          uint64_t full_cols, uint64_t seed, float scale, cudaStream_t st);
 
+// ---- caches whose slots are not positions (slots.cu, tree.cu) ------------------
+// Shared-memory limits on the current device (once per device, outside stream
+// capture).
+cudaError_t slots_configure();
+cudaError_t tree_configure();
+
 // Launch bookkeeping (counts kernels for vbs_cu_kernel_launches).
 void note_launches(uint64_t n);
 

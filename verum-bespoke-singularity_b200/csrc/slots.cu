@@ -1,0 +1,721 @@
+// slots.cu -- the cache whose slots are not positions: rotary positions with
+// a store into given slots, the choice of the slots that an eviction keeps,
+// and the move of listed rows. (The attention over such a cache: tree.cu.)
+//
+// The engine keeps position t in slot t (src/vbs_host_math.h:150-159, the
+// CACHE primitive) and turns every head by that one position
+// (src/vbs_host_math.h:38-51, ROTARY); these kernels take both as lists.
+#include "vbs_b200.h"
+#include "backend.h"
+#include "common.cuh"
+#include "kernels.h"
+
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <cmath>
+
+namespace vbs {
+
+namespace cg = cooperative_groups;
+
+bool kv_desc_ok(const vbs_cu_kv_t *kv) {
+    if (!kv || !kv->k || !kv->v || !kv->n_layers || !kv->max_ctx || !kv->n_kv_heads || !kv->n_seqs) return false;
+    if (kv->max_ctx > 0x7FFFFFFFu || !kv->head_dim || kv->head_dim % 8 || kv->head_dim > 256) return false;
+    if ((reinterpret_cast<uintptr_t>(kv->k) | reinterpret_cast<uintptr_t>(kv->v)) & 15) return false;
+    if (kv->n_kv_heads > 65535u || kv->n_seqs > 65535u) return false;
+    return kv->seq_stride % 8 == 0 && (kv->n_seqs == 1 || kv->seq_stride);
+}
+
+// ---------------------------------------------------------------------------
+// Rotary positions and store.
+//   q' = R q, K[slot] = fp16(R k), V[slot] = fp16(v); pair (a, b) of R:
+//   (a cos - b sin, a sin + b cos) at pos[axis] * turn circles.
+// The circle is 2^64 units, so position * turn is one wrapping 64-bit
+// product and its top 32 bits are the fraction of a circle, to 2^-32 for
+// positions up to 2^20 or so (turn itself is exact to 2^-53): the angle of a
+// far position costs no 64-bit float arithmetic.
+// Bound by memory: 8 bytes per query element, 6 per cached one. A thread owns
+// 8 dims (4 pairs) of every head it visits, so the four sines and cosines
+// are computed once and stay in registers; heads are spread over the block
+// (and, for few tokens, over blockIdx.y), and the loads of ROPE_U heads are
+// issued before the first is used.
+// ---------------------------------------------------------------------------
+constexpr int ROPE_THREADS = 256, ROPE_U = 4;
+
+struct RopeParams {
+    vbs_cu_rope_t r;
+    const float *q, *k, *v;
+    float *q_out;
+    uint16_t *kc, *vc;          // layer's first element of sequence 0
+    uint64_t q_stride, kv_stride, seq_stride, pos_step, head_step;
+    uint32_t nqh, nkh, max_ctx, n_seqs;
+    const int32_t *pos, *seq, *slot;
+    uint32_t *err;
+};
+
+__device__ __forceinline__ uint4 pack_kv(const float4 &a, const float4 &b) {
+    uint4 w;
+    w.x = f32_to_f16_kv(a.x) | ((uint32_t)f32_to_f16_kv(a.y) << 16);
+    w.y = f32_to_f16_kv(a.z) | ((uint32_t)f32_to_f16_kv(a.w) << 16);
+    w.z = f32_to_f16_kv(b.x) | ((uint32_t)f32_to_f16_kv(b.y) << 16);
+    w.w = f32_to_f16_kv(b.z) | ((uint32_t)f32_to_f16_kv(b.w) << 16);
+    return w;
+}
+
+__global__ void __launch_bounds__(ROPE_THREADS) rope_store_kernel(const __grid_constant__ RopeParams p) {
+    const uint32_t hd = p.r.head_dim, units = hd / 8, rows_blk = ROPE_THREADS / units;
+    const uint32_t u = threadIdx.x % units, tok = blockIdx.x;
+    uint32_t row = threadIdx.x / units + blockIdx.y * rows_blk;
+    if (threadIdx.x >= rows_blk * units) return;
+    const uint32_t step = rows_blk * gridDim.y, rot = p.r.rot_dim;
+    const uint32_t rows = p.nqh + (p.k ? 2 * p.nkh : 0u);
+    // dims of this thread: da.. and db.., 4 each; pairs are inside a float4
+    // (adjacent) or across the two (halves)
+    const bool turned = 8 * u < rot;
+    const bool halves = turned && p.r.halves;
+    const uint32_t da = halves ? 4 * u : 8 * u, db = halves ? rot / 2 + 4 * u : 8 * u + 4;
+
+    int32_t slot = -1;
+    uint64_t at0 = 0;
+    if (p.k) {
+        slot = p.slot[tok];
+        const int32_t s = p.seq ? p.seq[tok] : 0;
+        if (slot < -1 || slot >= (int32_t)p.max_ctx || s < 0 || s >= (int32_t)p.n_seqs) {
+            if (threadIdx.x == 0) dev_flag_error(p.err, DERR_BAD_ARG);
+            slot = -1;
+        }
+        if (slot >= 0) at0 = (uint64_t)s * p.seq_stride + (uint64_t)slot * p.pos_step;
+    }
+    float c[4], sn[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        c[i] = 1.f;
+        sn[i] = 0.f;
+        if (turned) {
+            const uint32_t pr = 4 * u + i;
+            const int64_t ps = p.pos[(uint64_t)tok * p.r.n_axes + p.r.axis[pr]];
+            const int32_t frac = (int32_t)(((uint64_t)ps * p.r.turn[pr]) >> 32);   // of a circle, in 2^-32
+            sincospif((float)frac * 0x1p-31f, &sn[i], &c[i]);
+        }
+    }
+    auto src = [&](uint32_t rw) -> const float * {
+        if (rw < p.nqh) return p.q + (uint64_t)tok * p.q_stride + (uint64_t)rw * hd;
+        const uint32_t h = rw - p.nqh;
+        return h < p.nkh ? p.k + (uint64_t)tok * p.kv_stride + (uint64_t)h * hd
+                         : p.v + (uint64_t)tok * p.kv_stride + (uint64_t)(h - p.nkh) * hd;
+    };
+    for (; row < rows; row += step * ROPE_U) {
+        float4 xa[ROPE_U], xb[ROPE_U];
+#pragma unroll
+        for (int j = 0; j < ROPE_U; ++j) {
+            const uint32_t rw = row + j * step;
+            if (rw >= rows || (rw >= p.nqh && slot < 0)) continue;
+            const float *s = src(rw);
+            xa[j] = *reinterpret_cast<const float4 *>(s + da);
+            xb[j] = *reinterpret_cast<const float4 *>(s + db);
+        }
+#pragma unroll
+        for (int j = 0; j < ROPE_U; ++j) {
+            const uint32_t rw = row + j * step;
+            if (rw >= rows || (rw >= p.nqh && slot < 0)) continue;
+            const float4 a = xa[j], b = xb[j];
+            float4 ya = a, yb = b;
+            if (turned && rw < p.nqh + p.nkh) {
+                if (halves) {
+                    ya = make_float4(a.x * c[0] - b.x * sn[0], a.y * c[1] - b.y * sn[1], a.z * c[2] - b.z * sn[2],
+                                     a.w * c[3] - b.w * sn[3]);
+                    yb = make_float4(a.x * sn[0] + b.x * c[0], a.y * sn[1] + b.y * c[1], a.z * sn[2] + b.z * c[2],
+                                     a.w * sn[3] + b.w * c[3]);
+                } else {
+                    ya = make_float4(a.x * c[0] - a.y * sn[0], a.x * sn[0] + a.y * c[0], a.z * c[1] - a.w * sn[1],
+                                     a.z * sn[1] + a.w * c[1]);
+                    yb = make_float4(b.x * c[2] - b.y * sn[2], b.x * sn[2] + b.y * c[2], b.z * c[3] - b.w * sn[3],
+                                     b.z * sn[3] + b.w * c[3]);
+                }
+            }
+            if (rw < p.nqh) {
+                float *d = p.q_out + ((uint64_t)tok * p.nqh + rw) * hd;
+                *reinterpret_cast<float4 *>(d + da) = ya;
+                *reinterpret_cast<float4 *>(d + db) = yb;
+            } else {
+                const uint32_t h = rw - p.nqh;
+                uint16_t *d = (h < p.nkh ? p.kc + at0 + h * p.head_step : p.vc + at0 + (h - p.nkh) * p.head_step);
+                const uint4 w = pack_kv(ya, yb);
+                if (halves) {   // the two quarters of the unit are apart
+                    *reinterpret_cast<uint2 *>(d + da) = make_uint2(w.x, w.y);
+                    *reinterpret_cast<uint2 *>(d + db) = make_uint2(w.z, w.w);
+                } else {
+                    *reinterpret_cast<uint4 *>(d + da) = w;
+                }
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Choice of the slots to keep: exact selection of the r-th highest of m scores
+// per list, ties to the lowest index, result ascending.
+// Scores become 32-bit keys in the scores' order and stay in shared memory,
+// so global memory is read once. The r-th highest key is found by narrowing
+// its range: a histogram of SEL_BINS equal bins over [min, max] of the keys,
+// then over the bin that holds it, at most three times (11 bits each). The
+// output place of a kept slot is the count of kept slots before it (ballots
+// and one scan). A cluster of 1, 2, 4 or 8 CTAs shares a list: each holds a
+// part of it, histograms are read from the other CTAs' shared memory.
+// ---------------------------------------------------------------------------
+constexpr uint32_t SEL_THREADS = 512, SEL_WARPS = SEL_THREADS / 32, SEL_BINS = 2048, SEL_CHUNK_MAX = 49152;
+constexpr uint32_t SEL_N_MAX = 8 * SEL_CHUNK_MAX;
+constexpr uint32_t SEL_HDR = 256;   // bytes of small shared state
+
+struct SelectParams {
+    const float *scores;
+    uint64_t stride;
+    uint32_t n_seqs, n_kv_heads, n_limit, keep, first, recent, chunk_max;
+    const int32_t *n;
+    int32_t *idx, *count;
+    uint32_t *err;
+};
+
+__device__ __forceinline__ uint32_t score_key(float f) {
+    const uint32_t u = __float_as_uint(f);
+    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return 0u;            // NaN: below everything
+    if ((u & 0x7FFFFFFFu) == 0u) return 0x80000000u;           // -0 is 0
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+// Exclusive scan of v over the block; total in *sum. sh: SEL_WARPS words.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *sh, uint32_t *sum) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= (uint32_t)o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) sh[warp] = x;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < SEL_WARPS; ++w) {
+        const uint32_t t = sh[w];
+        if (w < warp) before += t;
+        all += t;
+    }
+    *sum = all;
+    return before + x - v;
+}
+
+__global__ void __launch_bounds__(SEL_THREADS) cache_select_kernel(const SelectParams p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t C = cluster.num_blocks(), rank = cluster.block_rank();
+    const uint32_t list = blockIdx.x / C, s = list / p.n_kv_heads % p.n_seqs;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint32_t *hdr = reinterpret_cast<uint32_t *>(smem);        // [0,16) scan, 16 min, 17 max, 18 bin, 19 above, 20 gt, 21 ties
+    uint32_t *hist = reinterpret_cast<uint32_t *>(smem + SEL_HDR);
+    uint32_t *keys = hist + 2 * SEL_BINS;
+    uint32_t *cnt = keys + p.chunk_max;                        // [rows of 512][warps], kept for certain; then the ties
+    const uint32_t rows_max = p.chunk_max / SEL_THREADS;
+    uint32_t *cnt_tie = cnt + rows_max * SEL_WARPS;
+
+    const int32_t n_in = p.n[s];
+    int32_t *out = p.idx + (uint64_t)list * p.keep;
+    if (n_in < 0 || (uint32_t)n_in > p.n_limit) {              // the whole cluster takes the same way
+        if (tid == 0 && rank == 0) dev_flag_error(p.err, DERR_BAD_ARG);
+        return;
+    }
+    const uint32_t n = (uint32_t)n_in;
+    if (list % p.n_kv_heads == 0 && list / p.n_kv_heads < p.n_seqs && rank == 0 && tid == 0)
+        p.count[s] = (int32_t)min(n, p.keep);
+    if (n <= p.keep) {
+        for (uint32_t i = rank * SEL_THREADS + tid; i < p.keep; i += C * SEL_THREADS) out[i] = i < n ? (int32_t)i : -1;
+        return;
+    }
+    // n > keep >= first + recent: the scores between compete
+    const uint32_t m0 = p.first, m1 = n - p.recent;
+    uint32_t r = p.keep - p.first - p.recent;                  // of them stay (0: none)
+    const uint32_t chunk = ((n + C - 1) / C + SEL_THREADS - 1) / SEL_THREADS * SEL_THREADS;
+    const uint32_t c0 = min(n, rank * chunk), c1 = min(n, c0 + chunk), len = c1 - c0;
+    const float *src = p.scores + (uint64_t)list * p.stride + c0;
+
+    uint32_t kmin = 0xFFFFFFFFu, kmax = 0u;
+    for (uint32_t i = tid; i < len; i += SEL_THREADS) {
+        const uint32_t k = score_key(src[i]);
+        keys[i] = k;
+        if (c0 + i >= m0 && c0 + i < m1) { kmin = min(kmin, k); kmax = max(kmax, k); }
+    }
+    if (tid == 0) { hdr[16] = 0xFFFFFFFFu; hdr[17] = 0u; }
+    for (uint32_t i = tid; i < 2 * SEL_BINS; i += SEL_THREADS) hist[i] = 0u;
+    __syncthreads();
+    kmin = __reduce_min_sync(0xffffffffu, kmin);
+    kmax = __reduce_max_sync(0xffffffffu, kmax);
+    if (lane == 0) { atomicMin(&hdr[16], kmin); atomicMax(&hdr[17], kmax); }
+    cluster.sync();
+    for (uint32_t c = 0; c < C; ++c) {
+        const uint32_t *h = cluster.map_shared_rank(hdr, c);
+        kmin = min(kmin, h[16]);
+        kmax = max(kmax, h[17]);
+    }
+    // narrow [lo, lo + 2^bits) to one key
+    uint32_t lo = kmin, T = 0xFFFFFFFFu, need = 0;
+    if (r) {
+        uint32_t bits = kmax > kmin ? 32 - __clz(kmax - kmin) : 0;
+        for (uint32_t pass = 0;; ++pass) {
+            const uint32_t shift = bits > 11 ? bits - 11 : 0;
+            uint32_t *h = hist + (pass & 1) * SEL_BINS;
+            for (uint32_t i0 = 0; i0 < len; i0 += SEL_THREADS) {   // whole warps: the ballot needs all lanes
+                const uint32_t i = i0 + tid, at = c0 + i;
+                uint32_t bin = 0xFFFFFFFFu;
+                if (i < len && at >= m0 && at < m1) {
+                    const uint32_t d = keys[i] - lo;
+                    if (keys[i] >= lo && (bits == 32 || (d >> bits) == 0)) bin = d >> shift;
+                }
+                // the lowest bin is where equal scores gather: one add per warp
+                const uint32_t low = __ballot_sync(0xffffffffu, bin == 0);
+                if (bin == 0) {
+                    if (lane == (uint32_t)__ffs(low) - 1) atomicAdd(&h[0], (uint32_t)__popc(low));
+                } else if (bin < SEL_BINS) {
+                    atomicAdd(&h[bin], 1u);
+                }
+            }
+            cluster.sync();
+            uint32_t own[4], sum4 = 0;   // bins from the highest down, 4 per thread
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t b = SEL_BINS - 1 - (4 * tid + j);
+                own[j] = 0;
+                for (uint32_t c = 0; c < C; ++c) own[j] += cluster.map_shared_rank(h, c)[b];
+                sum4 += own[j];
+            }
+            uint32_t all;
+            uint32_t above = block_scan(sum4, hdr, &all);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (above < r && r <= above + own[j]) { hdr[18] = SEL_BINS - 1 - (4 * tid + j); hdr[19] = above; }
+                above += own[j];
+            }
+            // every CTA of the cluster has read the other buffer by now
+            for (uint32_t i = tid; i < SEL_BINS; i += SEL_THREADS) hist[((pass + 1) & 1) * SEL_BINS + i] = 0u;
+            __syncthreads();
+            lo += hdr[18] << shift;
+            r -= hdr[19];
+            bits = shift;
+            if (!shift) break;
+        }
+        T = lo;
+        need = r;
+    }
+    // counts per row of 512 and warp: above T (or always kept), and equal to T
+    const uint32_t rows = (len + SEL_THREADS - 1) / SEL_THREADS, ents = rows * SEL_WARPS;
+    auto kind = [&](uint32_t i) -> int {   // 0 dropped, 1 kept, 2 tied
+        if (i >= len) return 0;
+        const uint32_t at = c0 + i;
+        if (at < m0 || at >= m1) return 1;
+        if (!need) return 0;
+        return keys[i] > T ? 1 : (keys[i] == T ? 2 : 0);
+    };
+    for (uint32_t k = 0; k < rows; ++k) {
+        const int kd = kind(k * SEL_THREADS + tid);
+        const uint32_t b1 = __ballot_sync(0xffffffffu, kd == 1), b2 = __ballot_sync(0xffffffffu, kd == 2);
+        if (lane == 0) { cnt[k * SEL_WARPS + warp] = __popc(b1); cnt_tie[k * SEL_WARPS + warp] = __popc(b2); }
+    }
+    __syncthreads();
+    const uint32_t per = (ents + SEL_THREADS - 1) / SEL_THREADS;   // consecutive entries per thread, at most 3
+    uint32_t s1 = 0, s2 = 0;
+    for (uint32_t j = 0; j < per; ++j) {
+        const uint32_t e = tid * per + j;
+        if (e < ents) { s1 += cnt[e]; s2 += cnt_tie[e]; }
+    }
+    uint32_t all1, all2;
+    uint32_t b1 = block_scan(s1, hdr, &all1), b2 = block_scan(s2, hdr, &all2);
+    for (uint32_t j = 0; j < per; ++j) {
+        const uint32_t e = tid * per + j;
+        if (e < ents) {
+            const uint32_t x1 = cnt[e], x2 = cnt_tie[e];
+            cnt[e] = b1;
+            cnt_tie[e] = b2;
+            b1 += x1;
+            b2 += x2;
+        }
+    }
+    if (tid == 0) { hdr[20] = all1; hdr[21] = all2; }
+    cluster.sync();
+    uint32_t o1 = 0, o2 = 0;
+    for (uint32_t c = 0; c < rank; ++c) {
+        const uint32_t *h = cluster.map_shared_rank(hdr, c);
+        o1 += h[20];
+        o2 += h[21];
+    }
+    const uint32_t below = (1u << lane) - 1;
+    for (uint32_t k = 0; k < rows; ++k) {
+        const uint32_t i = k * SEL_THREADS + tid;
+        const int kd = kind(i);
+        const uint32_t g1 = __ballot_sync(0xffffffffu, kd == 1), g2 = __ballot_sync(0xffffffffu, kd == 2);
+        const uint32_t r1 = o1 + cnt[k * SEL_WARPS + warp] + __popc(g1 & below);
+        const uint32_t r2 = o2 + cnt_tie[k * SEL_WARPS + warp] + __popc(g2 & below);
+        if (kd == 1 || (kd == 2 && r2 < need)) out[r1 + min(r2, need)] = (int32_t)(c0 + i);   // n > keep: all places get filled
+    }
+    cluster.sync();   // nobody leaves while its shared memory is read
+}
+
+// ---------------------------------------------------------------------------
+// Row moves. Bound by memory: every row is read once and written once.
+// Apart: a thread moves 16-byte pieces of K and V of GA_U rows, all loads
+// before the first store. In place: rows only move down, so a CTA takes its
+// list in ascending batches (all of a batch's loads, a barrier, its stores);
+// the pieces of a row are independent of one another, so slices of the row
+// go to CTAs of their own.
+// ---------------------------------------------------------------------------
+constexpr uint32_t GA_THREADS = 256, GA_U = 4;
+
+struct GatherSide {
+    uint16_t *k, *v;
+    uint64_t seq_stride, layer_step, pos_step, head_step;
+    uint32_t max_ctx;
+};
+struct GatherParams {
+    GatherSide src, dst;
+    vbs_cu_gather_t g;
+    uint32_t n_seqs, n_kv_heads, cpr;   // 16-byte pieces per row
+    uint32_t slice;                     // in place: pieces per CTA
+    uint32_t *err;
+};
+
+struct GatherList {
+    const int32_t *idx;
+    uint32_t n;
+    int64_t src0, dst0;
+    uint64_t so, dof;        // element offsets of (sequence, layer, head) in the caches
+    uint64_t aux_s, aux_d;   // of the list's row in the weights and positions
+};
+
+__device__ __forceinline__ bool gather_list(const GatherParams &p, uint32_t list, GatherList &l) {
+    const uint32_t h = list % p.n_kv_heads, s = list / p.n_kv_heads % p.n_seqs, layer = list / p.n_kv_heads / p.n_seqs;
+    const int32_t n = p.g.count[s];
+    l.src0 = p.g.src_base ? p.g.src_base[s] : 0;
+    l.dst0 = p.g.dst_base ? p.g.dst_base[s] : 0;
+    l.idx = p.g.idx + layer * p.g.layer_stride + s * p.g.seq_stride + h * p.g.head_stride;
+    l.n = n < 0 ? 0u : (uint32_t)n;
+    l.so = s * p.src.seq_stride + layer * p.src.layer_step + h * p.src.head_step;
+    l.dof = s * p.dst.seq_stride + layer * p.dst.layer_step + h * p.dst.head_step;
+    l.aux_s = (uint64_t)list * p.src.max_ctx;
+    l.aux_d = (uint64_t)list * p.dst.max_ctx;
+    if (n < 0 || (uint32_t)n > p.g.n_max || l.dst0 < 0 || l.dst0 + n > (int64_t)p.dst.max_ctx) {
+        if (threadIdx.x == 0) dev_flag_error(p.err, DERR_BAD_ARG);
+        return false;
+    }
+    return true;
+}
+
+__global__ void __launch_bounds__(GA_THREADS) gather_apart_kernel(const __grid_constant__ GatherParams p, uint32_t nblk) {
+    const uint32_t list = blockIdx.x / nblk, rp = GA_THREADS / p.cpr;
+    GatherList l;
+    if (!gather_list(p, list, l)) return;
+    const uint32_t ch = threadIdx.x % p.cpr, r0 = blockIdx.x % nblk * (rp * GA_U) + threadIdx.x / p.cpr;
+    if (threadIdx.x >= rp * p.cpr) return;
+    int64_t from[GA_U];
+    uint4 k[GA_U], v[GA_U];
+#pragma unroll
+    for (uint32_t u = 0; u < GA_U; ++u) {
+        const uint32_t i = r0 + u * rp;
+        from[u] = i < l.n ? l.src0 + l.idx[i] : -1;
+        if (i < l.n && (from[u] < 0 || from[u] >= (int64_t)p.src.max_ctx)) {
+            dev_flag_error(p.err, DERR_BAD_ARG);
+            from[u] = -1;
+        }
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < GA_U; ++u) {
+        if (from[u] < 0) continue;
+        const uint64_t o = l.so + (uint64_t)from[u] * p.src.pos_step + ch * 8;
+        k[u] = *reinterpret_cast<const uint4 *>(p.src.k + o);
+        v[u] = *reinterpret_cast<const uint4 *>(p.src.v + o);
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < GA_U; ++u) {
+        if (from[u] < 0) continue;
+        const uint64_t to = (uint64_t)l.dst0 + r0 + u * rp;
+        const uint64_t o = l.dof + to * p.dst.pos_step + ch * 8;
+        *reinterpret_cast<uint4 *>(p.dst.k + o) = k[u];
+        *reinterpret_cast<uint4 *>(p.dst.v + o) = v[u];
+        if (ch == 0) {
+            if (p.g.weights_dst) p.g.weights_dst[l.aux_d + to] = p.g.weights_src[l.aux_s + from[u]];
+            if (p.g.pos_dst) p.g.pos_dst[l.aux_d + to] = p.g.pos_src[l.aux_s + from[u]];
+        }
+    }
+}
+
+__global__ void __launch_bounds__(GA_THREADS) gather_inplace_kernel(const __grid_constant__ GatherParams p) {
+    GatherList l;
+    if (!gather_list(p, blockIdx.x, l)) return;
+    // the list first: ascending, and nothing moves up
+    int bad = 0;
+    for (uint32_t i = threadIdx.x; i < l.n; i += GA_THREADS) {
+        const int64_t f = l.src0 + l.idx[i];
+        bad |= f < l.dst0 + i || f >= (int64_t)p.src.max_ctx || (i && l.idx[i] <= l.idx[i - 1]);
+    }
+    if (__syncthreads_or(bad)) {
+        if (threadIdx.x == 0) dev_flag_error(p.err, DERR_BAD_ARG);
+        return;
+    }
+    const uint32_t s0 = blockIdx.y * p.slice, w = min(p.slice, p.cpr - s0);   // this CTA's pieces of a row
+    const uint32_t rp = GA_THREADS / w, ch = s0 + threadIdx.x % w, rr = threadIdx.x / w;
+    const bool on = threadIdx.x < rp * w;
+    for (uint32_t b = 0; b < l.n; b += rp * GA_U) {
+        int64_t from[GA_U];
+        uint4 k[GA_U], v[GA_U];
+        float wt[GA_U];
+        int32_t ps[GA_U];
+#pragma unroll
+        for (uint32_t u = 0; u < GA_U; ++u) {
+            const uint32_t i = b + rr + u * rp;
+            from[u] = on && i < l.n ? l.src0 + l.idx[i] : -1;
+            if (from[u] == l.dst0 + i) from[u] = -1;   // stays where it is
+            if (from[u] < 0) continue;
+            const uint64_t o = l.so + (uint64_t)from[u] * p.src.pos_step + ch * 8;
+            k[u] = *reinterpret_cast<const uint4 *>(p.src.k + o);
+            v[u] = *reinterpret_cast<const uint4 *>(p.src.v + o);
+            if (ch == 0) {
+                if (p.g.weights_dst) wt[u] = p.g.weights_src[l.aux_s + from[u]];
+                if (p.g.pos_dst) ps[u] = p.g.pos_src[l.aux_s + from[u]];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t u = 0; u < GA_U; ++u) {
+            if (from[u] < 0) continue;
+            const uint64_t to = (uint64_t)l.dst0 + b + rr + u * rp;
+            const uint64_t o = l.dof + to * p.dst.pos_step + ch * 8;
+            *reinterpret_cast<uint4 *>(p.dst.k + o) = k[u];
+            *reinterpret_cast<uint4 *>(p.dst.v + o) = v[u];
+            if (ch == 0) {
+                if (p.g.weights_dst) p.g.weights_dst[l.aux_d + to] = wt[u];
+                if (p.g.pos_dst) p.g.pos_dst[l.aux_d + to] = ps[u];
+            }
+        }
+        // no barrier: the next batch reads rows behind all that this one
+        // writes, and writes only behind its own barrier
+    }
+}
+
+cudaError_t slots_configure() {
+    return cudaFuncSetAttribute(cache_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)(SEL_HDR + (2 * SEL_BINS + SEL_CHUNK_MAX + 2 * (SEL_CHUNK_MAX / 32)) * 4));
+}
+
+static GatherSide gather_side(const vbs_cu_kv_t *kv) {
+    GatherSide s = {};
+    s.k = kv->k;
+    s.v = kv->v;
+    s.seq_stride = kv->seq_stride;
+    s.layer_step = (uint64_t)kv->max_ctx * kv->n_kv_heads * kv->head_dim;
+    s.pos_step = kv->head_major ? kv->head_dim : (uint64_t)kv->n_kv_heads * kv->head_dim;
+    s.head_step = kv->head_major ? (uint64_t)kv->max_ctx * kv->head_dim : kv->head_dim;
+    s.max_ctx = kv->max_ctx;
+    return s;
+}
+
+// Elements from the first of a cache to behind its last.
+static uint64_t kv_extent(const vbs_cu_kv_t *kv) {
+    return (uint64_t)(kv->n_seqs - 1) * kv->seq_stride +
+           (uint64_t)kv->n_layers * kv->max_ctx * kv->n_kv_heads * kv->head_dim;
+}
+
+static bool overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && x < y + nb && y < x + na;
+}
+
+}  // namespace vbs
+
+using namespace vbs;
+
+extern "C" {
+
+int vbs_cu_rope_init(vbs_cu_rope_t *r, uint32_t head_dim, uint32_t rot_dim, uint32_t halves, float theta,
+                     const float *freq_factors, uint32_t n_axes, const uint32_t *sections, uint32_t interleaved) {
+    if (!r || !head_dim || head_dim % 8 || head_dim > 256 || !rot_dim || rot_dim % 8 || rot_dim > head_dim ||
+        !(theta > 0.f) || !std::isfinite(theta) || n_axes < 1 || n_axes > 4 || (n_axes > 1 && !sections)) {
+        latch_error("vbs_cu_rope_init: invalid arguments");
+        return -1;
+    }
+    const uint32_t pairs = rot_dim / 2;
+    uint64_t sum = 0;
+    for (uint32_t a = 0; sections && a < n_axes; ++a) sum += sections[a];
+    if (sections && sum != pairs) {
+        latch_error("vbs_cu_rope_init: sections of %llu pairs for %u", (unsigned long long)sum, pairs);
+        return -1;
+    }
+    vbs_cu_rope_t o = {};
+    o.head_dim = head_dim;
+    o.rot_dim = rot_dim;
+    o.n_axes = n_axes;
+    o.halves = halves ? 1u : 0u;
+    uint32_t a = 0, left = sections ? sections[0] : pairs;
+    for (uint32_t p = 0; p < pairs; ++p) {
+        double f = std::pow((double)theta, -2.0 * (double)p / (double)rot_dim);
+        if (freq_factors) f /= (double)freq_factors[p];
+        // circles per position in 2^-64: the fraction alone matters, and a
+        // double below 1 scales to an exact integer part
+        double c = f / (2.0 * M_PI);
+        if (!std::isfinite(c)) {
+            latch_error("vbs_cu_rope_init: frequency factor %u is not usable", p);
+            return -1;
+        }
+        c -= std::floor(c);
+        const double hi = std::floor(c * 4294967296.0);
+        const double lo = (c * 4294967296.0 - hi) * 4294967296.0;
+        o.turn[p] = ((uint64_t)hi << 32) + (uint64_t)lo;
+        if (interleaved && sections) {
+            const uint32_t ax = p % n_axes;
+            o.axis[p] = (uint8_t)((uint64_t)p < (uint64_t)n_axes * sections[ax] ? ax : 0u);
+        } else {
+            while (!left) left = sections[++a];   // the sections' sum is the pairs: a stays below n_axes
+            o.axis[p] = (uint8_t)a;
+            --left;
+        }
+    }
+    *r = o;
+    return 0;
+}
+
+int vbs_cu_rope_store(const vbs_cu_rope_t *r, const vbs_cu_kv_t *kv, uint32_t layer, const float *q, uint64_t q_stride,
+                      float *q_out, uint32_t n_q_heads, const float *k, const float *v, uint64_t kv_stride,
+                      uint32_t n_tokens, const int32_t *pos, const int32_t *seq, const int32_t *slot, void *stream) {
+    const bool turn = n_q_heads != 0, store = k || v;
+    bool ok = r && r->head_dim && r->head_dim % 8 == 0 && r->head_dim <= 256 && r->rot_dim && r->rot_dim % 8 == 0 &&
+              r->rot_dim <= r->head_dim && r->n_axes >= 1 && r->n_axes <= 4 && pos && (turn || store);
+    for (uint32_t p = 0; ok && p < r->rot_dim / 2; ++p) ok = r->axis[p] < r->n_axes;
+    if (ok && turn) {
+        const uint64_t row = (uint64_t)n_q_heads * r->head_dim;
+        if (!q_stride) q_stride = row;
+        ok = q && q_out && n_q_heads <= 65535u && q_stride >= row && q_stride % 4 == 0 && (q != q_out || q_stride == row) &&
+             !((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(q_out)) & 15);
+    }
+    if (ok && store) {
+        ok = k && v && slot && kv_desc_ok(kv) && layer < kv->n_layers && kv->head_dim == r->head_dim;
+        if (ok) {
+            const uint64_t row = (uint64_t)kv->n_kv_heads * kv->head_dim;
+            if (!kv_stride) kv_stride = row;
+            ok = kv_stride >= row && kv_stride % 4 == 0 &&
+                 !((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15);
+        }
+    }
+    if (!ok) {
+        latch_error("vbs_cu_rope_store: invalid arguments");
+        return -1;
+    }
+    DevState *d = backend_current();
+    if (!d) { latch_error("vbs_cu_rope_store: no usable device"); return -1; }
+    if (!n_tokens) return 0;
+    RopeParams p = {};
+    p.r = *r;
+    p.q = q; p.q_out = q_out; p.q_stride = q_stride; p.nqh = n_q_heads;
+    p.pos = pos; p.err = d->err;
+    if (store) {
+        const GatherSide c = gather_side(kv);
+        p.k = k; p.v = v; p.kv_stride = kv_stride; p.nkh = kv->n_kv_heads;
+        p.kc = c.k + layer * c.layer_step; p.vc = c.v + layer * c.layer_step;
+        p.seq_stride = c.seq_stride; p.pos_step = c.pos_step; p.head_step = c.head_step;
+        p.max_ctx = kv->max_ctx; p.n_seqs = kv->n_seqs; p.seq = seq; p.slot = slot;
+    }
+    // few tokens: a token's heads over several CTAs, until the SMs are covered
+    const uint32_t rows = p.nqh + 2 * p.nkh, blk = ROPE_THREADS / (r->head_dim / 8);
+    const uint32_t most = (rows + blk - 1) / blk, want = ((uint32_t)d->n_sm * 2 + n_tokens - 1) / n_tokens;
+    const dim3 grid(n_tokens, std::max(1u, std::min(most, want)));
+    note_launches(1);
+    rope_store_kernel<<<grid, ROPE_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    return cuda_ok(cudaGetLastError(), "rope_store") ? 0 : -1;
+}
+
+int vbs_cu_cache_select(const float *scores, uint64_t stride, uint32_t n_layers, uint32_t n_seqs, uint32_t n_kv_heads,
+                        const int32_t *n, uint32_t n_limit, uint32_t keep, uint32_t first, uint32_t recent, int32_t *idx,
+                        int32_t *count, void *stream) {
+    const uint64_t lists = (uint64_t)n_layers * n_seqs * n_kv_heads;
+    if (!scores || !n || !idx || !count || !n_layers || !n_seqs || !n_kv_heads || n_layers > 65535u || n_seqs > 65535u ||
+        n_kv_heads > 65535u || lists > (1u << 27) || !keep || keep > 0x7FFFFFFFu || (uint64_t)first + recent > keep ||
+        n_limit > stride || n_limit > SEL_N_MAX) {
+        latch_error("vbs_cu_cache_select: invalid arguments");
+        return -1;
+    }
+    DevState *d = backend_current();
+    if (!d) { latch_error("vbs_cu_cache_select: no usable device"); return -1; }
+    // CTAs per list: as many as the SMs have room for, 2048 scores each at
+    // least; more where a list does not fit one CTA's shared memory
+    uint32_t c = 1;
+    while (c < 8 && (n_limit > c * SEL_CHUNK_MAX || (lists * c * 2 <= (uint64_t)d->n_sm && n_limit > c * 2048u))) c *= 2;
+    SelectParams p = {};
+    p.scores = scores; p.stride = stride; p.n_seqs = n_seqs; p.n_kv_heads = n_kv_heads; p.n_limit = n_limit;
+    p.keep = keep; p.first = first; p.recent = recent; p.n = n; p.idx = idx; p.count = count; p.err = d->err;
+    p.chunk_max = std::max(1u, ((n_limit + c - 1) / c + SEL_THREADS - 1) / SEL_THREADS) * SEL_THREADS;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(lists * c));
+    cfg.blockDim = dim3(SEL_THREADS);
+    cfg.dynamicSmemBytes = SEL_HDR + (2 * SEL_BINS + p.chunk_max + 2 * (p.chunk_max / 32)) * 4;
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = c;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    note_launches(1);
+    return cuda_ok(cudaLaunchKernelEx(&cfg, cache_select_kernel, p), "cache_select") ? 0 : -1;
+}
+
+int vbs_cu_cache_gather(const vbs_cu_kv_t *src, const vbs_cu_kv_t *dst, const vbs_cu_gather_t *g, void *stream) {
+    bool ok = kv_desc_ok(src) && kv_desc_ok(dst) && g && g->idx && g->count && g->n_max && src->n_layers == dst->n_layers &&
+              src->n_seqs == dst->n_seqs && src->n_kv_heads == dst->n_kv_heads && src->head_dim == dst->head_dim &&
+              !g->weights_src == !g->weights_dst && !g->pos_src == !g->pos_dst && g->n_max <= 0x7FFFFFFFu;
+    const uint64_t lists = ok ? (uint64_t)src->n_layers * src->n_seqs * src->n_kv_heads : 0;
+    bool same = false;
+    if (ok) {
+        const uint64_t es = kv_extent(src) * 2, ed = kv_extent(dst) * 2;
+        const uint64_t as = lists * src->max_ctx * 4, ad = lists * dst->max_ctx * 4;
+        same = src->k == dst->k;
+        if (same)
+            ok = src->v == dst->v && src->max_ctx == dst->max_ctx && !src->head_major == !dst->head_major &&
+                 src->seq_stride == dst->seq_stride && g->weights_src == g->weights_dst && g->pos_src == g->pos_dst;
+        else
+            ok = !overlap(src->k, es, dst->k, ed) && !overlap(src->v, es, dst->v, ed) && !overlap(src->k, es, dst->v, ed) &&
+                 !overlap(src->v, es, dst->k, ed) && !overlap(g->weights_src, as, g->weights_dst, ad) &&
+                 !overlap(g->pos_src, as, g->pos_dst, ad);
+        ok = ok && lists <= (1u << 24);
+    }
+    if (!ok) {
+        latch_error("vbs_cu_cache_gather: invalid arguments");
+        return -1;
+    }
+    DevState *d = backend_current();
+    if (!d) { latch_error("vbs_cu_cache_gather: no usable device"); return -1; }
+    GatherParams p = {};
+    p.src = gather_side(src);
+    p.dst = gather_side(dst);
+    p.g = *g;
+    p.n_seqs = src->n_seqs;
+    p.n_kv_heads = src->n_kv_heads;
+    p.cpr = src->head_dim / 8;
+    p.err = d->err;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    note_launches(1);
+    if (same) {
+        // slices of at least 64 bytes, as many as cover the SMs four times
+        const uint32_t want = (uint32_t)std::min<uint64_t>(8, ((uint64_t)d->n_sm * 4 + lists - 1) / lists);
+        p.slice = std::max(std::min(4u, p.cpr), (p.cpr + want - 1) / want);
+        gather_inplace_kernel<<<dim3((unsigned)lists, (p.cpr + p.slice - 1) / p.slice), GA_THREADS, 0, st>>>(p);
+    } else {
+        const uint32_t rows = GA_THREADS / p.cpr * GA_U;
+        const uint64_t nblk = (std::min(g->n_max, dst->max_ctx) + rows - 1) / rows;
+        if (lists * nblk > 0x7FFFFFFFull) {
+            latch_error("vbs_cu_cache_gather: %llu lists of %u rows are too many for one call", (unsigned long long)lists,
+                        g->n_max);
+            return -1;
+        }
+        gather_apart_kernel<<<(unsigned)(lists * nblk), GA_THREADS, 0, st>>>(p, (uint32_t)nblk);
+    }
+    return cuda_ok(cudaGetLastError(), "cache_gather") ? 0 : -1;
+}
+
+}  // extern "C"

@@ -1,0 +1,739 @@
+// tree.cu -- attention of new tokens (a tree or chain of drafts, a chunk, one
+// token) over a cache whose slots are not positions.
+//
+//   x_rt = scale q_r . K_t;  capped: c tanh(x / c);  + slope_r (kpos_t - qpos_r)
+//   out_r = sum_t p_rt V_t,  p_rt = softmax over the visible t
+//   weights: W_t += sum over the rows of a KV head of p_rt
+//
+// Rows: the n_tok tokens x G query heads of one KV head, row r = token * G +
+// head, so a row tile's queries are read in runs. Every key of the context is
+// seen by every row, drafted key j by the rows whose mask has bit j.
+//
+// Work split: CTA = (KV head, row tile, part of the positions, sequence); the
+// parts' (m, l, o) go to the caller's workspace and tree_merge_kernel joins
+// them. One part writes the result itself.
+//
+// tree_mma_kernel: as the decode attention in attn.cu, 16 positions of K and V
+// per warp at a time through padded shared memory (cp.async, TREE_NST stages),
+// mma.sync m16n8k16 with fp32 accumulators, online softmax with a lazy
+// rescale. fp32 queries and weights are two fp16 halves each (x = hi + lo to
+// 2^-22); both halves run on the same B fragments into the same accumulators,
+// 16 rows per warp.
+//  * Queries are scaled per row by a power of two to 2^8..2^9, so neither half
+//    leaves fp16's range; the power goes into the score's factor (exact).
+//  * The softmax reference stays 6 below the running maximum (log2 units), so
+//    weights are 2^6 at the first and at most 2^14 before a rescale: small
+//    weights keep their low half above fp16's smallest numbers.
+//  * A block where some row does not see some key takes the masked path, which
+//    also looks for infinities and NaN among its values: 0 * inf would carry
+//    them into rows that do not see them, so such a block adds its values
+//    one visible key at a time.
+#include "vbs_b200.h"
+#include "backend.h"
+#include "common.cuh"
+#include "kernels.h"
+
+#include <algorithm>
+
+namespace vbs {
+
+bool kv_desc_ok(const vbs_cu_kv_t *kv);
+
+struct TreeParams {
+    const float *q;
+    float *out;
+    const uint16_t *kc, *vc;      // layer's first element of sequence 0
+    uint64_t seq_stride, pos_step, head_step;
+    uint32_t max_ctx, nkh, nqh, G, hd, n_tokens, words, window, ctx_limit;
+    uint32_t row_tiles, n_splits, per_split;
+    float scale, cap;
+    const float *slopes;
+    const int32_t *n_ctx, *n_tok;
+    const uint32_t *mask;
+    const int32_t *q_pos, *k_pos;
+    uint32_t k_pos_per_head;
+    const float *weights_in;
+    float *weights_out;
+    // workspace
+    float2 *part_ml;              // [slot][split][tile rows]
+    float *part_o;                // [slot][split][tile rows][hd], slot = (seq * nkh + kv head) * row_tiles + tile
+    float *lse;                   // [seq * nkh + kv head][rows], log2 units, with weights
+    float *scores;                // [seq * nkh + kv head][rows][score_ld], log2 units, with weights
+    uint32_t score_ld;
+    uint32_t *err;
+};
+
+constexpr float TREE_LOG2E = 1.4426950408889634f;
+constexpr float TREE_BELOW = 6.0f, TREE_LAZY = 14.0f;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Lengths of sequence b; false (flagged once) when they do not fit the cache
+// or the call's limit: the sequence is left alone.
+__device__ __forceinline__ bool tree_lengths(const TreeParams &p, uint32_t b, uint32_t &nc, uint32_t &nt) {
+    const int32_t c = p.n_ctx[b], t = p.n_tok ? p.n_tok[b] : (int32_t)p.n_tokens;
+    if (c < 0 || t < 0 || (uint32_t)t > p.n_tokens || (uint64_t)c + t > min(p.max_ctx, p.ctx_limit)) {
+        if (threadIdx.x == 0) dev_flag_error(p.err, DERR_BAD_ARG);
+        return false;
+    }
+    nc = (uint32_t)c;
+    nt = (uint32_t)t;
+    return true;
+}
+
+__device__ __forceinline__ int32_t tree_qpos(const TreeParams &p, uint32_t b, uint32_t i, uint32_t nc) {
+    return p.q_pos ? p.q_pos[(uint64_t)b * p.n_tokens + i] : (int32_t)(nc + i);
+}
+
+// First slot that any row can see: with a window over plain slots, behind
+// the lowest query position's window. All threads of the block call it.
+__device__ __forceinline__ uint32_t tree_first(const TreeParams &p, uint32_t b, uint32_t nc, uint32_t nt, int32_t *sh) {
+    if (!p.window || p.k_pos) return 0;
+    int32_t lo = 0x7FFFFFFF;
+    if (p.q_pos) {
+        for (uint32_t i = threadIdx.x; i < nt; i += blockDim.x) lo = min(lo, tree_qpos(p, b, i, nc));
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = lo;
+        __syncthreads();
+        for (uint32_t w = 0; w < blockDim.x / 32; ++w) lo = min(lo, sh[w]);
+        __syncthreads();
+    } else {
+        lo = (int32_t)nc;
+    }
+    const int64_t first = (int64_t)lo - p.window + 1;
+    return first <= 0 ? 0u : (uint32_t)min(first, (int64_t)nc);   // new tokens are always looked at
+}
+
+// This split's positions [t0, t1): equal parts, whole blocks of 64.
+__device__ __forceinline__ void tree_part(const TreeParams &p, uint32_t first, uint32_t end, uint32_t split, uint32_t &t0,
+                                          uint32_t &t1) {
+    const uint32_t span = end - first;
+    uint32_t per = (span + p.n_splits - 1) / p.n_splits;
+    per = max(p.per_split, (per + 63) / 64 * 64);
+    t0 = (uint32_t)min((uint64_t)end, first + (uint64_t)split * per);
+    t1 = min(end, t0 + per);
+}
+
+template <int HD, int WR, int WP> struct TreeCfg {
+    static constexpr int NW = WR * WP, THREADS = NW * 32;
+    static constexpr int ROWS = 16 * WR;
+    static constexpr int SP = HD > 128 ? 32 : 64;      // positions per stage
+    static constexpr int RSB = HD * 2 + 16;            // staged row bytes (padded)
+    static constexpr int KPOS = 2 * SP * RSB;          // offset of the stage's key positions
+    static constexpr int STAGE = KPOS + SP * 4;
+    static constexpr int NST = HD >= 128 ? 3 : 4;
+    static constexpr bool QREG = HD <= 128;            // query halves in registers
+    static constexpr int QSM = QREG ? 0 : ROWS * RSB * 2;
+    static constexpr int OLD = HD + 4;                 // floats per row in the join of the warps
+    static constexpr int JOIN = WP * ROWS * OLD * 4;
+    static constexpr int SMEM = QSM + (NST * STAGE > JOIN ? NST * STAGE : JOIN);
+    static_assert(SP % (16 * WP) == 0, "whole blocks of 16 per warp");
+};
+
+template <int HD, int WR, int WP>
+__global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(const __grid_constant__ TreeParams p) {
+    using C = TreeCfg<HD, WR, WP>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int32_t sh_min[C::NW];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int wr = warp % WR, wp = warp / WR;
+    const uint32_t kvh = blockIdx.x % p.nkh, tile = blockIdx.x / p.nkh, split = blockIdx.y, b = blockIdx.z;
+    const uint32_t G = p.G, R0 = tile * C::ROWS;
+    uint32_t nc, nt;
+    if (!tree_lengths(p, b, nc, nt) || R0 >= nt * G) return;
+    const uint32_t end = nc + nt, nrows = nt * G;
+    const uint32_t first = tree_first(p, b, nc, nt, sh_min);
+    uint32_t t0, t1;
+    tree_part(p, first, end, split, t0, t1);
+    const uint64_t slot = (uint64_t)(b * p.nkh + kvh) * p.row_tiles + tile;
+    float2 *ml = p.part_ml + (slot * p.n_splits + split) * C::ROWS;
+    if (t0 >= t1 && p.n_splits > 1) {   // no positions: an empty part
+        for (int r = threadIdx.x; r < C::ROWS; r += C::THREADS) ml[r] = make_float2(-INFINITY, 0.f);
+        return;
+    }
+    const uint32_t nch = (t1 - t0 + C::SP - 1) / C::SP;
+    const uint16_t *kb = p.kc + (uint64_t)b * p.seq_stride + (uint64_t)kvh * p.head_step;
+    const uint16_t *vb = p.vc + (uint64_t)b * p.seq_stride + (uint64_t)kvh * p.head_step;
+    const int32_t *kpos = p.k_pos ? p.k_pos + (uint64_t)(p.k_pos_per_head ? b * p.nkh + kvh : b) * p.max_ctx : nullptr;
+    const uint32_t sbase = smem_u32(smem) + C::QSM;
+    const uint32_t cpr = p.hd / 8;
+
+    auto issue = [&](uint32_t c) {
+        const uint32_t st = sbase + (c % C::NST) * C::STAGE;
+        const uint32_t pb = t0 + c * C::SP;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < 2 * C::SP * (HD / 8); i += C::THREADS) {
+            const int isv = i / (C::SP * (HD / 8)), r = (i / (HD / 8)) % C::SP;
+            const uint32_t ch = i % (HD / 8);
+            const bool ok = pb + r < t1 && ch < cpr;   // head_dim below HD: zeros
+            const uint16_t *src = (isv ? vb : kb) + (uint64_t)(ok ? pb + r : t0) * p.pos_step + (ok ? ch : 0) * 8;
+            cp_async16(st + (isv * C::SP + r) * C::RSB + ch * 16, src, ok ? 16u : 0u);
+        }
+        if (kpos && threadIdx.x < C::SP) {
+            const uint32_t t = pb + threadIdx.x;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(st + C::KPOS + threadIdx.x * 4),
+                         "l"(kpos + (t < t1 ? t : t0)), "r"(t < t1 ? 4u : 0u) : "memory");
+        }
+    };
+#pragma unroll
+    for (int c = 0; c < C::NST - 1; ++c) {
+        if ((uint32_t)c < nch) issue(c);
+        cp_async_commit();
+    }
+
+    // the two rows of this thread: g and g + 8 of the warp's 16
+    const int g = lane >> 2, qd = 2 * (lane & 3);
+    uint32_t row[2], tok[2];
+    bool on[2];
+    float fac[2], slope[2] = {0.f, 0.f};
+    int32_t qpos[2];
+    const float *qsrc[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        row[h] = R0 + 16 * wr + g + 8 * h;
+        on[h] = row[h] < nrows;
+        const uint32_t rr = on[h] ? row[h] : 0u;
+        tok[h] = rr / G;
+        const uint32_t head = kvh * G + rr % G;
+        qpos[h] = tree_qpos(p, b, tok[h], nc);
+        if (p.slopes) slope[h] = p.slopes[head] * TREE_LOG2E;
+        qsrc[h] = p.q + (((uint64_t)b * p.n_tokens + tok[h]) * p.nqh + head) * p.hd;
+    }
+    // query halves as A fragments, scaled by the row's power of two
+    uint32_t qh[C::QREG ? HD / 16 : 1][4], ql[C::QREG ? HD / 16 : 1][4];
+    {
+        float2 x[2][HD / 8];
+        float top[2] = {0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int n = 0; n < HD / 8; ++n) {
+                const bool ok = on[h] && 8 * n + qd < (int)p.hd;
+                x[h][n] = ok ? *reinterpret_cast<const float2 *>(qsrc[h] + 8 * n + qd) : make_float2(0.f, 0.f);
+                top[h] = fmaxf(top[h], fmaxf(fabsf(x[h][n].x), fabsf(x[h][n].y)));
+            }
+            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+            // 2^e with top in [2^8, 2^9) afterwards; zero, tiny or not finite: no scaling
+            int e = (int)((__float_as_uint(top[h]) >> 23) & 255u) - 127;
+            e = (e < -100 || e > 100) ? 0 : 8 - e;
+            const float up = __uint_as_float((uint32_t)(127 + e) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+            for (int n = 0; n < HD / 8; ++n) { x[h][n].x *= up; x[h][n].y *= up; }
+            fac[h] = p.scale * down;
+        }
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {   // a0, a2: row g; a1, a3: row g + 8; k half j / 2
+                const float2 v = x[j & 1][2 * kk + (j >> 1)];
+                const __half2 hi = __floats2half2_rn(v.x, v.y);
+                const float2 f = __half22float2(hi);
+                const __half2 lo = __floats2half2_rn(v.x - f.x, v.y - f.y);
+                if constexpr (C::QREG) {
+                    qh[kk][j] = *reinterpret_cast<const uint32_t *>(&hi);
+                    ql[kk][j] = *reinterpret_cast<const uint32_t *>(&lo);
+                } else if (wp == 0) {
+                    uint8_t *d = smem + (16 * wr + g + 8 * (j & 1)) * C::RSB + (16 * kk + 8 * (j >> 1) + qd) * 2;
+                    *reinterpret_cast<__half2 *>(d) = hi;
+                    *reinterpret_cast<__half2 *>(d + C::ROWS * C::RSB) = lo;
+                }
+            }
+        }
+    }
+    const float cap2 = p.cap * TREE_LOG2E;
+    const float pre = p.cap > 0.f ? 2.f * TREE_LOG2E / p.cap : TREE_LOG2E;   // capped: exponent of e^(2x / cap)
+    fac[0] *= pre;
+    fac[1] *= pre;
+    // highest query position of the rows, for the window's fast path
+    int32_t qmax = max(qpos[0], qpos[1]);
+    qmax = __reduce_max_sync(0xffffffffu, qmax);
+
+    float o[HD / 8][4];
+#pragma unroll
+    for (int n = 0; n < HD / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+    float mref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float *sc_out[2] = {nullptr, nullptr};
+    if (p.scores) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            sc_out[h] = p.scores + ((uint64_t)(b * p.nkh + kvh) * (p.n_tokens * G) + (on[h] ? row[h] : 0u)) * p.score_ld;
+    }
+
+    for (uint32_t c = 0; c < nch; ++c) {
+        if (c + C::NST - 1 < nch) issue(c + C::NST - 1);
+        cp_async_commit();
+        cp_async_wait<C::NST - 1>();
+        __syncthreads();
+        const uint32_t st = sbase + (c % C::NST) * C::STAGE;
+#pragma unroll 1
+        for (int sb = 16 * wp; sb < C::SP; sb += 16 * WP) {
+            const uint32_t tb = t0 + c * C::SP + sb;
+            if (tb >= t1) break;
+            const uint32_t kst = st + sb * C::RSB, vst = kst + C::SP * C::RSB;
+            float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; kk += 2) {
+                uint32_t ah[2][4], al[2][4];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    if constexpr (C::QREG) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) { ah[u][j] = qh[kk + u][j]; al[u][j] = ql[kk + u][j]; }
+                    } else {
+                        const uint32_t a = smem_u32(smem) + (16 * wr + (lane & 15)) * C::RSB + (16 * (kk + u) + 8 * (lane >> 4)) * 2;
+                        ldsm_x4(a, ah[u][0], ah[u][1], ah[u][2], ah[u][3]);
+                        ldsm_x4(a + C::ROWS * C::RSB, al[u][0], al[u][1], al[u][2], al[u][3]);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    uint32_t b0, b1, b2, b3;
+                    ldsm_x4(kst + (8 * j + (lane & 7)) * C::RSB + (16 * kk + 8 * (lane >> 3)) * 2, b0, b1, b2, b3);
+                    mma_f16_acc(s[j], al[0], b0, b1);
+                    mma_f16_acc(s[j], ah[0], b0, b1);
+                    mma_f16_acc(s[j], al[1], b2, b3);
+                    mma_f16_acc(s[j], ah[1], b2, b3);
+                }
+            }
+            // x[h][e]: row h, keys tb + {qd, qd+1, 8+qd, 9+qd}
+            float x[2][4] = {{s[0][0], s[0][1], s[1][0], s[1][1]}, {s[0][2], s[0][3], s[1][2], s[1][3]}};
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[h][e] *= fac[h];
+                    if (p.cap > 0.f)   // cap tanh(y) = cap (1 - 2 / (e^2y + 1)), in log2 units
+                        x[h][e] = cap2 - __fdividef(2.f * cap2, ex2(fminf(x[h][e], 126.f)) + 1.f);
+                }
+            uint32_t hidden = 0;   // bit 4 h + e: row h does not see key e
+            const bool plain = tb + 16 <= min(nc, t1) && !kpos && (!p.window || (int64_t)qmax - tb < (int64_t)p.window);
+            if (!plain || p.slopes) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t kl = qd + (e & 1) + 8 * (e >> 1), t = tb + kl;
+                    const bool in = t < t1, drafted = in && t >= nc;
+                    int32_t kp = (int32_t)t;
+                    if (kpos) asm volatile("ld.shared.s32 %0, [%1];" : "=r"(kp) : "r"(st + C::KPOS + (sb + kl) * 4));
+                    else if (drafted) kp = tree_qpos(p, b, t - nc, nc);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        bool see = in && kp >= 0;
+                        if (kpos == nullptr) see = in;
+                        if (drafted && on[h])
+                            see = see && (p.mask ? (p.mask[((uint64_t)b * p.n_tokens + tok[h]) * p.words + ((t - nc) >> 5)] >>
+                                                    ((t - nc) & 31)) & 1u
+                                                 : t - nc <= tok[h]);
+                        const int64_t dist = (int64_t)qpos[h] - kp;
+                        if (p.window) see = see && dist < (int64_t)p.window;
+                        if (p.slopes) x[h][e] -= slope[h] * (float)dist;
+                        if (!see) {
+                            x[h][e] = -INFINITY;
+                            hidden |= 1u << (4 * h + e);
+                        }
+                    }
+                }
+            }
+            if (p.scores) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (!on[h]) continue;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t t = tb + qd + (e & 1) + 8 * (e >> 1);
+                        if (t < t1) sc_out[h][t] = x[h][e];
+                    }
+                }
+            }
+            float pe[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float mx = fmaxf(fmaxf(x[h][0], x[h][1]), fmaxf(x[h][2], x[h][3]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                if (mx > mref[h] + TREE_LAZY) {
+                    const float r = ex2(mref[h] - (mx - TREE_BELOW));   // 0 on the first block
+                    mref[h] = mx - TREE_BELOW;
+                    l[h] *= r;
+#pragma unroll
+                    for (int n = 0; n < HD / 8; ++n) { o[n][2 * h] *= r; o[n][2 * h + 1] *= r; }
+                }
+                const float base = mref[h] == -INFINITY ? 0.f : mref[h];   // nothing seen so far: weights 0
+#pragma unroll
+                for (int e = 0; e < 4; ++e) pe[h][e] = ex2(x[h][e] - base);
+                l[h] += (pe[h][0] + pe[h][1]) + (pe[h][2] + pe[h][3]);
+            }
+            bool apart = false;
+            if (__any_sync(0xffffffffu, hidden != 0)) {
+                // some row does not see some key: values must be finite for 0 * v to be 0
+                bool bad = false;
+#pragma unroll 4
+                for (int i = lane; i < 16 * (HD / 8); i += 32) {
+                    const uint4 w = lds_u128(vst + (i / (HD / 8)) * C::RSB + (i % (HD / 8)) * 16);
+                    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        bad |= (ww[k] & 0x7C00u) == 0x7C00u || (ww[k] & 0x7C000000u) == 0x7C000000u;
+                }
+                apart = __any_sync(0xffffffffu, bad);
+            }
+            if (!apart) {
+                uint32_t ph[4], pl[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float u = pe[j & 1][2 * (j >> 1)], w = pe[j & 1][2 * (j >> 1) + 1];
+                    const __half2 hi = __floats2half2_rn(u, w);
+                    const float2 f = __half22float2(hi);
+                    const __half2 lo = __floats2half2_rn(u - f.x, w - f.y);
+                    ph[j] = *reinterpret_cast<const uint32_t *>(&hi);
+                    pl[j] = *reinterpret_cast<const uint32_t *>(&lo);
+                }
+#pragma unroll
+                for (int n = 0; n < HD / 8; n += 2) {
+                    uint32_t b0, b1, b2, b3;
+                    ldsm_x4_trans(vst + ((lane & 7) + 8 * ((lane >> 3) & 1)) * C::RSB + (8 * n + 8 * (lane >> 4)) * 2, b0, b1,
+                                  b2, b3);
+                    mma_f16_acc(o[n], pl, b0, b1);
+                    mma_f16_acc(o[n], ph, b0, b1);
+                    mma_f16_acc(o[n + 1], pl, b2, b3);
+                    mma_f16_acc(o[n + 1], ph, b2, b3);
+                }
+            } else {
+#pragma unroll 1
+                for (int k = 0; k < 16; ++k) {   // key k's weights of rows g, g + 8 sit in lane (k % 8) / 2 of the quad
+                    const int from = (lane & ~3) | ((k & 7) >> 1);
+                    float w[2];
+                    bool see[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float v = 0.f;
+                        uint32_t hid = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {   // all lanes shuffle; the key's element is kept
+                            const float t = __shfl_sync(0xffffffffu, pe[h][e], from);
+                            const uint32_t hb = __shfl_sync(0xffffffffu, (hidden >> (4 * h + e)) & 1u, from);
+                            if (e == 2 * (k >> 3) + (k & 1)) { v = t; hid = hb; }
+                        }
+                        w[h] = v;
+                        see[h] = !hid;
+                    }
+#pragma unroll
+                    for (int n = 0; n < HD / 8; ++n) {
+                        uint32_t vv;
+                        vv = lds_u32(vst + k * C::RSB + (8 * n + qd) * 2);
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&vv));
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            if (see[h]) { o[n][2 * h] = fmaf(w[h], f.x, o[n][2 * h]); o[n][2 * h + 1] = fmaf(w[h], f.y, o[n][2 * h + 1]); }
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+    cp_async_wait<0>();
+
+    // join the warps that shared these rows
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    }
+    __syncthreads();
+    float *sh = reinterpret_cast<float *>(smem + C::QSM);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float *d = sh + (wp * C::ROWS + 16 * wr + g + 8 * h) * C::OLD;
+        if ((lane & 3) == 0) { d[HD] = mref[h]; d[HD + 1] = l[h]; }
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n)
+            *reinterpret_cast<float2 *>(d + 8 * n + qd) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+    }
+    __syncthreads();
+    const uint32_t live = min((uint32_t)C::ROWS, nrows - R0), q4 = p.hd / 4;
+    float *po = p.part_o + (slot * p.n_splits + split) * C::ROWS * p.hd;
+    for (uint32_t i = threadIdx.x; i < live * q4; i += C::THREADS) {
+        const uint32_t r = i / q4, d = i % q4 * 4;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WP; ++w) M = fmaxf(M, sh[(w * C::ROWS + r) * C::OLD + HD]);
+        float L = 0.f;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WP; ++w) {
+            const float *x = sh + (w * C::ROWS + r) * C::OLD;
+            const float f = x[HD] == -INFINITY ? 0.f : ex2(x[HD] - M);
+            const float4 v = *reinterpret_cast<const float4 *>(x + d);
+            L += x[HD + 1] * f;
+            a.x = fmaf(v.x, f, a.x); a.y = fmaf(v.y, f, a.y); a.z = fmaf(v.z, f, a.z); a.w = fmaf(v.w, f, a.w);
+        }
+        if (p.n_splits > 1) {
+            if (d == 0) ml[r] = make_float2(M, L);
+            *reinterpret_cast<float4 *>(po + (uint64_t)r * p.hd + d) = a;
+        } else {
+            const uint32_t rr = R0 + r, head = kvh * G + rr % G;
+            const float il = L == 0.f ? 0.f : 1.f / L;   // nothing visible: zeros
+            if (L == 0.f) a = make_float4(0.f, 0.f, 0.f, 0.f);
+            *reinterpret_cast<float4 *>(p.out + (((uint64_t)b * p.n_tokens + rr / G) * p.nqh + head) * p.hd + d) =
+                make_float4(a.x * il, a.y * il, a.z * il, a.w * il);
+            if (p.lse && d == 0)
+                p.lse[(uint64_t)(b * p.nkh + kvh) * (p.n_tokens * G) + rr] = L == 0.f ? -INFINITY : M + log2f(L);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Join of the parts: one CTA per row, its warps over the parts, then the
+// warps' sums in order. Reads every part once.
+// ---------------------------------------------------------------------------
+constexpr int TREE_MW = 4;
+
+__global__ void __launch_bounds__(TREE_MW * 32) tree_merge_kernel(const __grid_constant__ TreeParams p, uint32_t tile_rows) {
+    __shared__ float sm_m[TREE_MW], sm_l[TREE_MW];
+    __shared__ float sm_o[TREE_MW][256];
+    const uint32_t r = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t nc, nt;
+    if (!tree_lengths(p, b, nc, nt) || r >= nt * p.G) return;
+    const uint32_t tile = r / tile_rows, ri = r % tile_rows;
+    const uint64_t slot = (uint64_t)(b * p.nkh + kvh) * p.row_tiles + tile;
+    const float2 *ml = p.part_ml + slot * p.n_splits * tile_rows + ri;
+    const float *po = p.part_o + (slot * p.n_splits * tile_rows + ri) * p.hd;
+    float M = -INFINITY;
+    for (uint32_t s = threadIdx.x; s < p.n_splits; s += TREE_MW * 32) M = fmaxf(M, ml[(uint64_t)s * tile_rows].x);
+    M = warp_max(M);
+    if (lane == 0) sm_m[warp] = M;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < TREE_MW; ++w) M = fmaxf(M, sm_m[w]);
+    float L = 0.f;
+    float4 a[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+    constexpr int U = 4;
+    for (uint32_t s0 = warp; s0 < p.n_splits; s0 += TREE_MW * U) {
+        float f[U];
+        float4 v[U][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t s = s0 + u * TREE_MW;
+            f[u] = 0.f;
+            float2 x = make_float2(-INFINITY, 0.f);
+            if (s < p.n_splits) x = ml[(uint64_t)s * tile_rows];
+            const bool live = !(x.y == 0.f);   // an empty part has no sums; a NaN goes through
+            if (live) { f[u] = ex2(x.x - M); L += x.y * f[u]; }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t d = (lane + 32 * k) * 4;
+                v[u][k] = live && d < p.hd ? *reinterpret_cast<const float4 *>(po + (uint64_t)s * tile_rows * p.hd + d)
+                                           : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                a[k].x = fmaf(v[u][k].x, f[u], a[k].x); a[k].y = fmaf(v[u][k].y, f[u], a[k].y);
+                a[k].z = fmaf(v[u][k].z, f[u], a[k].z); a[k].w = fmaf(v[u][k].w, f[u], a[k].w);
+            }
+    }
+    if (lane == 0) sm_l[warp] = L;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) *reinterpret_cast<float4 *>(&sm_o[warp][(lane + 32 * k) * 4]) = a[k];
+    __syncthreads();
+    L = 0.f;
+#pragma unroll
+    for (int w = 0; w < TREE_MW; ++w) L += sm_l[w];
+    const float il = L == 0.f ? 0.f : 1.f / L;
+    float *out = p.out + (((uint64_t)b * p.n_tokens + r / p.G) * p.nqh + kvh * p.G + r % p.G) * p.hd;
+    for (uint32_t d = threadIdx.x; d < p.hd; d += TREE_MW * 32) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < TREE_MW; ++w) v += sm_o[w][d];
+        out[d] = L == 0.f ? 0.f : v * il;
+    }
+    if (p.lse && threadIdx.x == 0)
+        p.lse[(uint64_t)(b * p.nkh + kvh) * (p.n_tokens * p.G) + r] = L == 0.f ? -INFINITY : M + log2f(L);
+}
+
+// ---------------------------------------------------------------------------
+// Attention weights per slot: W_t = W_in,t + sum over rows of
+// 2^(score - lse). One thread per slot, rows in order, so the sum does not
+// depend on the split.
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) tree_weights_kernel(const __grid_constant__ TreeParams p) {
+    __shared__ int32_t sh_min[8];
+    const uint32_t kvh = blockIdx.y, b = blockIdx.z;
+    uint32_t nc, nt;
+    if (!tree_lengths(p, b, nc, nt)) return;
+    const uint32_t first = tree_first(p, b, nc, nt, sh_min);
+    const uint32_t t = blockIdx.x * 256 + threadIdx.x;
+    if (t >= nc + nt) return;
+    const uint64_t at = (uint64_t)(b * p.nkh + kvh) * p.max_ctx + t;
+    float w = p.weights_in ? p.weights_in[at] : 0.f;
+    if (t >= first) {
+        const uint64_t base = (uint64_t)(b * p.nkh + kvh) * (p.n_tokens * p.G);
+        const uint32_t n = nt * p.G;
+        float sum = 0.f;
+#pragma unroll 4
+        for (uint32_t r = 0; r < n; ++r) {
+            const float z = p.lse[base + r];
+            const float e = ex2(p.scores[(base + r) * p.score_ld + t] - (z == -INFINITY ? 0.f : z));
+            sum += e;   // a row that sees nothing: every score -inf, weight 0
+        }
+        w += sum;
+    }
+    p.weights_out[at] = w;
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+struct TreePlan {
+    uint32_t rows, tile_rows, row_tiles, n_splits, per_split, score_ld;
+    size_t ml, o, lse, scores, bytes;   // offsets into the workspace, total
+};
+
+// Warps over rows and over positions of a CTA by the rows of a KV head: few
+// rows leave all warps to the positions (nothing is computed twice), more
+// rows share the staged keys.
+static uint32_t tree_warp_rows(uint32_t rows) { return rows <= 16 ? 1 : (rows <= 32 ? 2 : 4); }
+
+static TreePlan tree_plan(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t, int n_sm) {
+    TreePlan pl = {};
+    const uint32_t G = t->n_q_heads / kv->n_kv_heads;
+    pl.rows = t->n_tokens * G;
+    pl.tile_rows = 16 * tree_warp_rows(pl.rows);
+    pl.row_tiles = (pl.rows + pl.tile_rows - 1) / pl.tile_rows;
+    // parts: about two CTAs per SM, at least 64 positions each
+    const uint64_t ctas = (uint64_t)pl.row_tiles * kv->n_kv_heads * kv->n_seqs;
+    uint64_t s = ((uint64_t)n_sm * 2 + ctas - 1) / ctas;
+    s = std::max<uint64_t>(1, std::min<uint64_t>(s, (t->ctx_limit + 63) / 64));
+    pl.per_split = (uint32_t)(((t->ctx_limit + s - 1) / s + 63) / 64 * 64);
+    pl.n_splits = (t->ctx_limit + pl.per_split - 1) / pl.per_split;
+    auto take = [&](size_t n) { const size_t at = pl.bytes; pl.bytes += (n + 255) / 256 * 256; return at; };
+    const size_t heads = (size_t)kv->n_seqs * kv->n_kv_heads;
+    if (pl.n_splits > 1) {
+        pl.ml = take(heads * pl.row_tiles * pl.n_splits * pl.tile_rows * sizeof(float2));
+        pl.o = take(heads * pl.row_tiles * pl.n_splits * pl.tile_rows * kv->head_dim * sizeof(float));
+    }
+    if (t->weights_out) {
+        pl.score_ld = (t->ctx_limit + 3) / 4 * 4;
+        pl.lse = take(heads * pl.rows * sizeof(float));
+        pl.scores = take(heads * pl.rows * pl.score_ld * sizeof(float));
+    }
+    pl.bytes = std::max<size_t>(pl.bytes, 256);
+    return pl;
+}
+
+static bool tree_desc_ok(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t) {
+    if (!kv_desc_ok(kv) || !t || !t->n_q_heads || t->n_q_heads % kv->n_kv_heads || !t->n_tokens || !t->ctx_limit ||
+        t->ctx_limit > kv->max_ctx || !t->n_ctx)
+        return false;
+    if (t->n_tokens > 4096u || t->n_q_heads / kv->n_kv_heads > 256u) return false;
+    if (!(t->scale == t->scale) || !(t->softcap >= 0.f) || t->window > 0x7FFFFFFFu) return false;
+    return !(t->weights_in && !t->weights_out);
+}
+
+template <int HD, int WR, int WP> static cudaError_t tree_go(const TreeParams &p, dim3 grid, cudaStream_t st) {
+    using C = TreeCfg<HD, WR, WP>;
+    tree_mma_kernel<HD, WR, WP><<<grid, C::THREADS, C::SMEM, st>>>(p);
+    return cudaGetLastError();
+}
+template <int HD> static cudaError_t tree_go_rows(const TreeParams &p, uint32_t wr, dim3 grid, cudaStream_t st) {
+    constexpr int W = HD > 128 ? 2 : 4;   // 32 positions per stage: two warps of 16
+    if (wr == 1) return tree_go<HD, 1, W>(p, grid, st);
+    if (wr == 2) return tree_go<HD, 2, W>(p, grid, st);
+    return tree_go<HD, 4, 2>(p, grid, st);
+}
+template <int HD, int WR, int WP> static cudaError_t tree_cfg() {
+    return cudaFuncSetAttribute(tree_mma_kernel<HD, WR, WP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                TreeCfg<HD, WR, WP>::SMEM);
+}
+template <int HD> static cudaError_t tree_cfg_rows() {
+    constexpr int W = HD > 128 ? 2 : 4;
+    cudaError_t e = tree_cfg<HD, 1, W>();
+    if (e == cudaSuccess) e = tree_cfg<HD, 2, W>();
+    if (e == cudaSuccess) e = tree_cfg<HD, 4, 2>();
+    return e;
+}
+
+cudaError_t tree_configure() {
+    cudaError_t e = tree_cfg_rows<64>();
+    if (e == cudaSuccess) e = tree_cfg_rows<128>();
+    if (e == cudaSuccess) e = tree_cfg_rows<256>();
+    return e;
+}
+
+}  // namespace vbs
+
+using namespace vbs;
+
+extern "C" {
+
+size_t vbs_cu_tree_workspace(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t) {
+    if (!tree_desc_ok(kv, t)) {
+        latch_error("vbs_cu_tree_workspace: invalid arguments");
+        return 0;
+    }
+    DevState *d = backend_current();
+    if (!d) { latch_error("vbs_cu_tree_workspace: no usable device"); return 0; }
+    return tree_plan(kv, t, d->n_sm).bytes;
+}
+
+int vbs_cu_attention_tree(const vbs_cu_kv_t *kv, uint32_t layer, const vbs_cu_tree_t *t, const float *q, float *out, void *work,
+                          size_t work_bytes, void *stream) {
+    if (!tree_desc_ok(kv, t) || layer >= kv->n_layers || !q || !out || !work ||
+        ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(work)) & 15)) {
+        latch_error("vbs_cu_attention_tree: invalid arguments");
+        return -1;
+    }
+    DevState *d = backend_current();
+    if (!d) { latch_error("vbs_cu_attention_tree: no usable device"); return -1; }
+    const TreePlan pl = tree_plan(kv, t, d->n_sm);
+    if (work_bytes < pl.bytes) {
+        latch_error("vbs_cu_attention_tree: workspace of %zu bytes, needs %zu", work_bytes, pl.bytes);
+        return -1;
+    }
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    TreeParams p = {};
+    const uint64_t layer_step = (uint64_t)kv->max_ctx * kv->n_kv_heads * kv->head_dim;
+    p.q = q; p.out = out;
+    p.kc = kv->k + layer * layer_step;
+    p.vc = kv->v + layer * layer_step;
+    p.seq_stride = kv->seq_stride;
+    p.pos_step = kv->head_major ? kv->head_dim : (uint64_t)kv->n_kv_heads * kv->head_dim;
+    p.head_step = kv->head_major ? (uint64_t)kv->max_ctx * kv->head_dim : kv->head_dim;
+    p.max_ctx = kv->max_ctx; p.nkh = kv->n_kv_heads; p.nqh = t->n_q_heads; p.G = t->n_q_heads / kv->n_kv_heads;
+    p.hd = kv->head_dim; p.n_tokens = t->n_tokens; p.words = (t->n_tokens + 31) / 32; p.window = t->window;
+    p.ctx_limit = t->ctx_limit; p.row_tiles = pl.row_tiles; p.n_splits = pl.n_splits; p.per_split = pl.per_split;
+    p.scale = t->scale; p.cap = t->softcap; p.slopes = t->slopes; p.n_ctx = t->n_ctx; p.n_tok = t->n_tok;
+    p.mask = t->mask; p.q_pos = t->q_pos; p.k_pos = t->k_pos; p.k_pos_per_head = t->k_pos_per_head;
+    p.weights_in = t->weights_in; p.weights_out = t->weights_out;
+    uint8_t *w = static_cast<uint8_t *>(work);
+    p.part_ml = reinterpret_cast<float2 *>(w + pl.ml);
+    p.part_o = reinterpret_cast<float *>(w + pl.o);
+    if (t->weights_out) {
+        p.lse = reinterpret_cast<float *>(w + pl.lse);
+        p.scores = reinterpret_cast<float *>(w + pl.scores);
+        p.score_ld = pl.score_ld;
+    }
+    p.err = d->err;
+    const dim3 grid(kv->n_kv_heads * pl.row_tiles, pl.n_splits, kv->n_seqs);
+    const uint32_t wr = pl.tile_rows / 16;
+    note_launches(1u + (pl.n_splits > 1) + (t->weights_out != nullptr));
+    cudaError_t e = kv->head_dim <= 64 ? tree_go_rows<64>(p, wr, grid, st)
+                                       : (kv->head_dim <= 128 ? tree_go_rows<128>(p, wr, grid, st) : tree_go_rows<256>(p, wr, grid, st));
+    if (e == cudaSuccess && pl.n_splits > 1) {
+        tree_merge_kernel<<<dim3(pl.rows, kv->n_kv_heads, kv->n_seqs), TREE_MW * 32, 0, st>>>(p, pl.tile_rows);
+        e = cudaGetLastError();
+    }
+    if (e == cudaSuccess && t->weights_out) {
+        tree_weights_kernel<<<dim3((t->ctx_limit + 255) / 256, kv->n_kv_heads, kv->n_seqs), 256, 0, st>>>(p);
+        e = cudaGetLastError();
+    }
+    return cuda_ok(e, "attention_tree") ? 0 : -1;
+}
+
+}  // extern "C"

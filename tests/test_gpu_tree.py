@@ -298,3 +298,77 @@ def test_streams_and_graph(vbs, gpu, clean_errors):
         torch.cuda.synchronize()
         want, _ = c.want()
         np.testing.assert_allclose(out.cpu().numpy(), want, rtol=0, atol=4 * TOL)
+
+
+# ---- many rows of a KV head (other kernels than few rows) -------------------
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+def test_masked_places_may_hold_anything_many_rows(case, bad, hd):
+    c = case(seqs=2, tokens=37, nqh=8, nkh=2, hd=hd, n_ctx=(500, 3), pos=0, tree=True, window=64,
+             k_pos=lambda rng, c: padded(rng, c), head_major=hd == 96, seed=5)
+    c.sees[:, :, 2] = False
+    for x in (c.k, c.v):
+        for b in range(2):
+            end = c.n_ctx[b] + c.n_tok[b]
+            x[b, :, end:] = bad
+            x[b, :, c.n_ctx[b] + 2] = bad
+            x[b, :, :end][:, c.k_pos[b, :end] < 0] = bad
+            far = c.q_pos[b].min() - c.k_pos[b, :end] >= 64
+            x[b, :, :end][:, far] = bad
+    c.check(weights=True)
+    # visible to some rows: theirs turn, the others stay
+    c = case(tokens=40, nqh=4, nkh=1, hd=hd, n_ctx=(300,), window=100, seed=6)
+    c.v[0, 0, 205:207, 3] = bad    # tokens 0..4 (205) and 0..5 (206) see them
+    got, (want, _) = c.run(), c.want()
+    turned = ~np.isfinite(want)
+    assert turned[0, :6, :, 3].all() and turned.sum() == 6 * 4
+    assert (np.isnan(got) == np.isnan(want)).all() and (got[np.isinf(want)] == want[np.isinf(want)]).all()
+    np.testing.assert_allclose(got[~turned], want[~turned], rtol=0, atol=4 * TOL)
+
+
+@pytest.mark.parametrize("first", [0, 64, 200])
+def test_values_not_finite_in_any_tile(case, first):
+    """A value that its rows may see in the first, a middle or the last tile,
+    next to drafts that it is hidden from."""
+    c = case(tokens=30, nqh=4, nkh=1, hd=128, n_ctx=(first,), tree=True, seed=first)
+    c.sees[0] = np.eye(30, dtype=bool)
+    c.sees[0, :, 0] = True
+    c.v[0, 0, first + 7, 11] = np.inf
+    c.v[0, 0, first + 9] = np.nan
+    got, (want, _) = c.run(), c.want()
+    fine = np.isfinite(want)
+    assert (~fine).sum() == 4 + 4 * 128 and (got[0, 7, :, 11] == np.inf).all() and np.isnan(got[0, 9]).all()
+    np.testing.assert_allclose(got[fine], want[fine], rtol=0, atol=4 * TOL)
+
+
+@pytest.mark.parametrize("hd", [8, 24, 64, 72, 80, 128])
+@pytest.mark.parametrize("n_ctx,tokens", [(0, 5), (0, 130), (90, 33), (127, 1), (128, 64), (1000, 100), (4000, 17)])
+def test_many_rows(case, hd, n_ctx, tokens):
+    case(seqs=2, tokens=tokens, nqh=40, nkh=2, hd=hd, n_ctx=(n_ctx, n_ctx // 3), tree=True, head_major=hd % 3 == 0,
+         layers=2, layer=1, seed=hd + tokens).check()
+
+
+@pytest.mark.parametrize("cap,slopes,window,qscale", [(30.0, False, 0, 4.0), (0.0, True, 0, 1.0), (5.0, True, 333, 6.0)])
+@pytest.mark.parametrize("k_pos", [None, padded, evicted])
+def test_many_rows_options(case, cap, slopes, window, qscale, k_pos):
+    case(seqs=2, tokens=21, nqh=16, nkh=2, hd=128, n_ctx=(900, 1700), cap=cap, slopes=slopes, window=window, qscale=qscale,
+         tree=True, pos=0 if k_pos is None else 1700, k_pos=k_pos, seed=31).check(weights=True)
+
+
+def test_negative_scale_and_large_scores(case):
+    c = case(tokens=20, nqh=4, nkh=1, hd=128, n_ctx=(700,), seed=32)
+    c.scale = -c.scale
+    c.check()
+    c = case(tokens=3, nqh=4, nkh=1, hd=128, n_ctx=(700,), seed=33)
+    c.scale = -c.scale
+    c.check()
+
+
+def test_a_late_maximum_moves_the_reference(case):
+    """Scores that rise tile by tile, far beyond the lazy threshold."""
+    for tokens in (1, 20):
+        c = case(tokens=tokens, nqh=4, nkh=1, hd=64, n_ctx=(1500,), seed=34)
+        ramp = np.linspace(0, 40, c.M)
+        c.q[..., 0] = 1.0 / c.scale
+        c.k[0, 0, :, 0] = ramp.astype(np.float16)
+        c.check()

@@ -28,95 +28,12 @@
 //    also looks for infinities and NaN among its values: 0 * inf would carry
 //    them into rows that do not see them, so such a block adds its values
 //    one visible key at a time.
-#include "vbs_b200.h"
 #include "backend.h"
-#include "common.cuh"
-#include "kernels.h"
+#include "tree.cuh"
 
 #include <algorithm>
 
 namespace vbs {
-
-bool kv_desc_ok(const vbs_cu_kv_t *kv);
-
-struct TreeParams {
-    const float *q;
-    float *out;
-    const uint16_t *kc, *vc;      // layer's first element of sequence 0
-    uint64_t seq_stride, pos_step, head_step;
-    uint32_t max_ctx, nkh, nqh, G, hd, n_tokens, words, window, ctx_limit;
-    uint32_t row_tiles, n_splits, per_split;
-    float scale, cap;
-    const float *slopes;
-    const int32_t *n_ctx, *n_tok;
-    const uint32_t *mask;
-    const int32_t *q_pos, *k_pos;
-    uint32_t k_pos_per_head;
-    const float *weights_in;
-    float *weights_out;
-    // workspace
-    float2 *part_ml;              // [slot][split][tile rows]
-    float *part_o;                // [slot][split][tile rows][hd], slot = (seq * nkh + kv head) * row_tiles + tile
-    float *lse;                   // [seq * nkh + kv head][rows], log2 units, with weights
-    float *scores;                // [seq * nkh + kv head][rows][score_ld], log2 units, with weights
-    uint32_t score_ld;
-    uint32_t *err;
-};
-
-constexpr float TREE_LOG2E = 1.4426950408889634f;
-constexpr float TREE_BELOW = 6.0f, TREE_LAZY = 14.0f;
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Lengths of sequence b; false (flagged once) when they do not fit the cache
-// or the call's limit: the sequence is left alone.
-__device__ __forceinline__ bool tree_lengths(const TreeParams &p, uint32_t b, uint32_t &nc, uint32_t &nt) {
-    const int32_t c = p.n_ctx[b], t = p.n_tok ? p.n_tok[b] : (int32_t)p.n_tokens;
-    if (c < 0 || t < 0 || (uint32_t)t > p.n_tokens || (uint64_t)c + t > min(p.max_ctx, p.ctx_limit)) {
-        if (threadIdx.x == 0) dev_flag_error(p.err, DERR_BAD_ARG);
-        return false;
-    }
-    nc = (uint32_t)c;
-    nt = (uint32_t)t;
-    return true;
-}
-
-__device__ __forceinline__ int32_t tree_qpos(const TreeParams &p, uint32_t b, uint32_t i, uint32_t nc) {
-    return p.q_pos ? p.q_pos[(uint64_t)b * p.n_tokens + i] : (int32_t)(nc + i);
-}
-
-// First slot that any row can see: with a window over plain slots, behind
-// the lowest query position's window. All threads of the block call it.
-__device__ __forceinline__ uint32_t tree_first(const TreeParams &p, uint32_t b, uint32_t nc, uint32_t nt, int32_t *sh) {
-    if (!p.window || p.k_pos) return 0;
-    int32_t lo = 0x7FFFFFFF;
-    if (p.q_pos) {
-        for (uint32_t i = threadIdx.x; i < nt; i += blockDim.x) lo = min(lo, tree_qpos(p, b, i, nc));
-        lo = __reduce_min_sync(0xffffffffu, lo);
-        if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = lo;
-        __syncthreads();
-        for (uint32_t w = 0; w < blockDim.x / 32; ++w) lo = min(lo, sh[w]);
-        __syncthreads();
-    } else {
-        lo = (int32_t)nc;
-    }
-    const int64_t first = (int64_t)lo - p.window + 1;
-    return first <= 0 ? 0u : (uint32_t)min(first, (int64_t)nc);   // new tokens are always looked at
-}
-
-// This split's positions [t0, t1): equal parts, whole blocks of 64.
-__device__ __forceinline__ void tree_part(const TreeParams &p, uint32_t first, uint32_t end, uint32_t split, uint32_t &t0,
-                                          uint32_t &t1) {
-    const uint32_t span = end - first;
-    uint32_t per = (span + p.n_splits - 1) / p.n_splits;
-    per = max(p.per_split, (per + 63) / 64 * 64);
-    t0 = (uint32_t)min((uint64_t)end, first + (uint64_t)split * per);
-    t1 = min(end, t0 + per);
-}
 
 template <int HD, int WR, int WP> struct TreeCfg {
     static constexpr int NW = WR * WP, THREADS = NW * 32;
@@ -246,7 +163,7 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
         }
     }
     const float cap2 = p.cap * TREE_LOG2E;
-    const float pre = p.cap > 0.f ? 2.f * TREE_LOG2E / p.cap : TREE_LOG2E;   // capped: exponent of e^(2x / cap)
+    const float pre = p.cap > 0.f ? 1.f / p.cap : TREE_LOG2E;
     fac[0] *= pre;
     fac[1] *= pre;
     // highest query position of the rows, for the window's fast path
@@ -307,8 +224,7 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     x[h][e] *= fac[h];
-                    if (p.cap > 0.f)   // cap tanh(y) = cap (1 - 2 / (e^2y + 1)), in log2 units
-                        x[h][e] = cap2 - __fdividef(2.f * cap2, ex2(fminf(x[h][e], 126.f)) + 1.f);
+                    if (p.cap > 0.f) x[h][e] = tree_cap(x[h][e], cap2);
                 }
             uint32_t hidden = 0;   // bit 4 h + e: row h does not see key e
             const bool plain = tb + 16 <= min(nc, t1) && !kpos && (!p.window || (int64_t)qmax - tb < (int64_t)p.window);
@@ -592,6 +508,7 @@ __global__ void __launch_bounds__(256) tree_weights_kernel(const __grid_constant
 // ---------------------------------------------------------------------------
 struct TreePlan {
     uint32_t rows, tile_rows, row_tiles, n_splits, per_split, score_ld;
+    bool tc;                            // tree_tc_kernel
     size_t ml, o, lse, scores, bytes;   // offsets into the workspace, total
 };
 
@@ -600,17 +517,22 @@ struct TreePlan {
 // rows share the staged keys.
 static uint32_t tree_warp_rows(uint32_t rows) { return rows <= 16 ? 1 : (rows <= 32 ? 2 : 4); }
 
+constexpr uint32_t TREE_TC_MIN_ROWS = 17;
+
 static TreePlan tree_plan(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t, int n_sm) {
     TreePlan pl = {};
     const uint32_t G = t->n_q_heads / kv->n_kv_heads;
     pl.rows = t->n_tokens * G;
-    pl.tile_rows = 16 * tree_warp_rows(pl.rows);
+    pl.tc = kv->head_dim <= 128 && pl.rows >= TREE_TC_MIN_ROWS;
+    pl.tile_rows = pl.tc ? TREE_TC_ROWS : 16 * tree_warp_rows(pl.rows);
     pl.row_tiles = (pl.rows + pl.tile_rows - 1) / pl.tile_rows;
-    // parts: about two CTAs per SM, at least 64 positions each
+    // parts: about two CTAs per SM, at least 64 positions each; tree_tc_kernel
+    // fills an SM, so there one CTA each, in whole tiles
     const uint64_t ctas = (uint64_t)pl.row_tiles * kv->n_kv_heads * kv->n_seqs;
-    uint64_t s = ((uint64_t)n_sm * 2 + ctas - 1) / ctas;
-    s = std::max<uint64_t>(1, std::min<uint64_t>(s, (t->ctx_limit + 63) / 64));
-    pl.per_split = (uint32_t)(((t->ctx_limit + s - 1) / s + 63) / 64 * 64);
+    const uint32_t unit = pl.tc ? TREE_TC_SP : 64;
+    uint64_t s = pl.tc ? (uint64_t)n_sm / ctas : ((uint64_t)n_sm * 2 + ctas - 1) / ctas;
+    s = std::max<uint64_t>(1, std::min<uint64_t>(s, (t->ctx_limit + unit - 1) / unit));
+    pl.per_split = (uint32_t)(((t->ctx_limit + s - 1) / s + unit - 1) / unit * unit);
     pl.n_splits = (t->ctx_limit + pl.per_split - 1) / pl.per_split;
     auto take = [&](size_t n) { const size_t at = pl.bytes; pl.bytes += (n + 255) / 256 * 256; return at; };
     const size_t heads = (size_t)kv->n_seqs * kv->n_kv_heads;
@@ -634,6 +556,28 @@ static bool tree_desc_ok(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t) {
     if (t->n_tokens > 4096u || t->n_q_heads / kv->n_kv_heads > 256u) return false;
     if (!(t->scale == t->scale) || !(t->softcap >= 0.f) || t->window > 0x7FFFFFFFu) return false;
     return !(t->weights_in && !t->weights_out);
+}
+
+// Tensor map of one layer's keys or values, boxes of 64 dims x `rows`
+// positions. Encoded anew by every call (host arithmetic, no driver call).
+static cudaError_t tree_map(CUtensorMap *m, const uint16_t *base, const vbs_cu_kv_t *kv, uint32_t rows) {
+    using Fn = decltype(&cuTensorMapEncodeTiled);
+    static const Fn encode = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        return cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &r) == cudaSuccess &&
+                       r == cudaDriverEntryPointSuccess ? reinterpret_cast<Fn>(f) : nullptr;
+    }();
+    if (!encode) return cudaErrorNotSupported;
+    const uint64_t pos = kv->head_major ? kv->head_dim : (uint64_t)kv->n_kv_heads * kv->head_dim;
+    const uint64_t head = kv->head_major ? (uint64_t)kv->max_ctx * kv->head_dim : kv->head_dim;
+    const uint64_t seq = kv->n_seqs > 1 ? kv->seq_stride : pos * kv->max_ctx;
+    const cuuint64_t dims[4] = {kv->head_dim, kv->max_ctx, kv->n_kv_heads, kv->n_seqs};
+    const cuuint64_t strides[3] = {pos * 2, head * 2, seq * 2};
+    const cuuint32_t box[4] = {64, rows, 1, 1}, one[4] = {1, 1, 1, 1};
+    return encode(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<uint16_t *>(base), dims, strides, box, one,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
 template <int HD, int WR, int WP> static cudaError_t tree_go(const TreeParams &p, dim3 grid, cudaStream_t st) {
@@ -663,6 +607,7 @@ cudaError_t tree_configure() {
     cudaError_t e = tree_cfg_rows<64>();
     if (e == cudaSuccess) e = tree_cfg_rows<128>();
     if (e == cudaSuccess) e = tree_cfg_rows<256>();
+    if (e == cudaSuccess) e = tree_tc_configure();
     return e;
 }
 
@@ -723,7 +668,15 @@ int vbs_cu_attention_tree(const vbs_cu_kv_t *kv, uint32_t layer, const vbs_cu_tr
     const dim3 grid(kv->n_kv_heads * pl.row_tiles, pl.n_splits, kv->n_seqs);
     const uint32_t wr = pl.tile_rows / 16;
     note_launches(1u + (pl.n_splits > 1) + (t->weights_out != nullptr));
-    cudaError_t e = kv->head_dim <= 64 ? tree_go_rows<64>(p, wr, grid, st)
+    CUtensorMap km, vm;
+    cudaError_t e = cudaSuccess;
+    if (pl.tc) {
+        e = tree_map(&km, p.kc, kv, TREE_TC_SP);
+        if (e == cudaSuccess) e = tree_map(&vm, p.vc, kv, TREE_TC_SP);
+    }
+    if (e == cudaSuccess)
+        e = pl.tc ? tree_tc_launch(p, km, vm, kv->n_seqs, st)
+                    : kv->head_dim <= 64 ? tree_go_rows<64>(p, wr, grid, st)
                                        : (kv->head_dim <= 128 ? tree_go_rows<128>(p, wr, grid, st) : tree_go_rows<256>(p, wr, grid, st));
     if (e == cudaSuccess && pl.n_splits > 1) {
         tree_merge_kernel<<<dim3(pl.rows, kv->n_kv_heads, kv->n_seqs), TREE_MW * 32, 0, st>>>(p, pl.tile_rows);

@@ -1,0 +1,124 @@
+// tree.cuh -- what the kernels of the attention over a cache whose slots are
+// not positions share (tree.cu: mma.sync kernel, join, weights; tree_tc.cu:
+// tcgen05 kernel).
+#pragma once
+
+#include "vbs_b200.h"
+#include <cuda.h>
+#include "common.cuh"
+#include "kernels.h"
+
+namespace vbs {
+
+bool kv_desc_ok(const vbs_cu_kv_t *kv);
+
+struct TreeParams {
+    const float *q;
+    float *out;
+    const uint16_t *kc, *vc;      // layer's first element of sequence 0
+    uint64_t seq_stride, pos_step, head_step;
+    uint32_t max_ctx, nkh, nqh, G, hd, n_tokens, words, window, ctx_limit;
+    uint32_t row_tiles, n_splits, per_split;
+    float scale, cap;
+    const float *slopes;
+    const int32_t *n_ctx, *n_tok;
+    const uint32_t *mask;
+    const int32_t *q_pos, *k_pos;
+    uint32_t k_pos_per_head;
+    const float *weights_in;
+    float *weights_out;
+    // workspace
+    float2 *part_ml;              // [slot][split][tile rows]
+    float *part_o;                // [slot][split][tile rows][hd], slot = (seq * nkh + kv head) * row_tiles + tile
+    float *lse;                   // [seq * nkh + kv head][rows], log2 units, with weights
+    float *scores;                // [seq * nkh + kv head][rows][score_ld], log2 units, with weights
+    uint32_t score_ld;
+    uint32_t *err;
+};
+
+constexpr float TREE_LOG2E = 1.4426950408889634f;
+constexpr float TREE_BELOW = 6.0f, TREE_LAZY = 14.0f;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// cap * tanh(x / cap) in log2 units from y = x / cap. Below 1 the Pade form
+// y (945 + 105 y^2 + y^4) / (945 + 420 y^2 + 15 y^4) of tanh, off by 6e-8 at
+// most, so that small scores keep their relative accuracy (1 - 2 / (e^2y + 1)
+// alone would be off by 2^-24 of the cap); above 1 (e^2y - 1) / (e^2y + 1).
+__device__ __forceinline__ float tree_cap(float y, float cap2) {
+    const float a = fminf(fabsf(y), 30.f), z = y * y, e = ex2(a * (2.f * TREE_LOG2E));
+    const bool small = a < 1.f;
+    const float num = small ? a * fmaf(z, z + 105.f, 945.f) : e - 1.f;
+    const float den = small ? fmaf(z, fmaf(z, 15.f, 420.f), 945.f) : e + 1.f;
+    return y != y ? y : copysignf(cap2 * __fdividef(num, den), y);
+}
+
+// Lengths of sequence b; false (flagged once) when they do not fit the cache
+// or the call's limit: the sequence is left alone.
+__device__ __forceinline__ bool tree_lengths(const TreeParams &p, uint32_t b, uint32_t &nc, uint32_t &nt) {
+    const int32_t c = p.n_ctx[b], t = p.n_tok ? p.n_tok[b] : (int32_t)p.n_tokens;
+    if (c < 0 || t < 0 || (uint32_t)t > p.n_tokens || (uint64_t)c + t > min(p.max_ctx, p.ctx_limit)) {
+        if (threadIdx.x == 0) dev_flag_error(p.err, DERR_BAD_ARG);
+        return false;
+    }
+    nc = (uint32_t)c;
+    nt = (uint32_t)t;
+    return true;
+}
+
+__device__ __forceinline__ int32_t tree_qpos(const TreeParams &p, uint32_t b, uint32_t i, uint32_t nc) {
+    return p.q_pos ? p.q_pos[(uint64_t)b * p.n_tokens + i] : (int32_t)(nc + i);
+}
+
+// First slot that any row can see: with a window over plain slots, behind
+// the lowest query position's window. All threads of the block call it.
+__device__ __forceinline__ uint32_t tree_first(const TreeParams &p, uint32_t b, uint32_t nc, uint32_t nt, int32_t *sh) {
+    if (!p.window || p.k_pos) return 0;
+    int32_t lo = 0x7FFFFFFF;
+    if (p.q_pos) {
+        for (uint32_t i = threadIdx.x; i < nt; i += blockDim.x) lo = min(lo, tree_qpos(p, b, i, nc));
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = lo;
+        __syncthreads();
+        for (uint32_t w = 0; w < blockDim.x / 32; ++w) lo = min(lo, sh[w]);
+        __syncthreads();
+    } else {
+        lo = (int32_t)nc;
+    }
+    const int64_t first = (int64_t)lo - p.window + 1;
+    return first <= 0 ? 0u : (uint32_t)min(first, (int64_t)nc) / 64 * 64;   // new tokens are always looked at
+}
+
+// This split's positions [t0, t1): equal parts, whole blocks of 64.
+__device__ __forceinline__ void tree_part(const TreeParams &p, uint32_t first, uint32_t end, uint32_t split, uint32_t &t0,
+                                          uint32_t &t1) {
+    const uint32_t span = end - first;
+    uint32_t per = (span + p.n_splits - 1) / p.n_splits;
+    per = max(p.per_split, (per + 63) / 64 * 64);
+    t0 = (uint32_t)min((uint64_t)end, first + (uint64_t)split * per);
+    t1 = min(end, t0 + per);
+}
+
+// 64 dims x n positions of one KV head of a cache, from a tensor map of the
+// layer's keys or values ([head_dim][position][kv head][seq], rows of 128
+// bytes in shared memory, their 16-byte chunks XOR-ed with the position's
+// low three bits). Dims from head_dim on and positions from max_ctx on
+// arrive as zeros.
+__device__ __forceinline__ void tree_tma(uint32_t dst, const CUtensorMap *map, uint32_t dim, uint32_t pos, uint32_t head,
+                                         uint32_t seq, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+        ::"r"(dst), "l"(map), "r"(dim), "r"(pos), "r"(head), "r"(seq), "r"(bar) : "memory");
+}
+
+// tree_tc.cu: row tiles of TREE_TC_ROWS, head_dim up to 128.
+constexpr uint32_t TREE_TC_ROWS = 128, TREE_TC_SP = 128;
+cudaError_t tree_tc_configure();
+cudaError_t tree_tc_launch(const TreeParams &p, const CUtensorMap &km, const CUtensorMap &vm, uint32_t n_seqs,
+                           cudaStream_t st);
+
+}  // namespace vbs

@@ -3,7 +3,7 @@
 //
 //   x_rt = scale q_r . K_t;  capped: c tanh(x / c);  + slope_r (kpos_t - qpos_r)
 //   out_r = sum_t p_rt V_t,  p_rt = softmax over the visible t
-//   weights: W_t += sum over the rows of a KV head of p_rt
+//   (the weights W_t, sums over the rows of p_rt: tree_wt.cu)
 //
 // Rows: the n_tok tokens x G query heads of one KV head, row r = token * G +
 // head, so a row tile's queries are read in runs. Every key of the context is
@@ -60,6 +60,7 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
     const int wr = warp % WR, wp = warp / WR;
     const uint32_t kvh = blockIdx.x % p.nkh, tile = blockIdx.x / p.nkh, split = blockIdx.y, b = blockIdx.z;
     const uint32_t G = p.G, R0 = tile * C::ROWS;
+    pdl_launch_dependents();
     uint32_t nc, nt;
     if (!tree_lengths(p, b, nc, nt) || R0 >= nt * G) return;
     const uint32_t end = nc + nt, nrows = nt * G;
@@ -174,13 +175,6 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
 #pragma unroll
     for (int n = 0; n < HD / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
     float mref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    float *sc_out[2] = {nullptr, nullptr};
-    if (p.scores) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            sc_out[h] = p.scores + ((uint64_t)(b * p.nkh + kvh) * (p.n_tokens * G) + (on[h] ? row[h] : 0u)) * p.score_ld;
-    }
-
     for (uint32_t c = 0; c < nch; ++c) {
         if (c + C::NST - 1 < nch) issue(c + C::NST - 1);
         cp_async_commit();
@@ -251,17 +245,6 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
                             x[h][e] = -INFINITY;
                             hidden |= 1u << (4 * h + e);
                         }
-                    }
-                }
-            }
-            if (p.scores) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (!on[h]) continue;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t t = tb + qd + (e & 1) + 8 * (e >> 1);
-                        if (t < t1) sc_out[h][t] = x[h][e];
                     }
                 }
             }
@@ -403,66 +386,83 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
 }
 
 // ---------------------------------------------------------------------------
-// Join of the parts: one CTA per row, its warps over the parts, then the
-// warps' sums in order. Reads every part once.
+// Join of the parts: one CTA per row. The parts' maxima and sums are read at
+// once and become their factors in shared memory; then the warps share the
+// parts, TREE_MU loads in flight each, and their sums are added in order.
+// Launched as a programmatic dependent of the kernel that writes the parts:
+// it is on the SMs when that one ends.
 // ---------------------------------------------------------------------------
-constexpr int TREE_MW = 4;
+constexpr int TREE_MW = 8, TREE_MU = 8;
+constexpr uint32_t TREE_MAX_PARTS = 1024;
 
 __global__ void __launch_bounds__(TREE_MW * 32) tree_merge_kernel(const __grid_constant__ TreeParams p, uint32_t tile_rows) {
+    __shared__ float fac[TREE_MAX_PARTS];
     __shared__ float sm_m[TREE_MW], sm_l[TREE_MW];
-    __shared__ float sm_o[TREE_MW][256];
+    __shared__ __align__(16) float sm_o[TREE_MW][256];
     const uint32_t r = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t nc, nt;
-    if (!tree_lengths(p, b, nc, nt) || r >= nt * p.G) return;
-    const uint32_t tile = r / tile_rows, ri = r % tile_rows;
+    const bool live = tree_lengths(p, b, nc, nt) && r < nt * p.G;
+    pdl_wait();
+    pdl_launch_dependents();
+    if (!live) return;
+    const uint32_t tile = r / tile_rows, ri = r % tile_rows, ns = p.n_splits;
     const uint64_t slot = (uint64_t)(b * p.nkh + kvh) * p.row_tiles + tile;
-    const float2 *ml = p.part_ml + slot * p.n_splits * tile_rows + ri;
-    const float *po = p.part_o + (slot * p.n_splits * tile_rows + ri) * p.hd;
+    const float2 *ml = p.part_ml + slot * ns * tile_rows + ri;
+    const float *po = p.part_o + (slot * ns * tile_rows + ri) * p.hd;
+    float2 x[TREE_MAX_PARTS / (TREE_MW * 32)];
     float M = -INFINITY;
-    for (uint32_t s = threadIdx.x; s < p.n_splits; s += TREE_MW * 32) M = fmaxf(M, ml[(uint64_t)s * tile_rows].x);
+#pragma unroll
+    for (uint32_t k = 0; k < TREE_MAX_PARTS / (TREE_MW * 32); ++k) {
+        const uint32_t s = threadIdx.x + k * TREE_MW * 32;
+        x[k] = s < ns ? __ldcg(ml + (uint64_t)s * tile_rows) : make_float2(-INFINITY, 0.f);
+        M = fmaxf(M, x[k].x);
+    }
     M = warp_max(M);
     if (lane == 0) sm_m[warp] = M;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < TREE_MW; ++w) M = fmaxf(M, sm_m[w]);
     float L = 0.f;
-    float4 a[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-    constexpr int U = 4;
-    for (uint32_t s0 = warp; s0 < p.n_splits; s0 += TREE_MW * U) {
-        float f[U];
-        float4 v[U][2];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint32_t s = s0 + u * TREE_MW;
-            f[u] = 0.f;
-            float2 x = make_float2(-INFINITY, 0.f);
-            if (s < p.n_splits) x = ml[(uint64_t)s * tile_rows];
-            const bool live = !(x.y == 0.f);   // an empty part has no sums; a NaN goes through
-            if (live) { f[u] = ex2(x.x - M); L += x.y * f[u]; }
+    for (uint32_t k = 0; k < TREE_MAX_PARTS / (TREE_MW * 32); ++k) {
+        const uint32_t s = threadIdx.x + k * TREE_MW * 32;
+        const bool has = !(x[k].y == 0.f);   // an empty part has no sums (and wrote none); a NaN goes through
+        const float f = has ? ex2(x[k].x - M) : 0.f;
+        if (has) L += x[k].y * f;
+        if (s < ns) fac[s] = has ? f : -1.f;
+    }
+    L = warp_sum(L);
+    if (lane == 0) sm_l[warp] = L;
+    __syncthreads();
+    const uint32_t q4 = p.hd / 4;   // 16-byte pieces of a row; a warp covers 32 pieces, wider rows take two
+    for (uint32_t d0 = 0; d0 < q4; d0 += 32) {
+        const uint32_t d = d0 + lane;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (uint32_t s0 = warp; s0 < ns; s0 += TREE_MW * TREE_MU) {
+            float4 v[TREE_MU];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const uint32_t d = (lane + 32 * k) * 4;
-                v[u][k] = live && d < p.hd ? *reinterpret_cast<const float4 *>(po + (uint64_t)s * tile_rows * p.hd + d)
-                                           : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int u = 0; u < TREE_MU; ++u) {
+                const uint32_t s = s0 + u * TREE_MW;
+                v[u] = s < ns && !(fac[s] < 0.f) && d < q4 ? __ldcg(reinterpret_cast<const float4 *>(po + (uint64_t)s * tile_rows * p.hd) + d)
+                                                         : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int u = 0; u < TREE_MU; ++u) {
+                const uint32_t s = s0 + u * TREE_MW;
+                const float f = s < ns ? fac[s] : 0.f;   // -1 meets zeros
+                a.x = fmaf(v[u].x, f, a.x); a.y = fmaf(v[u].y, f, a.y);
+                a.z = fmaf(v[u].z, f, a.z); a.w = fmaf(v[u].w, f, a.w);
             }
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                a[k].x = fmaf(v[u][k].x, f[u], a[k].x); a[k].y = fmaf(v[u][k].y, f[u], a[k].y);
-                a[k].z = fmaf(v[u][k].z, f[u], a[k].z); a[k].w = fmaf(v[u][k].w, f[u], a[k].w);
-            }
+        *reinterpret_cast<float4 *>(&sm_o[warp][(lane + d0) * 4]) = a;
     }
-    if (lane == 0) sm_l[warp] = L;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) *reinterpret_cast<float4 *>(&sm_o[warp][(lane + 32 * k) * 4]) = a[k];
     __syncthreads();
     L = 0.f;
 #pragma unroll
     for (int w = 0; w < TREE_MW; ++w) L += sm_l[w];
     const float il = L == 0.f ? 0.f : 1.f / L;
-    float *out = p.out + (((uint64_t)b * p.n_tokens + r / p.G) * p.nqh + kvh * p.G + r % p.G) * p.hd;
+    const uint32_t tok = tree_token(p, r);
+    float *out = p.out + (((uint64_t)b * p.n_tokens + tok) * p.nqh + kvh * p.G + (r - tok * p.G)) * p.hd;
     for (uint32_t d = threadIdx.x; d < p.hd; d += TREE_MW * 32) {
         float v = 0.f;
 #pragma unroll
@@ -474,42 +474,12 @@ __global__ void __launch_bounds__(TREE_MW * 32) tree_merge_kernel(const __grid_c
 }
 
 // ---------------------------------------------------------------------------
-// Attention weights per slot: W_t = W_in,t + sum over rows of
-// 2^(score - lse). One thread per slot, rows in order, so the sum does not
-// depend on the split.
-// ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) tree_weights_kernel(const __grid_constant__ TreeParams p) {
-    __shared__ int32_t sh_min[8];
-    const uint32_t kvh = blockIdx.y, b = blockIdx.z;
-    uint32_t nc, nt;
-    if (!tree_lengths(p, b, nc, nt)) return;
-    const uint32_t first = tree_first(p, b, nc, nt, sh_min);
-    const uint32_t t = blockIdx.x * 256 + threadIdx.x;
-    if (t >= nc + nt) return;
-    const uint64_t at = (uint64_t)(b * p.nkh + kvh) * p.max_ctx + t;
-    float w = p.weights_in ? p.weights_in[at] : 0.f;
-    if (t >= first) {
-        const uint64_t base = (uint64_t)(b * p.nkh + kvh) * (p.n_tokens * p.G);
-        const uint32_t n = nt * p.G;
-        float sum = 0.f;
-#pragma unroll 4
-        for (uint32_t r = 0; r < n; ++r) {
-            const float z = p.lse[base + r];
-            const float e = ex2(p.scores[(base + r) * p.score_ld + t] - (z == -INFINITY ? 0.f : z));
-            sum += e;   // a row that sees nothing: every score -inf, weight 0
-        }
-        w += sum;
-    }
-    p.weights_out[at] = w;
-}
-
-// ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 struct TreePlan {
-    uint32_t rows, tile_rows, row_tiles, n_splits, per_split, score_ld;
+    uint32_t rows, tile_rows, row_tiles, n_splits, per_split;
     bool tc;                            // tree_tc_kernel
-    size_t ml, o, lse, scores, bytes;   // offsets into the workspace, total
+    size_t ml, o, lse, bytes;   // offsets into the workspace, total
 };
 
 // Warps over rows and over positions of a CTA by the rows of a KV head: few
@@ -524,14 +494,14 @@ static TreePlan tree_plan(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t, int n_s
     const uint32_t G = t->n_q_heads / kv->n_kv_heads;
     pl.rows = t->n_tokens * G;
     pl.tc = kv->head_dim <= 128 && pl.rows >= TREE_TC_MIN_ROWS;
-    pl.tile_rows = pl.tc ? TREE_TC_ROWS : 16 * tree_warp_rows(pl.rows);
+    pl.tile_rows = pl.tc ? (pl.rows > TREE_TC_ROWS ? 2 * TREE_TC_ROWS : TREE_TC_ROWS) : 16 * tree_warp_rows(pl.rows);
     pl.row_tiles = (pl.rows + pl.tile_rows - 1) / pl.tile_rows;
     // parts: about two CTAs per SM, at least 64 positions each; tree_tc_kernel
     // fills an SM, so there one CTA each, in whole tiles
     const uint64_t ctas = (uint64_t)pl.row_tiles * kv->n_kv_heads * kv->n_seqs;
     const uint32_t unit = pl.tc ? TREE_TC_SP : 64;
     uint64_t s = pl.tc ? (uint64_t)n_sm / ctas : ((uint64_t)n_sm * 2 + ctas - 1) / ctas;
-    s = std::max<uint64_t>(1, std::min<uint64_t>(s, (t->ctx_limit + unit - 1) / unit));
+    s = std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint64_t>(s, TREE_MAX_PARTS), (t->ctx_limit + unit - 1) / unit));
     pl.per_split = (uint32_t)(((t->ctx_limit + s - 1) / s + unit - 1) / unit * unit);
     pl.n_splits = (t->ctx_limit + pl.per_split - 1) / pl.per_split;
     auto take = [&](size_t n) { const size_t at = pl.bytes; pl.bytes += (n + 255) / 256 * 256; return at; };
@@ -540,11 +510,7 @@ static TreePlan tree_plan(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t, int n_s
         pl.ml = take(heads * pl.row_tiles * pl.n_splits * pl.tile_rows * sizeof(float2));
         pl.o = take(heads * pl.row_tiles * pl.n_splits * pl.tile_rows * kv->head_dim * sizeof(float));
     }
-    if (t->weights_out) {
-        pl.score_ld = (t->ctx_limit + 3) / 4 * 4;
-        pl.lse = take(heads * pl.rows * sizeof(float));
-        pl.scores = take(heads * pl.rows * pl.score_ld * sizeof(float));
-    }
+    if (t->weights_out) pl.lse = take(heads * pl.rows * sizeof(float));
     pl.bytes = std::max<size_t>(pl.bytes, 256);
     return pl;
 }
@@ -580,6 +546,19 @@ static cudaError_t tree_map(CUtensorMap *m, const uint16_t *base, const vbs_cu_k
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+static cudaError_t tree_merge_launch(const TreeParams &p, dim3 grid, uint32_t tile_rows, cudaStream_t st) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(TREE_MW * 32);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, tree_merge_kernel, p, tile_rows);
+}
+
 template <int HD, int WR, int WP> static cudaError_t tree_go(const TreeParams &p, dim3 grid, cudaStream_t st) {
     using C = TreeCfg<HD, WR, WP>;
     tree_mma_kernel<HD, WR, WP><<<grid, C::THREADS, C::SMEM, st>>>(p);
@@ -608,6 +587,10 @@ cudaError_t tree_configure() {
     if (e == cudaSuccess) e = tree_cfg_rows<128>();
     if (e == cudaSuccess) e = tree_cfg_rows<256>();
     if (e == cudaSuccess) e = tree_tc_configure();
+    if (e == cudaSuccess) e = tree_weights_configure();
+    // the join takes the attention kernels' split of shared memory and L1:
+    // changing it costs an SM several microseconds between kernels
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(tree_merge_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
     return e;
 }
 
@@ -659,33 +642,23 @@ int vbs_cu_attention_tree(const vbs_cu_kv_t *kv, uint32_t layer, const vbs_cu_tr
     uint8_t *w = static_cast<uint8_t *>(work);
     p.part_ml = reinterpret_cast<float2 *>(w + pl.ml);
     p.part_o = reinterpret_cast<float *>(w + pl.o);
-    if (t->weights_out) {
-        p.lse = reinterpret_cast<float *>(w + pl.lse);
-        p.scores = reinterpret_cast<float *>(w + pl.scores);
-        p.score_ld = pl.score_ld;
-    }
+    if (t->weights_out) p.lse = reinterpret_cast<float *>(w + pl.lse);
+    p.g_magic = (uint32_t)((0x100000000ull + p.G - 1) / p.G);
     p.err = d->err;
     const dim3 grid(kv->n_kv_heads * pl.row_tiles, pl.n_splits, kv->n_seqs);
     const uint32_t wr = pl.tile_rows / 16;
     note_launches(1u + (pl.n_splits > 1) + (t->weights_out != nullptr));
     CUtensorMap km, vm;
     cudaError_t e = cudaSuccess;
-    if (pl.tc) {
-        e = tree_map(&km, p.kc, kv, TREE_TC_SP);
-        if (e == cudaSuccess) e = tree_map(&vm, p.vc, kv, TREE_TC_SP);
-    }
+    if (pl.tc || t->weights_out) e = tree_map(&km, p.kc, kv, TREE_TC_SP);
+    if (e == cudaSuccess && pl.tc) e = tree_map(&vm, p.vc, kv, TREE_TC_SP);
     if (e == cudaSuccess)
-        e = pl.tc ? tree_tc_launch(p, km, vm, kv->n_seqs, st)
+        e = pl.tc ? tree_tc_launch(p, km, vm, kv->n_seqs, pl.tile_rows > TREE_TC_ROWS, st)
                     : kv->head_dim <= 64 ? tree_go_rows<64>(p, wr, grid, st)
                                        : (kv->head_dim <= 128 ? tree_go_rows<128>(p, wr, grid, st) : tree_go_rows<256>(p, wr, grid, st));
-    if (e == cudaSuccess && pl.n_splits > 1) {
-        tree_merge_kernel<<<dim3(pl.rows, kv->n_kv_heads, kv->n_seqs), TREE_MW * 32, 0, st>>>(p, pl.tile_rows);
-        e = cudaGetLastError();
-    }
-    if (e == cudaSuccess && t->weights_out) {
-        tree_weights_kernel<<<dim3((t->ctx_limit + 255) / 256, kv->n_kv_heads, kv->n_seqs), 256, 0, st>>>(p);
-        e = cudaGetLastError();
-    }
+    if (e == cudaSuccess && pl.n_splits > 1)
+        e = tree_merge_launch(p, dim3(pl.rows, kv->n_kv_heads, kv->n_seqs), pl.tile_rows, st);
+    if (e == cudaSuccess && t->weights_out) e = tree_weights_launch(p, km, kv->n_seqs, d->n_sm, st);
     return cuda_ok(e, "attention_tree") ? 0 : -1;
 }
 

@@ -31,8 +31,7 @@ struct TreeParams {
     float2 *part_ml;              // [slot][split][tile rows]
     float *part_o;                // [slot][split][tile rows][hd], slot = (seq * nkh + kv head) * row_tiles + tile
     float *lse;                   // [seq * nkh + kv head][rows], log2 units, with weights
-    float *scores;                // [seq * nkh + kv head][rows][score_ld], log2 units, with weights
-    uint32_t score_ld;
+    uint32_t g_magic;             // ceil(2^32 / G): row / G without a division
     uint32_t *err;
 };
 
@@ -72,6 +71,17 @@ __device__ __forceinline__ bool tree_lengths(const TreeParams &p, uint32_t b, ui
 
 __device__ __forceinline__ int32_t tree_qpos(const TreeParams &p, uint32_t b, uint32_t i, uint32_t nc) {
     return p.q_pos ? p.q_pos[(uint64_t)b * p.n_tokens + i] : (int32_t)(nc + i);
+}
+
+// Token of a row (row < 2^20, G <= 256: the product with the rounded-up
+// reciprocal is exact).
+__device__ __forceinline__ uint32_t tree_token(const TreeParams &p, uint32_t row) {
+    return p.G == 1 ? row : __umulhi(row, p.g_magic);
+}
+
+// Position of slot t (kpos: the row of k_pos, or NULL).
+__device__ __forceinline__ int32_t tree_kpos(const TreeParams &p, const int32_t *kpos, uint32_t b, uint32_t t, uint32_t nc) {
+    return kpos ? kpos[t] : (t < nc ? (int32_t)t : tree_qpos(p, b, t - nc, nc));
 }
 
 // First slot that any row can see: with a window over plain slots, behind
@@ -119,6 +129,10 @@ __device__ __forceinline__ void tree_tma(uint32_t dst, const CUtensorMap *map, u
 constexpr uint32_t TREE_TC_ROWS = 128, TREE_TC_SP = 128;
 cudaError_t tree_tc_configure();
 cudaError_t tree_tc_launch(const TreeParams &p, const CUtensorMap &km, const CUtensorMap &vm, uint32_t n_seqs,
-                           cudaStream_t st);
+                           uint32_t dual, cudaStream_t st);
+
+// tree_wt.cu: the weights per slot, after the attention wrote lse.
+cudaError_t tree_weights_configure();
+cudaError_t tree_weights_launch(const TreeParams &p, const CUtensorMap &km, uint32_t n_seqs, int n_sm, cudaStream_t st);
 
 }  // namespace vbs

@@ -39,7 +39,7 @@ bool kv_desc_ok(const vbs_cu_kv_t *kv) {
 // 8 dims (4 pairs) of every head it visits, so the four sines and cosines
 // are computed once and stay in registers; heads are spread over the block
 // (and, for few tokens, over blockIdx.y), and the loads of ROPE_U heads are
-// issued before the first is used.
+// issued before the first is used, the first ones before the angles.
 // ---------------------------------------------------------------------------
 constexpr int ROPE_THREADS = 256, ROPE_U = 4;
 
@@ -76,6 +76,24 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_store_kernel(const __grid_c
     const bool halves = turned && p.r.halves;
     const uint32_t da = halves ? 4 * u : 8 * u, db = halves ? rot / 2 + 4 * u : 8 * u + 4;
 
+    auto src = [&](uint32_t rw) -> const float * {
+        if (rw < p.nqh) return p.q + (uint64_t)tok * p.q_stride + (uint64_t)rw * hd;
+        const uint32_t h = rw - p.nqh;
+        return h < p.nkh ? p.k + (uint64_t)tok * p.kv_stride + (uint64_t)h * hd
+                         : p.v + (uint64_t)tok * p.kv_stride + (uint64_t)(h - p.nkh) * hd;
+    };
+    float4 xa[ROPE_U], xb[ROPE_U];
+    auto fetch = [&](uint32_t r0) {
+#pragma unroll
+        for (int j = 0; j < ROPE_U; ++j) {
+            const uint32_t rw = r0 + j * step;
+            if (rw >= rows) continue;   // (a token without a slot is read too: its slot is not waited for)
+            const float *s = src(rw);
+            xa[j] = *reinterpret_cast<const float4 *>(s + da);
+            xb[j] = *reinterpret_cast<const float4 *>(s + db);
+        }
+    };
+    fetch(row);
     int32_t slot = -1;
     uint64_t at0 = 0;
     if (p.k) {
@@ -99,22 +117,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_store_kernel(const __grid_c
             sincospif((float)frac * 0x1p-31f, &sn[i], &c[i]);
         }
     }
-    auto src = [&](uint32_t rw) -> const float * {
-        if (rw < p.nqh) return p.q + (uint64_t)tok * p.q_stride + (uint64_t)rw * hd;
-        const uint32_t h = rw - p.nqh;
-        return h < p.nkh ? p.k + (uint64_t)tok * p.kv_stride + (uint64_t)h * hd
-                         : p.v + (uint64_t)tok * p.kv_stride + (uint64_t)(h - p.nkh) * hd;
-    };
-    for (; row < rows; row += step * ROPE_U) {
-        float4 xa[ROPE_U], xb[ROPE_U];
-#pragma unroll
-        for (int j = 0; j < ROPE_U; ++j) {
-            const uint32_t rw = row + j * step;
-            if (rw >= rows || (rw >= p.nqh && slot < 0)) continue;
-            const float *s = src(rw);
-            xa[j] = *reinterpret_cast<const float4 *>(s + da);
-            xb[j] = *reinterpret_cast<const float4 *>(s + db);
-        }
+    for (; row < rows; row += step * ROPE_U, fetch(row)) {
 #pragma unroll
         for (int j = 0; j < ROPE_U; ++j) {
             const uint32_t rw = row + j * step;
@@ -157,16 +160,33 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_store_kernel(const __grid_c
 // Choice of the slots to keep: exact selection of the r-th highest of m scores
 // per list, ties to the lowest index, result ascending.
 // Scores become 32-bit keys in the scores' order and stay in shared memory,
-// so global memory is read once. The r-th highest key is found by narrowing
-// its range: a histogram of SEL_BINS equal bins over [min, max] of the keys,
-// then over the bin that holds it, at most three times (11 bits each). The
-// output place of a kept slot is the count of kept slots before it (ballots
-// and one scan). A cluster of 1, 2, 4 or 8 CTAs shares a list: each holds a
-// part of it, histograms are read from the other CTAs' shared memory.
+// so global memory is read once:
+//  1. stored, with a histogram of their top 12 bits (sign, exponent and three
+//     mantissa bits spread accumulated weights over a hundred bins or more);
+//     the bin that holds the r-th highest is known after it.
+//  2. what lies above that bin becomes a bit per key, what lies in it a short
+//     list, on which two more histograms (10 bits each) find the key; the
+//     list's keys above it join the bits, those equal to it get bits of their
+//     own. A bin with more than SEL_CAND keys (many equal scores) is searched
+//     in place instead of from the list.
+//  3. the kept slots are written from the bits, 32 keys a word: their places
+//     are the counts of kept slots before them.
+// (Bits in place of a third look at the keys, and groups of 32 keys that are
+// not at an edge without tests per key: 103.7 -> MEASURED for 1024 lists of
+// up to 16384, which instruction issue bounds.)
+// Every warp owns a run of consecutive keys and visits only those, so the
+// counts per warp are all that has to be scanned. A cluster of 1, 2, 4 or 8
+// CTAs shares a list: each holds a part of it, histograms and counts are read
+// from the other CTAs' shared memory.
 // ---------------------------------------------------------------------------
-constexpr uint32_t SEL_THREADS = 512, SEL_WARPS = SEL_THREADS / 32, SEL_BINS = 2048, SEL_CHUNK_MAX = 49152;
+constexpr uint32_t SEL_THREADS = 512, SEL_WARPS = SEL_THREADS / 32, SEL_CHUNK_MAX = 45056;
 constexpr uint32_t SEL_N_MAX = 8 * SEL_CHUNK_MAX;
-constexpr uint32_t SEL_HDR = 256;   // bytes of small shared state
+constexpr uint32_t SEL_BINS = 4096, SEL_BINS2 = 1024, SEL_CAND = 2048;
+constexpr int SEL_U = 8;            // keys in flight per thread
+// shared memory: state, histograms (12 bits, then 2 x 10), the list, the keys
+constexpr uint32_t SEL_STATE = 512, SEL_FIXED = SEL_STATE + (SEL_BINS + 2 * SEL_BINS2) * 4 + SEL_CAND * 2;
+
+__host__ __device__ constexpr uint32_t sel_keys_bytes(uint32_t chunk) { return ((chunk + 31) / 32 + SEL_WARPS) * 8 + (chunk + 3) / 4 * 16; }
 
 struct SelectParams {
     const float *scores;
@@ -184,27 +204,51 @@ __device__ __forceinline__ uint32_t score_key(float f) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Exclusive scan of v over the block; total in *sum. sh: SEL_WARPS words.
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *sh, uint32_t *sum) {
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint32_t x = v;
+// Adds 1 to a bin per lane (bin ~0: none); all lanes of the warp call it.
+// Lanes that agree (equal scores) make one addition.
+__device__ __forceinline__ void hist_add(uint32_t *h, uint32_t bin) {
+    const uint32_t b0 = __shfl_sync(0xffffffffu, bin, 0);
+    if (__all_sync(0xffffffffu, bin == b0)) {
+        if ((threadIdx.x & 31) == 0 && bin != 0xFFFFFFFFu) atomicAdd(&h[bin], 32u);
+    } else if (bin != 0xFFFFFFFFu) {
+        atomicAdd(&h[bin], 1u);
+    }
+}
+
+// The bin of `bins` (PER per thread) that holds the r-th highest, and how many
+// lie above it, summed over the cluster's histograms; in st[0], st[1]. st[2..]:
+// scratch. The block is synchronised on return.
+template <int PER>
+__device__ __forceinline__ void hist_find(cg::cluster_group &cluster, uint32_t *h, uint32_t r, uint32_t *st) {
+    const uint32_t C = cluster.num_blocks(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (C > 1) cluster.sync();
+    else __syncthreads();
+    uint32_t own[PER], sum = 0;   // bins from the highest down
+#pragma unroll
+    for (int j = 0; j < PER; ++j) own[j] = 0;
+    for (uint32_t c = 0; c < C; ++c) {
+        const uint32_t *o = C > 1 ? cluster.map_shared_rank(h, c) : h;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) own[j] += o[PER * SEL_THREADS - 1 - (PER * tid + j)];
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) sum += own[j];
+    uint32_t x = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= (uint32_t)o) x += y;
     }
+    if (lane == 31) st[2 + warp] = x;
     __syncthreads();
-    if (lane == 31) sh[warp] = x;
-    __syncthreads();
-    uint32_t before = 0, all = 0;
+    uint32_t above = x - sum;
+    for (uint32_t w = 0; w < warp; ++w) above += st[2 + w];
 #pragma unroll
-    for (uint32_t w = 0; w < SEL_WARPS; ++w) {
-        const uint32_t t = sh[w];
-        if (w < warp) before += t;
-        all += t;
+    for (int j = 0; j < PER; ++j) {
+        if (above < r && r <= above + own[j]) { st[0] = PER * SEL_THREADS - 1 - (PER * tid + j); st[1] = above; }
+        above += own[j];
     }
-    *sum = all;
-    return before + x - v;
+    __syncthreads();
 }
 
 __global__ void __launch_bounds__(SEL_THREADS) cache_select_kernel(const SelectParams p) {
@@ -213,12 +257,12 @@ __global__ void __launch_bounds__(SEL_THREADS) cache_select_kernel(const SelectP
     const uint32_t C = cluster.num_blocks(), rank = cluster.block_rank();
     const uint32_t list = blockIdx.x / C, s = list / p.n_kv_heads % p.n_seqs;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    uint32_t *hdr = reinterpret_cast<uint32_t *>(smem);        // [0,16) scan, 16 min, 17 max, 18 bin, 19 above, 20 gt, 21 ties
-    uint32_t *hist = reinterpret_cast<uint32_t *>(smem + SEL_HDR);
-    uint32_t *keys = hist + 2 * SEL_BINS;
-    uint32_t *cnt = keys + p.chunk_max;                        // [rows of 512][warps], kept for certain; then the ties
-    const uint32_t rows_max = p.chunk_max / SEL_THREADS;
-    uint32_t *cnt_tie = cnt + rows_max * SEL_WARPS;
+    uint32_t *st = reinterpret_cast<uint32_t *>(smem);   // [0,18) hist_find, 18 list length, 19 kept in all, 20 ties in all
+    uint32_t *n_sure = st + 24, *n_tie = n_sure + SEL_WARPS;   // per warp
+    uint32_t *h0 = reinterpret_cast<uint32_t *>(smem + SEL_STATE), *h1 = h0 + SEL_BINS, *h2 = h1 + SEL_BINS2;
+    uint16_t *cand = reinterpret_cast<uint16_t *>(h2 + SEL_BINS2);
+    const uint32_t words = (p.chunk_max + 31) / 32 + SEL_WARPS;   // a bit per key, runs of whole words
+    uint32_t *w_sure = reinterpret_cast<uint32_t *>(cand + SEL_CAND), *w_tie = w_sure + words, *keys = w_tie + words;
 
     const int32_t n_in = p.n[s];
     int32_t *out = p.idx + (uint64_t)list * p.keep;
@@ -233,130 +277,145 @@ __global__ void __launch_bounds__(SEL_THREADS) cache_select_kernel(const SelectP
         for (uint32_t i = rank * SEL_THREADS + tid; i < p.keep; i += C * SEL_THREADS) out[i] = i < n ? (int32_t)i : -1;
         return;
     }
-    // n > keep >= first + recent: the scores between compete
+    // n > keep >= first + recent: the scores between compete for r places
     const uint32_t m0 = p.first, m1 = n - p.recent;
-    uint32_t r = p.keep - p.first - p.recent;                  // of them stay (0: none)
-    const uint32_t chunk = ((n + C - 1) / C + SEL_THREADS - 1) / SEL_THREADS * SEL_THREADS;
-    const uint32_t c0 = min(n, rank * chunk), c1 = min(n, c0 + chunk), len = c1 - c0;
+    uint32_t r = p.keep - p.first - p.recent;
+    const uint32_t chunk = (n + C - 1) / C, c0 = min(n, rank * chunk), len = min(n, c0 + chunk) - c0;
+    const uint32_t seg = ((len + SEL_WARPS - 1) / SEL_WARPS + 31) / 32 * 32;   // keys per warp
+    const uint32_t s0 = min(len, warp * seg), s1 = min(len, s0 + seg);
     const float *src = p.scores + (uint64_t)list * p.stride + c0;
+    const uint32_t f0 = m0 > c0 ? m0 - c0 : 0u, f1 = m1 > c0 ? m1 - c0 : 0u;   // [f0, f1) of this part compete
 
-    uint32_t kmin = 0xFFFFFFFFu, kmax = 0u;
-    for (uint32_t i = tid; i < len; i += SEL_THREADS) {
-        const uint32_t k = score_key(src[i]);
-        keys[i] = k;
-        if (c0 + i >= m0 && c0 + i < m1) { kmin = min(kmin, k); kmax = max(kmax, k); }
-    }
-    if (tid == 0) { hdr[16] = 0xFFFFFFFFu; hdr[17] = 0u; }
-    for (uint32_t i = tid; i < 2 * SEL_BINS; i += SEL_THREADS) hist[i] = 0u;
+    for (uint32_t i = tid; i < SEL_BINS + 2 * SEL_BINS2; i += SEL_THREADS) h0[i] = 0u;
+    if (tid < 24 + 2 * SEL_WARPS) st[tid] = 0u;
     __syncthreads();
-    kmin = __reduce_min_sync(0xffffffffu, kmin);
-    kmax = __reduce_max_sync(0xffffffffu, kmax);
-    if (lane == 0) { atomicMin(&hdr[16], kmin); atomicMax(&hdr[17], kmax); }
-    cluster.sync();
-    for (uint32_t c = 0; c < C; ++c) {
-        const uint32_t *h = cluster.map_shared_rank(hdr, c);
-        kmin = min(kmin, h[16]);
-        kmax = max(kmax, h[17]);
+    // groups of 32 keys: whole, all of them competing; or at an edge
+    auto whole = [&](uint32_t i0) { return i0 >= f0 && i0 + 32 <= f1 && i0 + 32 <= s1; };
+    // 1. keys and their top 12 bits
+    for (uint32_t i0 = s0; i0 < s1; i0 += 32 * SEL_U) {
+        float v[SEL_U];
+#pragma unroll
+        for (int u = 0; u < SEL_U; ++u) v[u] = i0 + 32 * u + lane < s1 ? __ldcs(src + i0 + 32 * u + lane) : 0.f;
+#pragma unroll
+        for (int u = 0; u < SEL_U; ++u) {
+            const uint32_t g0 = i0 + 32 * u, i = g0 + lane, k = score_key(v[u]);
+            if (g0 >= s1) break;
+            if (whole(g0)) {
+                keys[i] = k;
+                hist_add(h0, k >> 20);
+            } else {
+                if (i < s1) keys[i] = k;
+                hist_add(h0, i < s1 && i >= f0 && i < f1 ? k >> 20 : 0xFFFFFFFFu);
+            }
+        }
     }
-    // narrow [lo, lo + 2^bits) to one key
-    uint32_t lo = kmin, T = 0xFFFFFFFFu, need = 0;
+    uint32_t T = 0xFFFFFFFFu, need = 0;   // kept: above T, and the first `need` equal to T
+    uint32_t b0 = SEL_BINS;               // r 0: nothing of them is kept
     if (r) {
-        uint32_t bits = kmax > kmin ? 32 - __clz(kmax - kmin) : 0;
-        for (uint32_t pass = 0;; ++pass) {
-            const uint32_t shift = bits > 11 ? bits - 11 : 0;
-            uint32_t *h = hist + (pass & 1) * SEL_BINS;
-            for (uint32_t i0 = 0; i0 < len; i0 += SEL_THREADS) {   // whole warps: the ballot needs all lanes
-                const uint32_t i = i0 + tid, at = c0 + i;
-                uint32_t bin = 0xFFFFFFFFu;
-                if (i < len && at >= m0 && at < m1) {
-                    const uint32_t d = keys[i] - lo;
-                    if (keys[i] >= lo && (bits == 32 || (d >> bits) == 0)) bin = d >> shift;
-                }
-                // the lowest bin is where equal scores gather: one add per warp
-                const uint32_t low = __ballot_sync(0xffffffffu, bin == 0);
-                if (bin == 0) {
-                    if (lane == (uint32_t)__ffs(low) - 1) atomicAdd(&h[0], (uint32_t)__popc(low));
-                } else if (bin < SEL_BINS) {
-                    atomicAdd(&h[bin], 1u);
-                }
-            }
-            cluster.sync();
-            uint32_t own[4], sum4 = 0;   // bins from the highest down, 4 per thread
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t b = SEL_BINS - 1 - (4 * tid + j);
-                own[j] = 0;
-                for (uint32_t c = 0; c < C; ++c) own[j] += cluster.map_shared_rank(h, c)[b];
-                sum4 += own[j];
-            }
-            uint32_t all;
-            uint32_t above = block_scan(sum4, hdr, &all);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (above < r && r <= above + own[j]) { hdr[18] = SEL_BINS - 1 - (4 * tid + j); hdr[19] = above; }
-                above += own[j];
-            }
-            // every CTA of the cluster has read the other buffer by now
-            for (uint32_t i = tid; i < SEL_BINS; i += SEL_THREADS) hist[((pass + 1) & 1) * SEL_BINS + i] = 0u;
-            __syncthreads();
-            lo += hdr[18] << shift;
-            r -= hdr[19];
-            bits = shift;
-            if (!shift) break;
-        }
-        T = lo;
-        need = r;
+        hist_find<SEL_BINS / SEL_THREADS>(cluster, h0, r, st);
+        b0 = st[0];
+        r -= st[1];
     }
-    // counts per row of 512 and warp: above T (or always kept), and equal to T
-    const uint32_t rows = (len + SEL_THREADS - 1) / SEL_THREADS, ents = rows * SEL_WARPS;
-    auto kind = [&](uint32_t i) -> int {   // 0 dropped, 1 kept, 2 tied
-        if (i >= len) return 0;
-        const uint32_t at = c0 + i;
-        if (at < m0 || at >= m1) return 1;
-        if (!need) return 0;
-        return keys[i] > T ? 1 : (keys[i] == T ? 2 : 0);
-    };
-    for (uint32_t k = 0; k < rows; ++k) {
-        const int kd = kind(k * SEL_THREADS + tid);
-        const uint32_t b1 = __ballot_sync(0xffffffffu, kd == 1), b2 = __ballot_sync(0xffffffffu, kd == 2);
-        if (lane == 0) { cnt[k * SEL_WARPS + warp] = __popc(b1); cnt_tie[k * SEL_WARPS + warp] = __popc(b2); }
+    // 2. above the bin (or not competing): a bit; in it: listed
+    const uint32_t below = (1u << lane) - 1, k_hi = b0 >= SEL_BINS - 1 ? 0xFFFFFFFFu : ((b0 + 1) << 20) - 1;   // the bin's highest key
+    for (uint32_t i0 = s0; i0 < s1; i0 += 32) {
+        const uint32_t i = i0 + lane;
+        bool sure, in;
+        if (whole(i0)) {
+            const uint32_t k = keys[i];
+            sure = k > k_hi;
+            in = (k >> 20) == b0;
+        } else {
+            const bool comp = i >= f0 && i < f1;
+            const uint32_t k = i < s1 ? keys[i] : 0u;
+            sure = i < s1 && (!comp || k > k_hi);
+            in = i < s1 && comp && (k >> 20) == b0;
+        }
+        const uint32_t m = __ballot_sync(0xffffffffu, in), g = __ballot_sync(0xffffffffu, sure);
+        if (lane == 0) { w_sure[i0 >> 5] = g; w_tie[i0 >> 5] = 0u; }
+        if (m) {
+            uint32_t at = 0;
+            if (lane == 0) at = atomicAdd(&st[18], (uint32_t)__popc(m));
+            at = __shfl_sync(0xffffffffu, at, 0) + __popc(m & below);
+            if (in && at < SEL_CAND) cand[at] = (uint16_t)i;
+        }
     }
     __syncthreads();
-    const uint32_t per = (ents + SEL_THREADS - 1) / SEL_THREADS;   // consecutive entries per thread, at most 3
-    uint32_t s1 = 0, s2 = 0;
-    for (uint32_t j = 0; j < per; ++j) {
-        const uint32_t e = tid * per + j;
-        if (e < ents) { s1 += cnt[e]; s2 += cnt_tie[e]; }
-    }
-    uint32_t all1, all2;
-    uint32_t b1 = block_scan(s1, hdr, &all1), b2 = block_scan(s2, hdr, &all2);
-    for (uint32_t j = 0; j < per; ++j) {
-        const uint32_t e = tid * per + j;
-        if (e < ents) {
-            const uint32_t x1 = cnt[e], x2 = cnt_tie[e];
-            cnt[e] = b1;
-            cnt_tie[e] = b2;
-            b1 += x1;
-            b2 += x2;
+    const uint32_t nc = st[18];
+    const bool listed = nc <= SEL_CAND;
+    // the keys of the bin, from the list or in place; whole warps call f
+    auto each = [&](auto f) {
+        if (listed) {
+            for (uint32_t j0 = warp * 32; j0 < nc; j0 += SEL_THREADS) {
+                const uint32_t j = j0 + lane, i = j < nc ? cand[j] : 0u;
+                f(j < nc, i, j < nc ? keys[i] : 0u);
+            }
+        } else {
+            for (uint32_t i0 = s0; i0 < s1; i0 += 32) {
+                const uint32_t i = i0 + lane, k = i < s1 ? keys[i] : 0u;
+                f(i < s1 && i >= f0 && i < f1 && k >> 20 == b0, i, k);
+            }
         }
+    };
+    if (r) {
+        each([&](bool c, uint32_t, uint32_t k) { hist_add(h1, c ? (k >> 10) & 1023u : 0xFFFFFFFFu); });
+        hist_find<SEL_BINS2 / SEL_THREADS>(cluster, h1, r, st);
+        const uint32_t b1 = st[0];
+        r -= st[1];
+        each([&](bool c, uint32_t, uint32_t k) { hist_add(h2, c && ((k >> 10) & 1023u) == b1 ? k & 1023u : 0xFFFFFFFFu); });
+        hist_find<SEL_BINS2 / SEL_THREADS>(cluster, h2, r, st);
+        T = (b0 << 20) | (b1 << 10) | st[0];
+        need = r - st[1];
+        each([&](bool c, uint32_t i, uint32_t k) {
+            if (c && k >= T) atomicOr(k > T ? &w_sure[i >> 5] : &w_tie[i >> 5], 1u << (i & 31));
+        });
     }
-    if (tid == 0) { hdr[20] = all1; hdr[21] = all2; }
-    cluster.sync();
-    uint32_t o1 = 0, o2 = 0;
+    __syncthreads();
+    // what each warp's run keeps for certain, and its ties
+    uint32_t at = 0, ties = 0;
+    for (uint32_t g = s0 / 32 + lane; g < (s1 + 31) / 32; g += 32) {
+        at += __popc(w_sure[g]);
+        ties += __popc(w_tie[g]);
+    }
+    at = __reduce_add_sync(0xffffffffu, at);
+    ties = __reduce_add_sync(0xffffffffu, ties);
+    if (lane == 0) {
+        n_sure[warp] = at;
+        n_tie[warp] = ties;
+    }
+    if (C > 1) {
+        if (lane == 0) {
+            atomicAdd(&st[19], at);
+            atomicAdd(&st[20], ties);
+        }
+        cluster.sync();
+    } else {
+        __syncthreads();
+    }
+    at = ties = 0;   // before this warp's run
     for (uint32_t c = 0; c < rank; ++c) {
-        const uint32_t *h = cluster.map_shared_rank(hdr, c);
-        o1 += h[20];
-        o2 += h[21];
+        const uint32_t *o = cluster.map_shared_rank(st, c);
+        at += o[19];
+        ties += o[20];
     }
-    const uint32_t below = (1u << lane) - 1;
-    for (uint32_t k = 0; k < rows; ++k) {
-        const uint32_t i = k * SEL_THREADS + tid;
-        const int kd = kind(i);
-        const uint32_t g1 = __ballot_sync(0xffffffffu, kd == 1), g2 = __ballot_sync(0xffffffffu, kd == 2);
-        const uint32_t r1 = o1 + cnt[k * SEL_WARPS + warp] + __popc(g1 & below);
-        const uint32_t r2 = o2 + cnt_tie[k * SEL_WARPS + warp] + __popc(g2 & below);
-        if (kd == 1 || (kd == 2 && r2 < need)) out[r1 + min(r2, need)] = (int32_t)(c0 + i);   // n > keep: all places get filled
+    for (uint32_t w = 0; w < warp; ++w) {
+        at += n_sure[w];
+        ties += n_tie[w];
     }
+    // 3. out: n > keep, so all places get filled
+    at += min(ties, need);
+    for (uint32_t i0 = s0; i0 < s1; i0 += 32) {
+        uint32_t g = w_sure[i0 >> 5];
+        const uint32_t e = w_tie[i0 >> 5];
+        if (e && ties < need) {   // the first of them, up to `need`
+            const bool mine = ((e >> lane) & 1u) && ties + __popc(e & below) < need;
+            g |= __ballot_sync(0xffffffffu, mine);
+        }
+        ties += __popc(e);
+        if ((g >> lane) & 1u) out[at + __popc(g & below)] = (int32_t)(c0 + i0 + lane);
+        at += __popc(g);
+    }
+    if (C == 1) return;
     cluster.sync();   // nobody leaves while its shared memory is read
 }
 
@@ -366,9 +425,11 @@ __global__ void __launch_bounds__(SEL_THREADS) cache_select_kernel(const SelectP
 // before the first store. In place: rows only move down, so a CTA takes its
 // list in ascending batches (all of a batch's loads, a barrier, its stores);
 // the pieces of a row are independent of one another, so slices of the row
-// go to CTAs of their own.
+// go to CTAs of their own. Lists of up to GA_WARP_MAX entries (an accepted
+// branch) take a warp each: 2048 lists of 5 rows of 256 bytes 9.7 us with a
+// CTA per list.
 // ---------------------------------------------------------------------------
-constexpr uint32_t GA_THREADS = 256, GA_U = 4;
+constexpr uint32_t GA_THREADS = 256, GA_U = 4, GA_WARP_MAX = 64;
 
 struct GatherSide {
     uint16_t *k, *v;
@@ -403,17 +464,20 @@ __device__ __forceinline__ bool gather_list(const GatherParams &p, uint32_t list
     l.aux_s = (uint64_t)list * p.src.max_ctx;
     l.aux_d = (uint64_t)list * p.dst.max_ctx;
     if (n < 0 || (uint32_t)n > p.g.n_max || l.dst0 < 0 || l.dst0 + n > (int64_t)p.dst.max_ctx) {
-        if (threadIdx.x == 0) dev_flag_error(p.err, DERR_BAD_ARG);
+        if ((threadIdx.x & 31) == 0) dev_flag_error(p.err, DERR_BAD_ARG);
         return false;
     }
     return true;
 }
 
 __global__ void __launch_bounds__(GA_THREADS) gather_apart_kernel(const __grid_constant__ GatherParams p, uint32_t nblk) {
-    const uint32_t list = blockIdx.x / nblk, rp = GA_THREADS / p.cpr;
+    // the heads of the same rows are neighbours in launch order: in the
+    // engine's order their rows are neighbours in memory
+    const uint32_t h = blockIdx.x % p.n_kv_heads, x = blockIdx.x / p.n_kv_heads;
+    const uint32_t list = x / nblk * p.n_kv_heads + h, rp = GA_THREADS / p.cpr;
     GatherList l;
     if (!gather_list(p, list, l)) return;
-    const uint32_t ch = threadIdx.x % p.cpr, r0 = blockIdx.x % nblk * (rp * GA_U) + threadIdx.x / p.cpr;
+    const uint32_t ch = threadIdx.x % p.cpr, r0 = x % nblk * (rp * GA_U) + threadIdx.x / p.cpr;
     if (threadIdx.x >= rp * p.cpr) return;
     int64_t from[GA_U];
     uint4 k[GA_U], v[GA_U];
@@ -500,9 +564,58 @@ __global__ void __launch_bounds__(GA_THREADS) gather_inplace_kernel(const __grid
     }
 }
 
+// In place, short lists: a warp per list, pieces of K and V in ascending rows,
+// 8 per lane at a time.
+__global__ void __launch_bounds__(GA_THREADS) gather_inplace_warp_kernel(const __grid_constant__ GatherParams p, uint32_t lists) {
+    const uint32_t list = blockIdx.x * (GA_THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    GatherList l;
+    if (list >= lists || !gather_list(p, list, l)) return;
+    bool bad = false;
+    for (uint32_t i = lane; i < l.n; i += 32) {
+        const int64_t f = l.src0 + l.idx[i];
+        bad |= f < l.dst0 + i || f >= (int64_t)p.src.max_ctx || (i && l.idx[i] <= l.idx[i - 1]);
+    }
+    if (__any_sync(0xffffffffu, bad)) {
+        if (lane == 0) dev_flag_error(p.err, DERR_BAD_ARG);
+        return;
+    }
+    const uint32_t per = 2 * p.cpr, total = l.n * per;   // pieces: row, then K's and V's
+    for (uint32_t k0 = 0; k0 < total; k0 += 32 * 8) {
+        uint4 v[8];
+        float w[8];
+        int32_t ps[8];
+        int64_t from[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const uint32_t k = k0 + 32 * u + lane, i = k / per, c = k - i * per;
+            from[u] = k < total ? l.src0 + l.idx[i] : -1;
+            if (from[u] == l.dst0 + i) from[u] = -1;   // stays where it is
+            if (from[u] < 0) continue;
+            const uint64_t o = l.so + (uint64_t)from[u] * p.src.pos_step;
+            v[u] = *reinterpret_cast<const uint4 *>((c < p.cpr ? p.src.k + o + c * 8 : p.src.v + o + (c - p.cpr) * 8));
+            if (c == 0) {
+                if (p.g.weights_dst) w[u] = p.g.weights_src[l.aux_s + from[u]];
+                if (p.g.pos_dst) ps[u] = p.g.pos_src[l.aux_s + from[u]];
+            }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            if (from[u] < 0) continue;
+            const uint32_t k = k0 + 32 * u + lane, i = k / per, c = k - i * per;
+            const uint64_t to = (uint64_t)l.dst0 + i, o = l.dof + to * p.dst.pos_step;
+            *reinterpret_cast<uint4 *>((c < p.cpr ? p.dst.k + o + c * 8 : p.dst.v + o + (c - p.cpr) * 8)) = v[u];
+            if (c == 0) {
+                if (p.g.weights_dst) p.g.weights_dst[l.aux_d + to] = w[u];
+                if (p.g.pos_dst) p.g.pos_dst[l.aux_d + to] = ps[u];
+            }
+        }
+    }
+}
+
 cudaError_t slots_configure() {
     return cudaFuncSetAttribute(cache_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)(SEL_HDR + (2 * SEL_BINS + SEL_CHUNK_MAX + 2 * (SEL_CHUNK_MAX / 32)) * 4));
+                                (int)(SEL_FIXED + sel_keys_bytes(SEL_CHUNK_MAX)));
 }
 
 static GatherSide gather_side(const vbs_cu_kv_t *kv) {
@@ -642,18 +755,18 @@ int vbs_cu_cache_select(const float *scores, uint64_t stride, uint32_t n_layers,
     }
     DevState *d = backend_current();
     if (!d) { latch_error("vbs_cu_cache_select: no usable device"); return -1; }
-    // CTAs per list: as many as the SMs have room for, 2048 scores each at
+    // CTAs per list: as many as the SMs have room for, 4096 scores each at
     // least; more where a list does not fit one CTA's shared memory
     uint32_t c = 1;
-    while (c < 8 && (n_limit > c * SEL_CHUNK_MAX || (lists * c * 2 <= (uint64_t)d->n_sm && n_limit > c * 2048u))) c *= 2;
+    while (c < 8 && (n_limit > c * SEL_CHUNK_MAX || (lists * c * 2 <= (uint64_t)d->n_sm && n_limit > c * 4096u))) c *= 2;
     SelectParams p = {};
     p.scores = scores; p.stride = stride; p.n_seqs = n_seqs; p.n_kv_heads = n_kv_heads; p.n_limit = n_limit;
     p.keep = keep; p.first = first; p.recent = recent; p.n = n; p.idx = idx; p.count = count; p.err = d->err;
-    p.chunk_max = std::max(1u, ((n_limit + c - 1) / c + SEL_THREADS - 1) / SEL_THREADS) * SEL_THREADS;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(lists * c));
     cfg.blockDim = dim3(SEL_THREADS);
-    cfg.dynamicSmemBytes = SEL_HDR + (2 * SEL_BINS + p.chunk_max + 2 * (p.chunk_max / 32)) * 4;
+    p.chunk_max = (n_limit + c - 1) / c;
+    cfg.dynamicSmemBytes = SEL_FIXED + sel_keys_bytes(p.chunk_max);
     cfg.stream = static_cast<cudaStream_t>(stream);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -700,7 +813,10 @@ int vbs_cu_cache_gather(const vbs_cu_kv_t *src, const vbs_cu_kv_t *dst, const vb
     p.err = d->err;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     note_launches(1);
-    if (same) {
+    if (same && g->n_max <= GA_WARP_MAX) {
+        const uint32_t per = GA_THREADS / 32;
+        gather_inplace_warp_kernel<<<(unsigned)((lists + per - 1) / per), GA_THREADS, 0, st>>>(p, (uint32_t)lists);
+    } else if (same) {
         // slices of at least 64 bytes, as many as cover the SMs four times
         const uint32_t want = (uint32_t)std::min<uint64_t>(8, ((uint64_t)d->n_sm * 4 + lists - 1) / lists);
         p.slice = std::max(std::min(4u, p.cpr), (p.cpr + want - 1) / want);

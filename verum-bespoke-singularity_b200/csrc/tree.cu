@@ -386,14 +386,60 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
 }
 
 // ---------------------------------------------------------------------------
-// Join of the parts: one CTA per row. The parts' maxima and sums are read at
+// Join of the parts. Few rows, or more than 32 parts: one CTA per row. The parts' maxima and sums are read at
 // once and become their factors in shared memory; then the warps share the
 // parts, TREE_MU loads in flight each, and their sums are added in order.
-// Launched as a programmatic dependent of the kernel that writes the parts:
-// it is on the SMs when that one ends.
+// Both are launched as programmatic dependents of the kernel that writes the
+// parts: they are on the SMs when that one ends.
 // ---------------------------------------------------------------------------
 constexpr int TREE_MW = 8, TREE_MU = 8;
 constexpr uint32_t TREE_MAX_PARTS = 1024;
+
+// Many rows of up to 32 parts: a warp per row, a lane per part for the factors, TREE_MU
+// parts' loads in flight. (A CTA per row took 22 us for 4032 rows of 8 parts.)
+__global__ void __launch_bounds__(TREE_MW * 32) tree_merge_warp_kernel(const __grid_constant__ TreeParams p, uint32_t tile_rows) {
+    const uint32_t r = blockIdx.x * TREE_MW + (threadIdx.x >> 5), kvh = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31;
+    uint32_t nc, nt;
+    const bool live = tree_lengths(p, b, nc, nt) && r < nt * p.G;
+    pdl_wait();
+    pdl_launch_dependents();
+    if (!live) return;
+    const uint32_t tile = r / tile_rows, ri = r - tile * tile_rows, ns = p.n_splits;
+    const uint64_t slot = (uint64_t)(b * p.nkh + kvh) * p.row_tiles + tile;
+    const float *po = p.part_o + (slot * ns * tile_rows + ri) * p.hd;
+    const float2 x = lane < ns ? __ldcg(p.part_ml + (slot * ns + lane) * tile_rows + ri) : make_float2(-INFINITY, 0.f);
+    const float M = warp_max(x.x);
+    const bool has = !(x.y == 0.f);   // an empty part has no sums (and wrote none); a NaN goes through
+    const float f = has ? ex2(x.x - M) : 0.f;
+    const float L = warp_sum(has ? x.y * f : 0.f);
+    const uint32_t parts = __ballot_sync(0xffffffffu, has);
+    const float il = L == 0.f ? 0.f : 1.f / L;
+    const uint32_t tok = tree_token(p, r), q4 = p.hd / 4;
+    float *out = p.out + (((uint64_t)b * p.n_tokens + tok) * p.nqh + kvh * p.G + (r - tok * p.G)) * p.hd;
+    for (uint32_t d0 = 0; d0 < q4; d0 += 32) {   // wider rows take two rounds
+        const uint32_t d = d0 + lane;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (uint32_t s0 = 0; s0 < ns; s0 += TREE_MU) {
+            float4 v[TREE_MU];
+#pragma unroll
+            for (int u = 0; u < TREE_MU; ++u)
+                v[u] = ((parts >> ((s0 + u) & 31)) & 1u) && s0 + u < ns && d < q4
+                           ? __ldcg(reinterpret_cast<const float4 *>(po + (uint64_t)(s0 + u) * tile_rows * p.hd) + d)
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int u = 0; u < TREE_MU; ++u) {
+                const float g = __shfl_sync(0xffffffffu, f, (s0 + u) & 31);
+                a.x = fmaf(v[u].x, g, a.x); a.y = fmaf(v[u].y, g, a.y);
+                a.z = fmaf(v[u].z, g, a.z); a.w = fmaf(v[u].w, g, a.w);
+            }
+        }
+        if (L == 0.f) a = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (d < q4) reinterpret_cast<float4 *>(out)[d] = make_float4(a.x * il, a.y * il, a.z * il, a.w * il);
+    }
+    if (p.lse && lane == 0)
+        p.lse[(uint64_t)(b * p.nkh + kvh) * (p.n_tokens * p.G) + r] = L == 0.f ? -INFINITY : M + log2f(L);
+}
 
 __global__ void __launch_bounds__(TREE_MW * 32) tree_merge_kernel(const __grid_constant__ TreeParams p, uint32_t tile_rows) {
     __shared__ float fac[TREE_MAX_PARTS];
@@ -546,17 +592,19 @@ static cudaError_t tree_map(CUtensorMap *m, const uint16_t *base, const vbs_cu_k
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-static cudaError_t tree_merge_launch(const TreeParams &p, dim3 grid, uint32_t tile_rows, cudaStream_t st) {
+static cudaError_t tree_merge_launch(const TreeParams &p, uint32_t rows, uint32_t n_seqs, uint32_t tile_rows, uint32_t n_sm, cudaStream_t st) {
+    // a CTA per row while they all fit the SMs at once (8 each): shorter; a warp per row behind that
+    const bool few = p.n_splits <= 32 && (uint64_t)rows * p.nkh * n_seqs > 8u * n_sm;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
+    cfg.gridDim = dim3(few ? (rows + TREE_MW - 1) / TREE_MW : rows, p.nkh, n_seqs);
     cfg.blockDim = dim3(TREE_MW * 32);
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, tree_merge_kernel, p, tile_rows);
+    return few ? cudaLaunchKernelEx(&cfg, tree_merge_warp_kernel, p, tile_rows) : cudaLaunchKernelEx(&cfg, tree_merge_kernel, p, tile_rows);
 }
 
 template <int HD, int WR, int WP> static cudaError_t tree_go(const TreeParams &p, dim3 grid, cudaStream_t st) {
@@ -591,6 +639,7 @@ cudaError_t tree_configure() {
     // the join takes the attention kernels' split of shared memory and L1:
     // changing it costs an SM several microseconds between kernels
     if (e == cudaSuccess) e = cudaFuncSetAttribute(tree_merge_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(tree_merge_warp_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
     return e;
 }
 
@@ -657,7 +706,7 @@ int vbs_cu_attention_tree(const vbs_cu_kv_t *kv, uint32_t layer, const vbs_cu_tr
                     : kv->head_dim <= 64 ? tree_go_rows<64>(p, wr, grid, st)
                                        : (kv->head_dim <= 128 ? tree_go_rows<128>(p, wr, grid, st) : tree_go_rows<256>(p, wr, grid, st));
     if (e == cudaSuccess && pl.n_splits > 1)
-        e = tree_merge_launch(p, dim3(pl.rows, kv->n_kv_heads, kv->n_seqs), pl.tile_rows, st);
+        e = tree_merge_launch(p, pl.rows, kv->n_seqs, pl.tile_rows, d->n_sm, st);
     if (e == cudaSuccess && t->weights_out) e = tree_weights_launch(p, km, kv->n_seqs, d->n_sm, st);
     return cuda_ok(e, "attention_tree") ? 0 : -1;
 }

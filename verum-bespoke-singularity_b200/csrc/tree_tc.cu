@@ -63,11 +63,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
     float *fac_sm = reinterpret_cast<float *>(hs + H_FAC);
 
     // the queries start on their way before anything else is known
-    TcQ<128> q0, q1;
-    if (warp < TC_LOADER) {
-        tc_q_load(p, R0 + 16 * warp + (lane & 7), kvh, b, q0);
-        tc_q_load(p, R0 + 16 * warp + 8 + (lane & 7), kvh, b, q1);
-    }
+    TcQ<128> q;
+    if (warp < TC_LOADER) tc_q_load(p, R0 + 16 * warp + (lane & 7), kvh, b, q);
     pdl_launch_dependents();
     uint32_t nc, nt;
     if (!tree_lengths(p, b, nc, nt) || R0 >= nt * p.G) return;
@@ -134,18 +131,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
         hi = __reduce_max_sync(0xffffffffu, hi);
         if (lane == 0) *reinterpret_cast<int32_t *>(hs + H_QMAX) = hi;
     } else {
-        for (uint32_t x = 0;; ++x) {   // 128 rows, dual twice
-            uint8_t *at = smem + tp.q_off + x * q_bytes;
-            const uint32_t r = 16 * warp + (lane & 7);
-            const float g0 = tc_q_store(p, q0, at, TREE_TC_ROWS * 16, q_bytes / 2, r, chunks);
-            const float g1 = tc_q_store(p, q1, at, TREE_TC_ROWS * 16, q_bytes / 2, r + 8, chunks);
-            if (lane < 8) {
-                fac_sm[x * TREE_TC_ROWS + r] = g0;
-                fac_sm[x * TREE_TC_ROWS + r + 8] = g1;
-            }
-            if (x == two) break;
-            tc_q_load(p, R0 + TREE_TC_ROWS + 16 * warp + (lane & 7), kvh, b, q0);
-            tc_q_load(p, R0 + TREE_TC_ROWS + 16 * warp + 8 + (lane & 7), kvh, b, q1);
+        // 8 rows at a time, two times 8 per warp and 128 rows
+#pragma unroll 1
+        for (uint32_t g = 0; g < (two ? 4u : 2u); ++g) {
+            const uint32_t r = 16 * warp + 8 * (g & 1) + (lane & 7), x = g >> 1;
+            TcQ<128> next;
+            tc_q_load(p, R0 + TREE_TC_ROWS * ((g + 1) >> 1) + 16 * warp + 8 * ((g + 1) & 1) + (lane & 7), kvh, b, next);
+            const float f = tc_q_store(p, q, smem + tp.q_off + x * q_bytes, TREE_TC_ROWS * 16, q_bytes / 2, r, chunks);
+            if (lane < 8) fac_sm[x * TREE_TC_ROWS + r] = f;
+            q = next;
         }
         tc_proxy();
     }
@@ -244,11 +238,32 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
         // the threads that look at one tile's values together: a stream, or
         // both where they share the tiles
         const uint32_t bar = two ? 2 : 2 + w, bar_n = 32 * (two ? aw0 + aw1 : aw), bar_r = r + (two && w ? 32 * aw0 : 0u);
+        // the lane's key positions of the next tile
+        const uint32_t tstep = two ? TREE_TC_SP : 2 * TREE_TC_SP;
+        uint32_t tn = t0 + (two ? 0u : w * TREE_TC_SP);
+        int32_t kn[4] = {0, 0, 0, 0};
+        if (kpos && active && tn + TREE_TC_SP <= min(nc, t1)) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) kn[k] = kpos[tn + 32 * k + lane];
+        }
+        tn += tstep;
         for (uint32_t n = active ? w : steps; n < steps; n += 2) {
             const uint32_t i = two ? n >> 1 : n, tb = t0 + i * TREE_TC_SP;
             const int nval = (int)min(TREE_TC_SP, t1 - tb);
-            // every row of the tile sees all of its positions
-            const bool whole = tb + TREE_TC_SP <= min(nc, t1) && !kpos && (!p.window || qmax - (int32_t)tb < (int32_t)p.window);
+            // every row of the tile sees all of its positions: by the lowest
+            // key position of the tile, negative for a hole
+            int32_t low = (int32_t)tb;
+            const bool context = tb + TREE_TC_SP <= min(nc, t1);
+            if (kpos && context) {
+                low = min(min(kn[0], kn[1]), min(kn[2], kn[3]));
+                low = __reduce_min_sync(0xffffffffu, low);
+            }
+            if (kpos && tn + TREE_TC_SP <= nc) {   // the next tile's, ahead
+#pragma unroll
+                for (int k = 0; k < 4; ++k) kn[k] = kpos[tn + 32 * k + lane];
+            }
+            tn += tstep;
+            const bool whole = context && low >= 0 && (!p.window || qmax - low < (int32_t)p.window);
             dead = dead || !all(!*bad && waits(base + H_S + 8 * w, (n >> 1) & 1u));
             if (dead) {   // a wait ran out: only the barriers are kept company
                 if (!whole && bar_or(bar, bar_n, false) && bar_or(bar, bar_n, false))
@@ -256,7 +271,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                 continue;
             }
             tc_after();
-            const bool plain = whole && !p.slopes && !(p.cap > 0.f);
+            // plain: the scores as the product left them, times the row's
+            // factor, plus (linear) slope * (slot - query position)
+            const bool linear = p.slopes && !kpos, plain = whole && (!p.slopes || linear) && !(p.cap > 0.f);
+            const float lin0 = (float)((int32_t)tb - qp);
             float mx = -INFINITY;
             if (plain) {
                 uint32_t s[2][32];
@@ -265,64 +283,68 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     if (c < 3) tc_ld32(sa + 32 * (c + 1), s[(c + 1) & 1]);
+                    if (linear) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            s[c & 1][e] = __float_as_uint(fmaf(slope, lin0 + (float)(32 * c + e), __uint_as_float(s[c & 1][e]) * fac));
+                    }
                     mx = fmaxf(mx, max32(s[c & 1]));
                     if (c < 3) tc_wait_ld(s[(c + 1) & 1]);
                 }
-                mx *= fac;
+                if (!linear) mx *= fac;
             } else {
-                // scores as the formula has them, back into tensor memory;
-                // `see`: bit e, this row sees position tb + 32 c + e
+                // scores as the formula has them, back into tensor memory, 8 at
+                // a time (short code: it runs for few tiles, out of cold
+                // instruction caches)
                 const bool by_slot = !kpos && tb + TREE_TC_SP <= nc;   // the tile's positions are its slots
                 const float cap2 = p.cap * TREE_LOG2E;
                 bool hidden = (nval & 15) != 0;                        // stale rows behind the end in the last product
+                uint32_t see = 0;     // bit e: this row sees the e-th next position
+                int32_t kp = 0;       // key position of slot (32's first + lane), handed round where rows need them
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    const uint32_t t = tb + 32 * c;
-                    uint32_t s[32];
-                    tc_ld32(sa + 32 * c, s);
-                    const uint32_t inside = ones(nval - 32 * c);
-                    uint32_t see = on ? tree_sees(p, b, tok, t, nc, nval - 32 * c) : inside;
-                    // lane's key position of this 32, handed round where rows need them
-                    int32_t kp = (int32_t)t + lane;
-                    if (!by_slot && (kpos || p.window || p.slopes) && lane < nval - 32 * c) kp = tree_kpos(p, kpos, b, t + lane, nc);
-                    if (by_slot) {
-                        if (p.window) see &= ~ones(qp - (int32_t)p.window + 1 - (int32_t)t);
-                    } else if (p.window || __any_sync(0xffffffffu, kpos && kp < 0)) {
-                        uint32_t in = __ballot_sync(0xffffffffu, !kpos || kp >= 0);
-                        if (p.window) {
-#pragma unroll 8
-                            for (int e = 0; e < 32; ++e)
-                                if (qp - __shfl_sync(0xffffffffu, kp, e) >= (int32_t)p.window) in &= ~(1u << e);
+                for (int c = 0; c < 16; ++c) {
+                    const uint32_t t = tb + 8 * c;
+                    uint32_t x[8];
+                    tc_ld8(sa + 8 * c, x);
+                    if (!(c & 3)) {
+                        const uint32_t inside = ones(nval - 8 * c);
+                        see = on ? tree_sees(p, b, tok, t, nc, nval - 8 * c) : inside;
+                        kp = (int32_t)t + lane;
+                        if (!by_slot && (kpos || p.window || p.slopes) && lane < nval - 8 * c) kp = tree_kpos(p, kpos, b, t + lane, nc);
+                        if (by_slot) {
+                            if (p.window) see &= ~ones(qp - (int32_t)p.window + 1 - (int32_t)t);
+                        } else {
+                            if (kpos) see &= __ballot_sync(0xffffffffu, kp >= 0);
+                            if (p.window) {
+#pragma unroll 4
+                                for (int e = 0; e < 32; ++e)
+                                    if (qp - __shfl_sync(0xffffffffu, kp, e) >= (int32_t)p.window) see &= ~(1u << e);
+                            }
                         }
-                        see &= in;
+                        hidden |= on && see != inside;
                     }
-                    hidden |= on && see != inside;
-                    tc_wait_ld(s);
+                    tc_wait_ld(x);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * fac);
+                    for (int e = 0; e < 8; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * fac);
                     if (p.cap > 0.f) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(tree_cap(__uint_as_float(s[e]), cap2));
+                        for (int e = 0; e < 8; ++e) x[e] = __float_as_uint(tree_cap(__uint_as_float(x[e]), cap2));
                     }
                     if (p.slopes) {
-                        if (by_slot) {
-                            const float d = (float)((int32_t)t - qp);
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(fmaf(slope, d + (float)e, __uint_as_float(s[e])));
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                s[e] = __float_as_uint(fmaf(slope, (float)(__shfl_sync(0xffffffffu, kp, e) - qp), __uint_as_float(s[e])));
+                        for (int e = 0; e < 8; ++e) {
+                            const int32_t k = by_slot ? (int32_t)t + e : __shfl_sync(0xffffffffu, kp, 8 * (c & 3) + e);
+                            x[e] = __float_as_uint(fmaf(slope, (float)(k - qp), __uint_as_float(x[e])));
                         }
                     }
-                    if (see != 0xFFFFFFFFu) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (!((see >> e) & 1u)) s[e] = 0xFF800000u;
+                    for (int e = 0; e < 8; ++e) {
+                        if (!((see >> e) & 1u)) x[e] = 0xFF800000u;
+                        mx = fmaxf(mx, __uint_as_float(x[e]));
                     }
+                    see >>= 8;
                     __syncwarp();
-                    mx = fmaxf(mx, max32(s));
-                    tc_st32(sa + 32 * c, s);
+                    tc_st8(sa + 8 * c, x);
                 }
                 tc_wait_st();
                 if (!whole && bar_or(bar, bar_n, hidden)) {
@@ -331,9 +353,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                     const uint32_t vx = 2 * i + 1, va = stage0 + (vx % tp.ns) * slot;
                     const bool here = waits(base + H_FULL + 8 * (vx % tp.ns), (vx / tp.ns) & 1u);
                     bool odd = false;
-                    for (uint32_t k = bar_r; here && k < slot / 16; k += bar_n) {
-                        const uint4 v = lds_u128(va + k * 16);
-                        odd |= not_finite2(v.x) || not_finite2(v.y) || not_finite2(v.z) || not_finite2(v.w);
+                    if (here) {
+#pragma unroll 8
+                        for (uint32_t k = bar_r; k < slot / 16; k += bar_n) {
+                            const uint4 v = *reinterpret_cast<const uint4 *>(smem + (vx % tp.ns) * slot + k * 16);
+                            odd |= not_finite2(v.x) | not_finite2(v.y) | not_finite2(v.z) | not_finite2(v.w);
+                        }
                     }
                     if (bar_or(bar, bar_n, odd)) {
                         // rare: the rows that see such values add them here,
@@ -402,7 +427,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                     }
                 }
             }
-            const float f1 = plain ? fac : 1.f, b1 = mref == -INFINITY ? 0.f : mref;
+            const float f1 = plain && !linear ? fac : 1.f, b1 = mref == -INFINITY ? 0.f : mref;
             const float2 f = make_float2(f1, f1), bs = make_float2(-b1, -b1);
             uint32_t s[2][16];
             tc_ld16(sa, s[0]);
@@ -415,6 +440,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                 for (int u = 0; u < 2; ++u) {
                     if (c < 3 || !u) tc_ld16(sa + 32 * c + 16 * (u + 1), s[u ^ 1]);
                     uint32_t hw[8], lw[8];
+                    if (plain && linear) {
+                        const float d = lin0 + (float)(32 * c + 16 * u);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) s[u][e] = __float_as_uint(fmaf(slope, d + (float)e, __uint_as_float(s[u][e]) * fac));
+                    }
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
                         const float2 x = fma2(make_float2(__uint_as_float(s[u][e]), __uint_as_float(s[u][e + 1])), f, bs);
@@ -453,44 +483,54 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
         if (active && ok && (two || join || w == 0)) {
             const bool many = p.n_splits > 1;
             const float il = many ? 1.f : (L == 0.f ? 0.f : 1.f / L);
-            float *dst = many ? p.part_o + ((slot_id * p.n_splits + split) * TR + ri) * p.hd
-                              : p.out + (((uint64_t)b * p.n_tokens + tok) * p.nqh + head) * p.hd;
+            float *part = p.part_o + (slot_id * p.n_splits + split) * TR * p.hd;
+            float *out = p.out + ((uint64_t)b * p.n_tokens * p.nqh + kvh * p.G) * p.hd;
             const uint32_t cpr = p.hd / 8, c0 = join && w ? cpr / 2 : 0u, c1 = join && !w ? cpr / 2 : cpr;
             const uint32_t o0 = tmem + ((32u * wq) << 16) + 256 + (join ? 0u : 128u * w);
             const uint32_t pitch = p.hd * 4 + 16;   // a row's bytes: conflict-free for a thread per row
             const uint32_t rows_at = stage0 + 2 * TREE_TC_ROWS * 8, row = rows_at + ri * pitch;
-#pragma unroll 1
-            for (uint32_t c8 = c0; c8 < c1; ++c8) {
-                uint32_t x[8], y[8];
-                tc_ld8(o0 + 8 * c8, x);
-                if (join) tc_ld8(o0 + 128 + 8 * c8, y);
+#pragma unroll 2
+            for (uint32_t c8 = c0; c8 < c1; c8 += 2) {   // 16 dims (the last 8 may lie behind the row: not kept)
+                uint32_t x[16], y[16];
+                tc_ld16(o0 + 8 * c8, x);
+                if (join) tc_ld16(o0 + 128 + 8 * c8, y);
                 tc_wait_ld(x);
                 if (join) tc_wait_ld(y);
-                float v[8];
+                float v[16];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
+                for (int k = 0; k < 16; ++k) {
                     v[k] = __uint_as_float(x[k]) * f0;
                     if (join) v[k] = fmaf(__uint_as_float(y[k]), f1, v[k]);
                     v[k] = !many && L == 0.f ? 0.f : v[k] * il;
                 }
-                asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(row + 32 * c8), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]) : "memory");
-                asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(row + 32 * c8 + 16), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
+#pragma unroll
+                for (int k = 0; k < 16; k += 4)
+                    if (c8 + k / 8 < c1)
+                        asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(row + 32 * c8 + 4 * k), "f"(v[k]), "f"(v[k + 1]), "f"(v[k + 2]), "f"(v[k + 3]) : "memory");
             }
             if (on && (two || w == 0)) {
                 if (many) ml[ri] = make_float2(M, L);
                 else if (p.lse) p.lse[(uint64_t)(b * p.nkh + kvh) * (p.n_tokens * p.G) + rr] = L == 0.f ? -INFINITY : M + log2f(L);
             }
             __syncwarp();
-            // the warp's rows leave in whole sectors: lane = 16-byte piece, several rows at once where they are short
+            // the warp's rows leave in whole sectors: lane = 16-byte piece, several
+            // rows at once where they are short, 8 loads before their stores
             const uint32_t q4 = 2 * (c1 - c0), r0 = ri - lane, live = min(32u, nrows - r0);
             if (q4) {   // at most 32
-                const uint32_t rpp = 32 / q4, sub = lane / q4, d = lane - sub * q4;
-#pragma unroll 4
-                for (uint32_t x = 0; x < live; x += rpp) {
-                    const uint32_t rw = x + sub;
-                    float *to = reinterpret_cast<float *>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(dst), min(rw, 31u)));
-                    if (sub < rpp && rw < live)
-                        *reinterpret_cast<uint4 *>(to + 8 * c0 + 4 * d) = lds_u128(rows_at + (r0 + rw) * pitch + 32 * c0 + 16 * d);
+                const uint32_t rpp = 32 / q4, sub = lane / q4, d = 8 * c0 + 4 * (lane - sub * q4);
+                const uint8_t *from = smem + 2 * TREE_TC_ROWS * 8 + d * 4;
+#pragma unroll 1
+                for (uint32_t x = sub; x < live; x += 8 * rpp) {
+                    uint4 v[8];
+#pragma unroll
+                    for (uint32_t u = 0; u < 8; ++u)
+                        if (x + u * rpp < live) v[u] = *reinterpret_cast<const uint4 *>(from + (r0 + x + u * rpp) * pitch);
+#pragma unroll
+                    for (uint32_t u = 0; u < 8; ++u) {
+                        const uint32_t rw = r0 + x + u * rpp, gr = R0 + rw, tk = tree_token(p, gr);
+                        float *to = many ? part + (uint64_t)rw * p.hd : out + ((uint64_t)tk * p.nqh + (gr - tk * p.G)) * p.hd;
+                        if (sub < rpp && x + u * rpp < live) *reinterpret_cast<uint4 *>(to + d) = v[u];
+                    }
                 }
             }
         }

@@ -272,7 +272,8 @@ cudaError_t tree_weights_launch(const TreeParams &t, const CUtensorMap &km, uint
     // one CTA per SM: as many tiles each as that takes, at most WT_TILES
     const uint32_t tiles = (t.ctx_limit + TREE_TC_SP - 1) / TREE_TC_SP;
     const uint64_t units = (uint64_t)t.nkh * n_seqs;
-    p.per = (uint32_t)std::min<uint64_t>(WT_TILES, std::max<uint64_t>(1, (tiles * units + n_sm - 1) / n_sm));
+    const uint32_t parts = (uint32_t)std::max<uint64_t>(1, n_sm / units);
+    p.per = std::min(WT_TILES, (tiles + parts - 1) / parts);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;

@@ -378,7 +378,7 @@ VBS_API int vbs_cu_attention_tree(const vbs_cu_kv_t *kv, uint32_t layer, const v
  * highest scores, `keep` in all. idx[list][keep] receives them in ascending
  * order, -1 behind them; count[seq] = min(n, keep). Of equal scores the lower
  * slot is kept; a NaN counts as the lowest score, -0 as 0. first + recent <=
- * keep; n_limit at most 360448. */
+ * keep; n_limit at most 3145728. */
 VBS_API int vbs_cu_cache_select(const float *scores, uint64_t stride, uint32_t n_layers, uint32_t n_seqs, uint32_t n_kv_heads,
                                 const int32_t *n, uint32_t n_limit, uint32_t keep, uint32_t first, uint32_t recent,
                                 int32_t *idx, int32_t *count, void *stream);

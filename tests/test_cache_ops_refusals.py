@@ -102,7 +102,7 @@ def test_cache_select_refuses(vbs):
                 idx=FAKE, count=FAKE)
     for bad in (dict(scores=None), dict(n=None), dict(idx=None), dict(count=None), dict(n_layers=0), dict(n_seqs=0),
                 dict(n_kv_heads=0), dict(n_limit=101), dict(keep=0), dict(first=8), dict(recent=9),
-                dict(stride=1 << 20, n_limit=360449), dict(first=0xFFFFFFFF, recent=11)):
+                dict(stride=1 << 22, n_limit=3145729), dict(first=0xFFFFFFFF, recent=11)):
         refused(vbs, lambda: vbs.cache_select(**{**good, **bad}))
 
 

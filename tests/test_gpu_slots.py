@@ -202,7 +202,7 @@ def test_select(vbs, kind, n, keep, first, recent):
                 assert (idx[l, s, h] == ref.select(x[l, s, h], m, keep, first, recent)).all(), (l, s, h)
 
 
-@pytest.mark.parametrize("n,keep,lists", [(20000, 3000, 1), (70000, 2048, 1), (131072, 65537, 2), (360448, 5, 1), (60000, 20000, 40)])
+@pytest.mark.parametrize("n,keep,lists", [(20000, 3000, 1), (70000, 2048, 1), (131072, 65537, 2), (360448, 5, 1), (3145728, 1000, 1), (60000, 20000, 40)])
 def test_select_long(vbs, n, keep, lists):
     rng = np.random.default_rng(n)
     x = scores_of("ties", rng, (1, 1, lists, n))

@@ -159,35 +159,34 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_store_kernel(const __grid_c
 // ---------------------------------------------------------------------------
 // Choice of the slots to keep: exact selection of the r-th highest of m scores
 // per list, ties to the lowest index, result ascending.
-// Scores become 32-bit keys in the scores' order and stay in shared memory,
-// so global memory is read once:
-//  1. stored, with a histogram of their top 12 bits (sign, exponent and three
-//     mantissa bits spread accumulated weights over a hundred bins or more);
-//     the bin that holds the r-th highest is known after it.
-//  2. what lies above that bin becomes a bit per key, what lies in it a short
-//     list, on which two more histograms (10 bits each) find the key; the
-//     list's keys above it join the bits, those equal to it get bits of their
-//     own. A bin with more than SEL_CAND keys (many equal scores) is searched
-//     in place instead of from the list.
+// Scores become 32-bit keys in the scores' order:
+//  1. a histogram of the keys' top 12 bits (sign, exponent and three mantissa
+//     bits spread accumulated weights over a hundred bins or more); the bin
+//     that holds the r-th highest is known after it.
+//  2. the scores again (out of L2 now): what lies above that bin becomes a bit
+//     per key, what lies in it a short list, on which two more histograms (10
+//     bits each) find the key; the list's keys above it join the bits, those
+//     equal to it get bits of their own. A bin with more than SEL_CAND keys
+//     (many equal scores) is searched in place instead of from the list.
 //  3. the kept slots are written from the bits, 32 keys a word: their places
 //     are the counts of kept slots before them.
-// (Bits in place of a third look at the keys, and groups of 32 keys that are
-// not at an edge without tests per key: 103.7 -> MEASURED for 1024 lists of
-// up to 16384, which instruction issue bounds.)
 // Every warp owns a run of consecutive keys and visits only those, so the
-// counts per warp are all that has to be scanned. A cluster of 1, 2, 4 or 8
-// CTAs shares a list: each holds a part of it, histograms and counts are read
-// from the other CTAs' shared memory.
+// counts per warp are all that has to be scanned. Reading twice instead of
+// keeping the keys in shared memory leaves room for four CTAs per SM instead
+// of two: the steps are short and wait for one another, and other CTAs fill
+// the waits (1024 lists of up to 16384: 77.6 us with the keys kept). A cluster
+// of 2, 4 or 8 CTAs shares a list only where there are few long ones:
+// histograms and counts are then read from the other CTAs' shared memory.
 // ---------------------------------------------------------------------------
-constexpr uint32_t SEL_THREADS = 512, SEL_WARPS = SEL_THREADS / 32, SEL_CHUNK_MAX = 45056;
+constexpr uint32_t SEL_THREADS = 512, SEL_WARPS = SEL_THREADS / 32, SEL_CHUNK_MAX = 393216;
 constexpr uint32_t SEL_N_MAX = 8 * SEL_CHUNK_MAX;
 constexpr uint32_t SEL_BINS = 4096, SEL_BINS2 = 1024, SEL_CAND = 2048;
 constexpr int SEL_U = 8;            // keys in flight per thread
-// shared memory: state, histograms (12 bits, then 2 x 10), the list, the keys
-constexpr uint32_t SEL_STATE = 512, SEL_FIXED = SEL_STATE + (SEL_BINS + 2 * SEL_BINS2) * 4 + SEL_CAND * 2;
+// shared memory: state, histograms (12 bits, then 2 x 10), the list, the bits
+constexpr uint32_t SEL_STATE = 512, SEL_FIXED = SEL_STATE + (SEL_BINS + 2 * SEL_BINS2) * 4 + SEL_CAND * 8;
 
-__host__ __device__ constexpr uint32_t sel_keys_bytes(uint32_t chunk) { return ((chunk + 31) / 32 + SEL_WARPS) * 8 + (chunk + 3) / 4 * 16; }
-
+// a bit per key, runs of whole 128s
+__host__ __device__ constexpr uint32_t sel_words(uint32_t chunk) { return ((chunk + SEL_WARPS - 1) / SEL_WARPS + 127) / 128 * 4 * SEL_WARPS; }
 struct SelectParams {
     const float *scores;
     uint64_t stride;
@@ -198,21 +197,17 @@ struct SelectParams {
 };
 
 __device__ __forceinline__ uint32_t score_key(float f) {
-    const uint32_t u = __float_as_uint(f);
-    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return 0u;            // NaN: below everything
-    if ((u & 0x7FFFFFFFu) == 0u) return 0x80000000u;           // -0 is 0
-    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    const uint32_t u = __float_as_uint(f + 0.f);               // -0 is 0
+    return f != f ? 0u : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);   // NaN: below everything
 }
 
-// Adds 1 to a bin per lane (bin ~0: none); all lanes of the warp call it.
-// Lanes that agree (equal scores) make one addition.
+// Adds 1 to a bin per lane (bin ~0: none); all lanes of the warp call it. The
+// lanes that agree with the first make one addition (equal scores).
 __device__ __forceinline__ void hist_add(uint32_t *h, uint32_t bin) {
     const uint32_t b0 = __shfl_sync(0xffffffffu, bin, 0);
-    if (__all_sync(0xffffffffu, bin == b0)) {
-        if ((threadIdx.x & 31) == 0 && bin != 0xFFFFFFFFu) atomicAdd(&h[bin], 32u);
-    } else if (bin != 0xFFFFFFFFu) {
-        atomicAdd(&h[bin], 1u);
-    }
+    const uint32_t same = __ballot_sync(0xffffffffu, bin == b0);
+    const bool first = (threadIdx.x & 31) == 0;
+    if (bin != 0xFFFFFFFFu && (first || bin != b0)) atomicAdd(&h[bin], first ? (uint32_t)__popc(same) : 1u);
 }
 
 // The bin of `bins` (PER per thread) that holds the r-th highest, and how many
@@ -260,9 +255,8 @@ __global__ void __launch_bounds__(SEL_THREADS) cache_select_kernel(const SelectP
     uint32_t *st = reinterpret_cast<uint32_t *>(smem);   // [0,18) hist_find, 18 list length, 19 kept in all, 20 ties in all
     uint32_t *n_sure = st + 24, *n_tie = n_sure + SEL_WARPS;   // per warp
     uint32_t *h0 = reinterpret_cast<uint32_t *>(smem + SEL_STATE), *h1 = h0 + SEL_BINS, *h2 = h1 + SEL_BINS2;
-    uint16_t *cand = reinterpret_cast<uint16_t *>(h2 + SEL_BINS2);
-    const uint32_t words = (p.chunk_max + 31) / 32 + SEL_WARPS;   // a bit per key, runs of whole words
-    uint32_t *w_sure = reinterpret_cast<uint32_t *>(cand + SEL_CAND), *w_tie = w_sure + words, *keys = w_tie + words;
+    uint2 *cand = reinterpret_cast<uint2 *>(h2 + SEL_BINS2);   // key, place
+    uint32_t *w_sure = reinterpret_cast<uint32_t *>(cand + SEL_CAND), *w_tie = w_sure + sel_words(p.chunk_max);
 
     const int32_t n_in = p.n[s];
     int32_t *out = p.idx + (uint64_t)list * p.keep;
@@ -281,7 +275,7 @@ __global__ void __launch_bounds__(SEL_THREADS) cache_select_kernel(const SelectP
     const uint32_t m0 = p.first, m1 = n - p.recent;
     uint32_t r = p.keep - p.first - p.recent;
     const uint32_t chunk = (n + C - 1) / C, c0 = min(n, rank * chunk), len = min(n, c0 + chunk) - c0;
-    const uint32_t seg = ((len + SEL_WARPS - 1) / SEL_WARPS + 31) / 32 * 32;   // keys per warp
+    const uint32_t seg = ((len + SEL_WARPS - 1) / SEL_WARPS + 127) / 128 * 128;   // keys per warp
     const uint32_t s0 = min(len, warp * seg), s1 = min(len, s0 + seg);
     const float *src = p.scores + (uint64_t)list * p.stride + c0;
     const uint32_t f0 = m0 > c0 ? m0 - c0 : 0u, f1 = m1 > c0 ? m1 - c0 : 0u;   // [f0, f1) of this part compete
@@ -289,23 +283,24 @@ __global__ void __launch_bounds__(SEL_THREADS) cache_select_kernel(const SelectP
     for (uint32_t i = tid; i < SEL_BINS + 2 * SEL_BINS2; i += SEL_THREADS) h0[i] = 0u;
     if (tid < 24 + 2 * SEL_WARPS) st[tid] = 0u;
     __syncthreads();
-    // groups of 32 keys: whole, all of them competing; or at an edge
-    auto whole = [&](uint32_t i0) { return i0 >= f0 && i0 + 32 <= f1 && i0 + 32 <= s1; };
-    // 1. keys and their top 12 bits
+    // 4 groups of 32 keys: whole, all of them competing; or at an edge
+    auto whole = [&](uint32_t i0) { return i0 >= f0 && i0 + 128 <= f1 && i0 + 128 <= s1; };
+    // 1. the keys' top 12 bits
     for (uint32_t i0 = s0; i0 < s1; i0 += 32 * SEL_U) {
         float v[SEL_U];
 #pragma unroll
-        for (int u = 0; u < SEL_U; ++u) v[u] = i0 + 32 * u + lane < s1 ? __ldcs(src + i0 + 32 * u + lane) : 0.f;
+        for (int u = 0; u < SEL_U; ++u) v[u] = i0 + 32 * u + lane < s1 ? __ldg(src + i0 + 32 * u + lane) : 0.f;
 #pragma unroll
-        for (int u = 0; u < SEL_U; ++u) {
-            const uint32_t g0 = i0 + 32 * u, i = g0 + lane, k = score_key(v[u]);
-            if (g0 >= s1) break;
-            if (whole(g0)) {
-                keys[i] = k;
-                hist_add(h0, k >> 20);
+        for (int w = 0; w < SEL_U; w += 4) {
+            if (whole(i0 + 32 * w)) {
+#pragma unroll
+                for (int u = w; u < w + 4; ++u) hist_add(h0, score_key(v[u]) >> 20);
             } else {
-                if (i < s1) keys[i] = k;
-                hist_add(h0, i < s1 && i >= f0 && i < f1 ? k >> 20 : 0xFFFFFFFFu);
+#pragma unroll 1
+                for (int u = 0; u < 4; ++u) {
+                    const uint32_t i = i0 + 32 * (w + u) + lane, k = score_key(u == 0 ? v[w] : u == 1 ? v[w + 1] : u == 2 ? v[w + 2] : v[w + 3]);
+                    hist_add(h0, i < s1 && i >= f0 && i < f1 ? k >> 20 : 0xFFFFFFFFu);
+                }
             }
         }
     }
@@ -318,26 +313,45 @@ __global__ void __launch_bounds__(SEL_THREADS) cache_select_kernel(const SelectP
     }
     // 2. above the bin (or not competing): a bit; in it: listed
     const uint32_t below = (1u << lane) - 1, k_hi = b0 >= SEL_BINS - 1 ? 0xFFFFFFFFu : ((b0 + 1) << 20) - 1;   // the bin's highest key
-    for (uint32_t i0 = s0; i0 < s1; i0 += 32) {
-        const uint32_t i = i0 + lane;
-        bool sure, in;
-        if (whole(i0)) {
-            const uint32_t k = keys[i];
-            sure = k > k_hi;
-            in = (k >> 20) == b0;
-        } else {
-            const bool comp = i >= f0 && i < f1;
-            const uint32_t k = i < s1 ? keys[i] : 0u;
-            sure = i < s1 && (!comp || k > k_hi);
-            in = i < s1 && comp && (k >> 20) == b0;
-        }
-        const uint32_t m = __ballot_sync(0xffffffffu, in), g = __ballot_sync(0xffffffffu, sure);
-        if (lane == 0) { w_sure[i0 >> 5] = g; w_tie[i0 >> 5] = 0u; }
-        if (m) {
-            uint32_t at = 0;
-            if (lane == 0) at = atomicAdd(&st[18], (uint32_t)__popc(m));
-            at = __shfl_sync(0xffffffffu, at, 0) + __popc(m & below);
-            if (in && at < SEL_CAND) cand[at] = (uint16_t)i;
+    const uint32_t k_lo = b0 << 20;   // and its lowest (no bin: k_hi ~0 and an empty list)
+    for (uint32_t j0 = s0; j0 < s1; j0 += 32 * SEL_U) {
+        float v[SEL_U];
+#pragma unroll
+        for (int u = 0; u < SEL_U; ++u) v[u] = j0 + 32 * u + lane < s1 ? __ldg(src + j0 + 32 * u + lane) : 0.f;
+#pragma unroll
+        for (int x = 0; x < SEL_U; x += 4) {
+            const uint32_t i0 = j0 + 32 * x;
+            if (i0 >= s1) break;
+            bool in[4], any = false;
+            uint32_t g[4], k[4];
+            const bool all_in = whole(i0);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                k[u] = score_key(v[x + u]);
+                bool sure = k[u] > k_hi;
+                in[u] = b0 < SEL_BINS && k[u] - k_lo < (1u << 20);
+                if (!all_in) {
+                    const uint32_t i = i0 + 32 * u + lane;
+                    const bool comp = i >= f0 && i < f1;
+                    sure = i < s1 && (!comp || sure);
+                    in[u] = in[u] && i < s1 && comp;
+                }
+                g[u] = __ballot_sync(0xffffffffu, sure);
+                any |= in[u];
+            }
+            if (lane == 0) {   // runs are whole 128s
+                *reinterpret_cast<uint4 *>(&w_sure[i0 >> 5]) = make_uint4(g[0], g[1], g[2], g[3]);
+                *reinterpret_cast<uint4 *>(&w_tie[i0 >> 5]) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            if (any) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (in[u]) {
+                        const uint32_t at = atomicAdd(&st[18], 1u);
+                        if (at < SEL_CAND) cand[at] = make_uint2(k[u], i0 + 32 * u + lane);
+                    }
+            }
+            __syncwarp();
         }
     }
     __syncthreads();
@@ -347,12 +361,12 @@ __global__ void __launch_bounds__(SEL_THREADS) cache_select_kernel(const SelectP
     auto each = [&](auto f) {
         if (listed) {
             for (uint32_t j0 = warp * 32; j0 < nc; j0 += SEL_THREADS) {
-                const uint32_t j = j0 + lane, i = j < nc ? cand[j] : 0u;
-                f(j < nc, i, j < nc ? keys[i] : 0u);
+                const uint2 e = j0 + lane < nc ? cand[j0 + lane] : make_uint2(0u, 0u);
+                f(j0 + lane < nc, e.y, e.x);
             }
         } else {
             for (uint32_t i0 = s0; i0 < s1; i0 += 32) {
-                const uint32_t i = i0 + lane, k = i < s1 ? keys[i] : 0u;
+                const uint32_t i = i0 + lane, k = i < s1 ? score_key(__ldg(src + i)) : 0u;
                 f(i < s1 && i >= f0 && i < f1 && k >> 20 == b0, i, k);
             }
         }
@@ -367,13 +381,13 @@ __global__ void __launch_bounds__(SEL_THREADS) cache_select_kernel(const SelectP
         T = (b0 << 20) | (b1 << 10) | st[0];
         need = r - st[1];
         each([&](bool c, uint32_t i, uint32_t k) {
-            if (c && k >= T) atomicOr(k > T ? &w_sure[i >> 5] : &w_tie[i >> 5], 1u << (i & 31));
+            if (c && k >= T) atomicOr((k > T ? w_sure : w_tie) + (i >> 5), 1u << (i & 31));
         });
     }
     __syncthreads();
     // what each warp's run keeps for certain, and its ties
     uint32_t at = 0, ties = 0;
-    for (uint32_t g = s0 / 32 + lane; g < (s1 + 31) / 32; g += 32) {
+    for (uint32_t g = s0 / 32 + lane; s0 < s1 && g < (s1 + 127) / 128 * 4; g += 32) {   // (a run may be empty)
         at += __popc(w_sure[g]);
         ties += __popc(w_tie[g]);
     }
@@ -404,16 +418,27 @@ __global__ void __launch_bounds__(SEL_THREADS) cache_select_kernel(const SelectP
     }
     // 3. out: n > keep, so all places get filled
     at += min(ties, need);
-    for (uint32_t i0 = s0; i0 < s1; i0 += 32) {
-        uint32_t g = w_sure[i0 >> 5];
-        const uint32_t e = w_tie[i0 >> 5];
-        if (e && ties < need) {   // the first of them, up to `need`
-            const bool mine = ((e >> lane) & 1u) && ties + __popc(e & below) < need;
-            g |= __ballot_sync(0xffffffffu, mine);
+    const bool tied = n_tie[warp] != 0;
+    for (uint32_t i0 = s0; i0 < s1; i0 += 128) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(&w_sure[i0 >> 5]);
+        uint32_t g[4] = {w.x, w.y, w.z, w.w};
+        if (tied) {   // the first of them, up to `need`
+            const uint4 t = *reinterpret_cast<const uint4 *>(&w_tie[i0 >> 5]);
+            const uint32_t e[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const bool mine = ((e[u] >> lane) & 1u) && ties + __popc(e[u] & below) < need;
+                g[u] |= __ballot_sync(0xffffffffu, mine);
+                ties += __popc(e[u]);
+            }
         }
-        ties += __popc(e);
-        if ((g >> lane) & 1u) out[at + __popc(g & below)] = (int32_t)(c0 + i0 + lane);
-        at += __popc(g);
+        int32_t *o = out + at;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if ((g[u] >> lane) & 1u) o[__popc(g[u] & below)] = (int32_t)(c0 + i0 + 32 * u + lane);
+            o += __popc(g[u]);
+        }
+        at = (uint32_t)(o - out);
     }
     if (C == 1) return;
     cluster.sync();   // nobody leaves while its shared memory is read
@@ -615,7 +640,7 @@ __global__ void __launch_bounds__(GA_THREADS) gather_inplace_warp_kernel(const _
 
 cudaError_t slots_configure() {
     return cudaFuncSetAttribute(cache_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)(SEL_FIXED + sel_keys_bytes(SEL_CHUNK_MAX)));
+                                (int)(SEL_FIXED + 8 * sel_words(SEL_CHUNK_MAX)));
 }
 
 static GatherSide gather_side(const vbs_cu_kv_t *kv) {
@@ -756,7 +781,7 @@ int vbs_cu_cache_select(const float *scores, uint64_t stride, uint32_t n_layers,
     DevState *d = backend_current();
     if (!d) { latch_error("vbs_cu_cache_select: no usable device"); return -1; }
     // CTAs per list: as many as the SMs have room for, 4096 scores each at
-    // least; more where a list does not fit one CTA's shared memory
+    // least; more where the bits of a list do not fit one CTA's shared memory
     uint32_t c = 1;
     while (c < 8 && (n_limit > c * SEL_CHUNK_MAX || (lists * c * 2 <= (uint64_t)d->n_sm && n_limit > c * 4096u))) c *= 2;
     SelectParams p = {};
@@ -766,7 +791,7 @@ int vbs_cu_cache_select(const float *scores, uint64_t stride, uint32_t n_layers,
     cfg.gridDim = dim3((unsigned)(lists * c));
     cfg.blockDim = dim3(SEL_THREADS);
     p.chunk_max = (n_limit + c - 1) / c;
-    cfg.dynamicSmemBytes = SEL_FIXED + sel_keys_bytes(p.chunk_max);
+    cfg.dynamicSmemBytes = SEL_FIXED + 8 * sel_words(p.chunk_max);
     cfg.stream = static_cast<cudaStream_t>(stream);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;

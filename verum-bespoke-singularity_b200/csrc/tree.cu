@@ -13,12 +13,14 @@
 // parts' (m, l, o) go to the caller's workspace and tree_merge_kernel joins
 // them. One part writes the result itself.
 //
-// tree_mma_kernel: as the decode attention in attn.cu, 16 positions of K and V
-// per warp at a time through padded shared memory (cp.async, TREE_NST stages),
-// mma.sync m16n8k16 with fp32 accumulators, online softmax with a lazy
-// rescale. fp32 queries and weights are two fp16 halves each (x = hi + lo to
-// 2^-22); both halves run on the same B fragments into the same accumulators,
-// 16 rows per warp.
+// tree_mma_kernel (few rows, or head_dim above 128): stages of 64 positions of
+// K and V come by TMA (128-byte swizzle: ldmatrix without bank conflicts), the
+// warps take blocks of 16 positions in turn and wait for stages, never for one
+// another; the warp that ends a stage's last block fills it again: mma.sync m16n8k16 with fp32
+// accumulators, online softmax with a lazy rescale, joined at the end. fp32
+// queries and weights are two fp16 halves each (x = hi + lo to 2^-22); both
+// halves run on the same B fragments into the same accumulators, 16 rows per
+// warp. Bound by memory up to some 40 rows. (More rows: tree_tc.cu.)
 //  * Queries are scaled per row by a power of two to 2^8..2^9, so neither half
 //    leaves fp16's range; the power goes into the score's factor (exact).
 //  * The softmax reference stays 6 below the running maximum (log2 units), so
@@ -38,24 +40,31 @@ namespace vbs {
 template <int HD, int WR, int WP> struct TreeCfg {
     static constexpr int NW = WR * WP, THREADS = NW * 32;
     static constexpr int ROWS = 16 * WR;
-    static constexpr int SP = HD > 128 ? 32 : 64;      // positions per stage
-    static constexpr int RSB = HD * 2 + 16;            // staged row bytes (padded)
-    static constexpr int KPOS = 2 * SP * RSB;          // offset of the stage's key positions
-    static constexpr int STAGE = KPOS + SP * 4;
-    static constexpr int NST = HD >= 128 ? 3 : 4;
+    static constexpr int SP = 64;                      // positions per stage, 4 blocks of 16
+    static constexpr int BLKS = HD / 64;               // boxes of 64 dims
+    static constexpr int BOX = SP * 128, HALF = BLKS * BOX, STAGE = 2 * HALF;   // keys, then values
+    static constexpr int NST = 3;
     static constexpr bool QREG = HD <= 128;            // query halves in registers
-    static constexpr int QSM = QREG ? 0 : ROWS * RSB * 2;
+    static constexpr int QRS = HD * 2 + 16, QSM = QREG ? 0 : ROWS * QRS * 2;
     static constexpr int OLD = HD + 4;                 // floats per row in the join of the warps
     static constexpr int JOIN = WP * ROWS * OLD * 4;
-    static constexpr int SMEM = QSM + (NST * STAGE > JOIN ? NST * STAGE : JOIN);
-    static_assert(SP % (16 * WP) == 0, "whole blocks of 16 per warp");
+    static constexpr int BODY = NST * STAGE > JOIN ? NST * STAGE : JOIN;
+    static constexpr int SMEM = BODY + QSM;
+    static constexpr int CTAS = SMEM <= 113 * 1024 ? 2 : 1;   // per SM
+    static_assert(WP % 4 == 0, "a stage's 4 blocks go to 4 warps");
 };
 
 template <int HD, int WR, int WP>
-__global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(const __grid_constant__ TreeParams p) {
+__global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(const __grid_constant__ TreeParams p,
+                                                                                const __grid_constant__ CUtensorMap km,
+                                                                                const __grid_constant__ CUtensorMap vm) {
     using C = TreeCfg<HD, WR, WP>;
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ int32_t sh_min[C::NW];
+    __shared__ __align__(8) uint64_t bars[2 * C::NST];   // full, empty
+    __shared__ uint32_t used[C::NST], issued[C::NST];   // blocks of the stage that are through; 1 + the stage's last tile
+    __shared__ int sh_bad;
+    volatile int *bad = &sh_bad;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int wr = warp % WR, wp = warp / WR;
     const uint32_t kvh = blockIdx.x % p.nkh, tile = blockIdx.x / p.nkh, split = blockIdx.y, b = blockIdx.z;
@@ -73,34 +82,31 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
         for (int r = threadIdx.x; r < C::ROWS; r += C::THREADS) ml[r] = make_float2(-INFINITY, 0.f);
         return;
     }
-    const uint32_t nch = (t1 - t0 + C::SP - 1) / C::SP;
-    const uint16_t *kb = p.kc + (uint64_t)b * p.seq_stride + (uint64_t)kvh * p.head_step;
-    const uint16_t *vb = p.vc + (uint64_t)b * p.seq_stride + (uint64_t)kvh * p.head_step;
+    const uint32_t nch = (t1 - t0 + C::SP - 1) / C::SP, blks = (p.hd + 63) / 64;
     const int32_t *kpos = p.k_pos ? p.k_pos + (uint64_t)(p.k_pos_per_head ? b * p.nkh + kvh : b) * p.max_ctx : nullptr;
-    const uint32_t sbase = smem_u32(smem) + C::QSM;
-    const uint32_t cpr = p.hd / 8;
-
-    auto issue = [&](uint32_t c) {
-        const uint32_t st = sbase + (c % C::NST) * C::STAGE;
-        const uint32_t pb = t0 + c * C::SP;
-#pragma unroll 4
-        for (int i = threadIdx.x; i < 2 * C::SP * (HD / 8); i += C::THREADS) {
-            const int isv = i / (C::SP * (HD / 8)), r = (i / (HD / 8)) % C::SP;
-            const uint32_t ch = i % (HD / 8);
-            const bool ok = pb + r < t1 && ch < cpr;   // head_dim below HD: zeros
-            const uint16_t *src = (isv ? vb : kb) + (uint64_t)(ok ? pb + r : t0) * p.pos_step + (ok ? ch : 0) * 8;
-            cp_async16(st + (isv * C::SP + r) * C::RSB + ch * 16, src, ok ? 16u : 0u);
-        }
-        if (kpos && threadIdx.x < C::SP) {
-            const uint32_t t = pb + threadIdx.x;
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(st + C::KPOS + threadIdx.x * 4),
-                         "l"(kpos + (t < t1 ? t : t0)), "r"(t < t1 ? 4u : 0u) : "memory");
-        }
+    const uint32_t sbase = smem_u32(smem), full0 = smem_u32(bars), empty0 = full0 + 8 * C::NST;
+    auto waits = [&](uint32_t bar, uint32_t parity) -> bool {
+        if (mbar_wait_bounded(bar, parity, kWaitNs)) return true;
+        *bad = 1;
+        return false;
     };
-#pragma unroll
-    for (int c = 0; c < C::NST - 1; ++c) {
-        if ((uint32_t)c < nch) issue(c);
-        cp_async_commit();
+    // stage c's keys and values (one thread)
+    auto load = [&](uint32_t c) {
+        const uint32_t s = c % C::NST, st = sbase + s * C::STAGE;
+        issued[s] = c + 1;
+        mbar_arrive_expect_tx(full0 + 8 * s, 2 * blks * C::BOX);
+        for (uint32_t k = 0; k < blks; ++k) tree_tma(st + k * C::BOX, &km, 64 * k, t0 + c * C::SP, kvh, b, full0 + 8 * s);
+        for (uint32_t k = 0; k < blks; ++k) tree_tma(st + C::HALF + k * C::BOX, &vm, 64 * k, t0 + c * C::SP, kvh, b, full0 + 8 * s);
+    };
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::NST; ++s) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 4 * WR);
+            used[s] = issued[s] = 0;
+        }
+        sh_bad = 0;
+        mbar_fence_init();
+        for (uint32_t c = 0; c < min(nch, (uint32_t)C::NST); ++c) load(c);
     }
 
     // the two rows of this thread: g and g + 8 of the warp's 16
@@ -156,9 +162,9 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
                     qh[kk][j] = *reinterpret_cast<const uint32_t *>(&hi);
                     ql[kk][j] = *reinterpret_cast<const uint32_t *>(&lo);
                 } else if (wp == 0) {
-                    uint8_t *d = smem + (16 * wr + g + 8 * (j & 1)) * C::RSB + (16 * kk + 8 * (j >> 1) + qd) * 2;
+                    uint8_t *d = smem + C::BODY + (16 * wr + g + 8 * (j & 1)) * C::QRS + (16 * kk + 8 * (j >> 1) + qd) * 2;
                     *reinterpret_cast<__half2 *>(d) = hi;
-                    *reinterpret_cast<__half2 *>(d + C::ROWS * C::RSB) = lo;
+                    *reinterpret_cast<__half2 *>(d + C::ROWS * C::QRS) = lo;
                 }
             }
         }
@@ -167,7 +173,7 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
     const float pre = p.cap > 0.f ? 1.f / p.cap : TREE_LOG2E;
     fac[0] *= pre;
     fac[1] *= pre;
-    // highest query position of the rows, for the window's fast path
+    // highest query position of the warp's rows, for the window's fast path
     int32_t qmax = max(qpos[0], qpos[1]);
     qmax = __reduce_max_sync(0xffffffffu, qmax);
 
@@ -175,20 +181,24 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
 #pragma unroll
     for (int n = 0; n < HD / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
     float mref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    for (uint32_t c = 0; c < nch; ++c) {
-        if (c + C::NST - 1 < nch) issue(c + C::NST - 1);
-        cp_async_commit();
-        cp_async_wait<C::NST - 1>();
-        __syncthreads();
-        const uint32_t st = sbase + (c % C::NST) * C::STAGE;
-#pragma unroll 1
-        for (int sb = 16 * wp; sb < C::SP; sb += 16 * WP) {
-            const uint32_t tb = t0 + c * C::SP + sb;
-            if (tb >= t1) break;
-            const uint32_t kst = st + sb * C::RSB, vst = kst + C::SP * C::RSB;
+    __syncthreads();   // barriers, and queries in shared memory
+    // blocks of 16 positions in turn over the position warps; a block's key
+    // positions (lane: position) are read one block ahead
+    const uint32_t kks = (p.hd + 31) / 32 * 2, ns = (p.hd + 15) / 16 * 2;   // 16s of dims with keys, 8s with values
+    auto kp_at = [&](uint32_t t) { return lane < 16 && t + lane < t1 ? tree_kpos(p, kpos, b, t + lane, nc) : 0x7FFFFFFF; };
+    const bool want_pos = kpos || p.window || p.slopes;
+    int32_t kn = want_pos ? kp_at(t0 + 16 * wp) : 0;
+    for (uint32_t tb = t0 + 16 * wp, j = wp; tb < t1; tb += 16 * WP, j += WP) {
+        const uint32_t c = j / 4, st = sbase + c % C::NST * C::STAGE;
+        const int32_t kp = kn;
+        if (want_pos) kn = kp_at(tb + 16 * WP);
+        if (!__all_sync(0xffffffffu, !*bad && waits(full0 + 8 * (c % C::NST), (c / C::NST) & 1u))) break;
+        {
+            const uint32_t kst = st + 16 * (j & 3) * 128, vst = kst + C::HALF, sw = lane & 7;
             float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
             for (int kk = 0; kk < HD / 16; kk += 2) {
+                if (kk >= (int)kks) break;
                 uint32_t ah[2][4], al[2][4];
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
@@ -196,15 +206,15 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
 #pragma unroll
                         for (int j = 0; j < 4; ++j) { ah[u][j] = qh[kk + u][j]; al[u][j] = ql[kk + u][j]; }
                     } else {
-                        const uint32_t a = smem_u32(smem) + (16 * wr + (lane & 15)) * C::RSB + (16 * (kk + u) + 8 * (lane >> 4)) * 2;
+                        const uint32_t a = sbase + C::BODY + (16 * wr + (lane & 15)) * C::QRS + (16 * (kk + u) + 8 * (lane >> 4)) * 2;
                         ldsm_x4(a, ah[u][0], ah[u][1], ah[u][2], ah[u][3]);
-                        ldsm_x4(a + C::ROWS * C::RSB, al[u][0], al[u][1], al[u][2], al[u][3]);
+                        ldsm_x4(a + C::ROWS * C::QRS, al[u][0], al[u][1], al[u][2], al[u][3]);
                     }
                 }
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     uint32_t b0, b1, b2, b3;
-                    ldsm_x4(kst + (8 * j + (lane & 7)) * C::RSB + (16 * kk + 8 * (lane >> 3)) * 2, b0, b1, b2, b3);
+                    ldsm_x4(kst + (kk >> 2) * C::BOX + (8 * j + (lane & 7)) * 128 + ((((2 * kk) & 7) + (lane >> 3)) ^ sw) * 16, b0, b1, b2, b3);
                     mma_f16_acc(s[j], al[0], b0, b1);
                     mma_f16_acc(s[j], ah[0], b0, b1);
                     mma_f16_acc(s[j], al[1], b2, b3);
@@ -221,26 +231,25 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
                     if (p.cap > 0.f) x[h][e] = tree_cap(x[h][e], cap2);
                 }
             uint32_t hidden = 0;   // bit 4 h + e: row h does not see key e
-            const bool plain = tb + 16 <= min(nc, t1) && !kpos && (!p.window || (int64_t)qmax - tb < (int64_t)p.window);
+            // every row sees every position: by the lowest key position
+            const bool context = tb + 16 <= min(nc, t1);
+            const int32_t low = want_pos && context ? __reduce_min_sync(0xffffffffu, kp) : 0;
+            const bool plain = context && (!kpos || low >= 0) && (!p.window || qmax - low < (int32_t)p.window);
             if (!plain || p.slopes) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const uint32_t kl = qd + (e & 1) + 8 * (e >> 1), t = tb + kl;
+                    const int32_t k = want_pos ? __shfl_sync(0xffffffffu, kp, kl) : 0;
                     const bool in = t < t1, drafted = in && t >= nc;
-                    int32_t kp = (int32_t)t;
-                    if (kpos) asm volatile("ld.shared.s32 %0, [%1];" : "=r"(kp) : "r"(st + C::KPOS + (sb + kl) * 4));
-                    else if (drafted) kp = tree_qpos(p, b, t - nc, nc);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        bool see = in && kp >= 0;
-                        if (kpos == nullptr) see = in;
+                        bool see = in && (!kpos || k >= 0);
                         if (drafted && on[h])
                             see = see && (p.mask ? (p.mask[((uint64_t)b * p.n_tokens + tok[h]) * p.words + ((t - nc) >> 5)] >>
                                                     ((t - nc) & 31)) & 1u
                                                  : t - nc <= tok[h]);
-                        const int64_t dist = (int64_t)qpos[h] - kp;
-                        if (p.window) see = see && dist < (int64_t)p.window;
-                        if (p.slopes) x[h][e] -= slope[h] * (float)dist;
+                        if (p.window) see = see && qpos[h] - k < (int32_t)p.window;
+                        if (p.slopes) x[h][e] = fmaf(slope[h], (float)(k - qpos[h]), x[h][e]);
                         if (!see) {
                             x[h][e] = -INFINITY;
                             hidden |= 1u << (4 * h + e);
@@ -271,8 +280,8 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
                 // some row does not see some key: values must be finite for 0 * v to be 0
                 bool bad = false;
 #pragma unroll 4
-                for (int i = lane; i < 16 * (HD / 8); i += 32) {
-                    const uint4 w = lds_u128(vst + (i / (HD / 8)) * C::RSB + (i % (HD / 8)) * 16);
+                for (uint32_t i = lane; i < 16 * 8 * blks; i += 32) {
+                    const uint4 w = lds_u128(vst + (i >> 7) * C::BOX + (i & 127) * 16);
                     const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
@@ -293,9 +302,10 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
                 }
 #pragma unroll
                 for (int n = 0; n < HD / 8; n += 2) {
+                    if (n >= (int)ns) break;
                     uint32_t b0, b1, b2, b3;
-                    ldsm_x4_trans(vst + ((lane & 7) + 8 * ((lane >> 3) & 1)) * C::RSB + (8 * n + 8 * (lane >> 4)) * 2, b0, b1,
-                                  b2, b3);
+                    ldsm_x4_trans(vst + (n >> 3) * C::BOX + ((lane & 7) + 8 * ((lane >> 3) & 1)) * 128 + (((n & 7) + (lane >> 4)) ^ sw) * 16, b0,
+                                  b1, b2, b3);
                     mma_f16_acc(o[n], pl, b0, b1);
                     mma_f16_acc(o[n], ph, b0, b1);
                     mma_f16_acc(o[n + 1], pl, b2, b3);
@@ -322,8 +332,9 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
                     }
 #pragma unroll
                     for (int n = 0; n < HD / 8; ++n) {
+                        if (n >= (int)ns) break;
                         uint32_t vv;
-                        vv = lds_u32(vst + k * C::RSB + (8 * n + qd) * 2);
+                        vv = lds_u32(vst + (n >> 3) * C::BOX + k * 128 + (((n & 7) ^ (k & 7)) << 4) + qd * 2);
                         const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&vv));
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
@@ -332,9 +343,19 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
                 }
             }
         }
-        __syncthreads();
+        __syncwarp();
+        if (lane == 0) {
+            // the stage's last block fills it again (it waits for arrivals
+            // that are all made by then)
+            const uint32_t s = c % C::NST;
+            mbar_arrive(empty0 + 8 * s);
+            if (atomicAdd(&used[s], 1u) == 4 * WR - 1) {
+                used[s] = 0;
+                if (c + C::NST < nch && waits(empty0 + 8 * s, (c / C::NST) & 1u)) load(c + C::NST);
+            }
+        }
+        __syncwarp();
     }
-    cp_async_wait<0>();
 
     // join the warps that shared these rows
 #pragma unroll
@@ -342,8 +363,8 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
     }
-    __syncthreads();
-    float *sh = reinterpret_cast<float *>(smem + C::QSM);
+    __syncthreads();   // all stages are used up
+    float *sh = reinterpret_cast<float *>(smem);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         float *d = sh + (wp * C::ROWS + 16 * wr + g + 8 * h) * C::OLD;
@@ -353,6 +374,14 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
             *reinterpret_cast<float2 *>(d + 8 * n + qd) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
     }
     __syncthreads();
+    if (*bad) {
+        if (threadIdx.x == 0) {
+            dev_flag_error(p.err, DERR_TIMEOUT_FULL);
+            for (int s = 0; s < C::NST; ++s)   // copies may still be landing
+                if (issued[s]) mbar_wait_bounded(full0 + 8 * s, ((issued[s] - 1) / C::NST) & 1u, kWaitNs);
+        }
+        return;
+    }
     const uint32_t live = min((uint32_t)C::ROWS, nrows - R0), q4 = p.hd / 4;
     float *po = p.part_o + (slot * p.n_splits + split) * C::ROWS * p.hd;
     for (uint32_t i = threadIdx.x; i < live * q4; i += C::THREADS) {
@@ -528,11 +557,12 @@ struct TreePlan {
     size_t ml, o, lse, bytes;   // offsets into the workspace, total
 };
 
-// Warps over rows and over positions of a CTA by the rows of a KV head: few
-// rows leave all warps to the positions (nothing is computed twice), more
-// rows share the staged keys.
-static uint32_t tree_warp_rows(uint32_t rows) { return rows <= 16 ? 1 : (rows <= 32 ? 2 : 4); }
+// Rows per CTA of tree_mma_kernel: 16 a warp.
+static uint32_t tree_warp_rows(uint32_t rows) { return rows <= 16 ? 1 : 2; }
 
+// More than 16 rows of a KV head go to tree_tc_kernel: its products cost the
+// same for 1 row and for 128, and from there on they cost less than
+// mma.sync's (64 rows x 4096 positions x 8 KV heads: 31.9 us and 20.5).
 constexpr uint32_t TREE_TC_MIN_ROWS = 17;
 
 static TreePlan tree_plan(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t, int n_sm) {
@@ -542,14 +572,22 @@ static TreePlan tree_plan(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t, int n_s
     pl.tc = kv->head_dim <= 128 && pl.rows >= TREE_TC_MIN_ROWS;
     pl.tile_rows = pl.tc ? (pl.rows > TREE_TC_ROWS ? 2 * TREE_TC_ROWS : TREE_TC_ROWS) : 16 * tree_warp_rows(pl.rows);
     pl.row_tiles = (pl.rows + pl.tile_rows - 1) / pl.tile_rows;
-    // parts: about two CTAs per SM, at least 64 positions each; tree_tc_kernel
-    // fills an SM, so there one CTA each, in whole tiles
+    // Parts of the positions: the number that ends first, counting whole
+    // waves of CTAs, a part's positions, what a CTA costs besides (in
+    // positions: tree_tc_kernel some 640, the other some 128) and the join.
+    // Only a plan: the kernels divide what the lengths on the device leave.
     const uint64_t ctas = (uint64_t)pl.row_tiles * kv->n_kv_heads * kv->n_seqs;
-    const uint32_t unit = pl.tc ? TREE_TC_SP : 64;
-    uint64_t s = pl.tc ? (uint64_t)n_sm / ctas : ((uint64_t)n_sm * 2 + ctas - 1) / ctas;
-    s = std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint64_t>(s, TREE_MAX_PARTS), (t->ctx_limit + unit - 1) / unit));
-    pl.per_split = (uint32_t)(((t->ctx_limit + s - 1) / s + unit - 1) / unit * unit);
-    pl.n_splits = (t->ctx_limit + pl.per_split - 1) / pl.per_split;
+    const uint64_t slots = (uint64_t)n_sm * (pl.tc || kv->head_dim > 128 ? 1 : 2);
+    const uint32_t unit = pl.tc ? TREE_TC_SP : 64, extra = pl.tc ? 640 : 128, join = pl.tc ? 384 : 128;
+    uint32_t span = t->ctx_limit;
+    if (t->window && !t->k_pos) span = (uint32_t)std::min<uint64_t>(span, (uint64_t)t->window + t->n_tokens + 63);
+    uint64_t best = ~0ull;
+    for (uint32_t s = 1; s <= std::min(TREE_MAX_PARTS, (span + unit - 1) / unit); ++s) {
+        const uint32_t per = ((span + s - 1) / s + unit - 1) / unit * unit, parts = (span + per - 1) / per;
+        const uint64_t cost = (ctas * parts + slots - 1) / slots * (per + extra) + (parts > 1 ? join : 0);
+        if (cost < best) { best = cost; pl.per_split = per; pl.n_splits = parts; }
+        if (ctas * s > 16 * slots) break;
+    }
     auto take = [&](size_t n) { const size_t at = pl.bytes; pl.bytes += (n + 255) / 256 * 256; return at; };
     const size_t heads = (size_t)kv->n_seqs * kv->n_kv_heads;
     if (pl.n_splits > 1) {
@@ -607,33 +645,21 @@ static cudaError_t tree_merge_launch(const TreeParams &p, uint32_t rows, uint32_
     return few ? cudaLaunchKernelEx(&cfg, tree_merge_warp_kernel, p, tile_rows) : cudaLaunchKernelEx(&cfg, tree_merge_kernel, p, tile_rows);
 }
 
-template <int HD, int WR, int WP> static cudaError_t tree_go(const TreeParams &p, dim3 grid, cudaStream_t st) {
+template <int HD, int WR, int WP>
+static cudaError_t tree_go(const TreeParams &p, const CUtensorMap &km, const CUtensorMap &vm, dim3 grid, cudaStream_t st) {
     using C = TreeCfg<HD, WR, WP>;
-    tree_mma_kernel<HD, WR, WP><<<grid, C::THREADS, C::SMEM, st>>>(p);
+    tree_mma_kernel<HD, WR, WP><<<grid, C::THREADS, C::SMEM, st>>>(p, km, vm);
     return cudaGetLastError();
-}
-template <int HD> static cudaError_t tree_go_rows(const TreeParams &p, uint32_t wr, dim3 grid, cudaStream_t st) {
-    constexpr int W = HD > 128 ? 2 : 4;   // 32 positions per stage: two warps of 16
-    if (wr == 1) return tree_go<HD, 1, W>(p, grid, st);
-    if (wr == 2) return tree_go<HD, 2, W>(p, grid, st);
-    return tree_go<HD, 4, 2>(p, grid, st);
 }
 template <int HD, int WR, int WP> static cudaError_t tree_cfg() {
     return cudaFuncSetAttribute(tree_mma_kernel<HD, WR, WP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 TreeCfg<HD, WR, WP>::SMEM);
 }
-template <int HD> static cudaError_t tree_cfg_rows() {
-    constexpr int W = HD > 128 ? 2 : 4;
-    cudaError_t e = tree_cfg<HD, 1, W>();
-    if (e == cudaSuccess) e = tree_cfg<HD, 2, W>();
-    if (e == cudaSuccess) e = tree_cfg<HD, 4, 2>();
-    return e;
-}
-
 cudaError_t tree_configure() {
-    cudaError_t e = tree_cfg_rows<64>();
-    if (e == cudaSuccess) e = tree_cfg_rows<128>();
-    if (e == cudaSuccess) e = tree_cfg_rows<256>();
+    cudaError_t e = tree_cfg<64, 1, 4>();
+    if (e == cudaSuccess) e = tree_cfg<128, 1, 4>();
+    if (e == cudaSuccess) e = tree_cfg<256, 1, 8>();
+    if (e == cudaSuccess) e = tree_cfg<256, 2, 4>();
     if (e == cudaSuccess) e = tree_tc_configure();
     if (e == cudaSuccess) e = tree_weights_configure();
     // the join takes the attention kernels' split of shared memory and L1:
@@ -695,19 +721,20 @@ int vbs_cu_attention_tree(const vbs_cu_kv_t *kv, uint32_t layer, const vbs_cu_tr
     p.g_magic = (uint32_t)((0x100000000ull + p.G - 1) / p.G);
     p.err = d->err;
     const dim3 grid(kv->n_kv_heads * pl.row_tiles, pl.n_splits, kv->n_seqs);
-    const uint32_t wr = pl.tile_rows / 16;
     note_launches(1u + (pl.n_splits > 1) + (t->weights_out != nullptr));
-    CUtensorMap km, vm;
-    cudaError_t e = cudaSuccess;
-    if (pl.tc || t->weights_out) e = tree_map(&km, p.kc, kv, TREE_TC_SP);
-    if (e == cudaSuccess && pl.tc) e = tree_map(&vm, p.vc, kv, TREE_TC_SP);
+    CUtensorMap km, vm, wm;
+    cudaError_t e = tree_map(&km, p.kc, kv, pl.tc ? TREE_TC_SP : 64);
+    if (e == cudaSuccess) e = tree_map(&vm, p.vc, kv, pl.tc ? TREE_TC_SP : 64);
+    if (e == cudaSuccess && t->weights_out) e = tree_map(&wm, p.kc, kv, TREE_TC_SP);
     if (e == cudaSuccess)
-        e = pl.tc ? tree_tc_launch(p, km, vm, kv->n_seqs, pl.tile_rows > TREE_TC_ROWS, st)
-                    : kv->head_dim <= 64 ? tree_go_rows<64>(p, wr, grid, st)
-                                       : (kv->head_dim <= 128 ? tree_go_rows<128>(p, wr, grid, st) : tree_go_rows<256>(p, wr, grid, st));
+        e = pl.tc                     ? tree_tc_launch(p, km, vm, kv->n_seqs, pl.tile_rows > TREE_TC_ROWS, st)
+            : kv->head_dim <= 64      ? tree_go<64, 1, 4>(p, km, vm, grid, st)
+            : kv->head_dim <= 128     ? tree_go<128, 1, 4>(p, km, vm, grid, st)
+            : pl.tile_rows == 16      ? tree_go<256, 1, 8>(p, km, vm, grid, st)
+                                      : tree_go<256, 2, 4>(p, km, vm, grid, st);
     if (e == cudaSuccess && pl.n_splits > 1)
         e = tree_merge_launch(p, pl.rows, kv->n_seqs, pl.tile_rows, d->n_sm, st);
-    if (e == cudaSuccess && t->weights_out) e = tree_weights_launch(p, km, kv->n_seqs, d->n_sm, st);
+    if (e == cudaSuccess && t->weights_out) e = tree_weights_launch(p, wm, kv->n_seqs, d->n_sm, st);
     return cuda_ok(e, "attention_tree") ? 0 : -1;
 }
 

@@ -557,39 +557,52 @@ struct TreePlan {
     size_t ml, o, lse, bytes;   // offsets into the workspace, total
 };
 
-// Rows per CTA of tree_mma_kernel: 16 a warp.
-static uint32_t tree_warp_rows(uint32_t rows) { return rows <= 16 ? 1 : 2; }
-
-// More than 16 rows of a KV head go to tree_tc_kernel: its products cost the
-// same for 1 row and for 128, and from there on they cost less than
-// mma.sync's (64 rows x 4096 positions x 8 KV heads: 31.9 us and 20.5).
-constexpr uint32_t TREE_TC_MIN_ROWS = 17;
+// The parts of one kernel's plan: the number that ends first, counting whole
+// waves of CTAs on `slots`, a position's and a CTA's time, and the join's.
+// Only a plan: the kernels divide what the lengths on the device leave.
+struct TreeParts { uint64_t ns; uint32_t per, parts; };
+static TreeParts tree_parts(uint64_t ctas, uint64_t slots, uint32_t span, uint32_t unit, uint32_t pos_ns, uint32_t cta_ns, uint32_t join_ns) {
+    TreeParts best = {~0ull, 0, 0};
+    for (uint32_t s = 1; s <= std::min(TREE_MAX_PARTS, (span + unit - 1) / unit); ++s) {
+        const uint32_t per = ((span + s - 1) / s + unit - 1) / unit * unit, parts = (span + per - 1) / per;
+        const uint64_t ns = (ctas * parts + slots - 1) / slots * ((uint64_t)per * pos_ns + cta_ns) + (parts > 1 ? join_ns : 0);
+        if (ns < best.ns) best = {ns, per, parts};
+        if (ctas * s > 16 * slots) break;
+    }
+    return best;
+}
 
 static TreePlan tree_plan(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t, int n_sm) {
     TreePlan pl = {};
-    const uint32_t G = t->n_q_heads / kv->n_kv_heads;
+    const uint32_t G = t->n_q_heads / kv->n_kv_heads, hd = kv->head_dim;
     pl.rows = t->n_tokens * G;
-    pl.tc = kv->head_dim <= 128 && pl.rows >= TREE_TC_MIN_ROWS;
-    pl.tile_rows = pl.tc ? (pl.rows > TREE_TC_ROWS ? 2 * TREE_TC_ROWS : TREE_TC_ROWS) : 16 * tree_warp_rows(pl.rows);
-    pl.row_tiles = (pl.rows + pl.tile_rows - 1) / pl.tile_rows;
-    // Parts of the positions: the number that ends first, counting whole
-    // waves of CTAs, a part's positions, what a CTA costs besides (in
-    // positions: tree_tc_kernel some 640, the other some 128) and the join.
-    // Only a plan: the kernels divide what the lengths on the device leave.
-    const uint64_t ctas = (uint64_t)pl.row_tiles * kv->n_kv_heads * kv->n_seqs;
-    const uint64_t slots = (uint64_t)n_sm * (pl.tc || kv->head_dim > 128 ? 1 : 2);
-    const uint32_t unit = pl.tc ? TREE_TC_SP : 64, extra = pl.tc ? 640 : 128, join = pl.tc ? 384 : 128;
     uint32_t span = t->ctx_limit;
     if (t->window && !t->k_pos) span = (uint32_t)std::min<uint64_t>(span, (uint64_t)t->window + t->n_tokens + 63);
-    uint64_t best = ~0ull;
-    for (uint32_t s = 1; s <= std::min(TREE_MAX_PARTS, (span + unit - 1) / unit); ++s) {
-        const uint32_t per = ((span + s - 1) / s + unit - 1) / unit * unit, parts = (span + per - 1) / per;
-        const uint64_t cost = (ctas * parts + slots - 1) / slots * (per + extra) + (parts > 1 ? join : 0);
-        if (cost < best) { best = cost; pl.per_split = per; pl.n_splits = parts; }
-        if (ctas * s > 16 * slots) break;
+    const uint64_t heads = (uint64_t)kv->n_kv_heads * kv->n_seqs;
+    auto tiles = [&](uint32_t rows) { return (pl.rows + rows - 1) / rows; };
+    // tree_mma_kernel: 16 rows a CTA (32 above head_dim 128, where a CTA has an
+    // SM to itself); tree_tc_kernel: 128 rows, 256 if there are more. The tc
+    // kernel's time for a position is the same for 1 row and for 128 but its
+    // start is the longer. Measured on full SMs, ns per position and CTA:
+    // mma 40 (head_dim 128, two CTAs per SM), 20 (64), 25 (256, one per SM);
+    // tc 16 and 33 (128: 128 rows, 256 rows), 13 and 25 (64).
+    pl.tile_rows = hd > 128 && pl.rows > 16 ? 32 : 16;
+    TreeParts best = hd > 128 ? tree_parts(heads * tiles(pl.tile_rows), n_sm, span, 64, 25, 4000, 2000)
+                              : tree_parts(heads * tiles(16), 2ull * n_sm, span, 64, hd > 64 ? 40 : 20, 2500, 2000);
+    if (hd <= 128) {
+        const uint32_t wide = pl.rows > TREE_TC_ROWS;
+        const TreeParts tc = tree_parts(heads * tiles(TREE_TC_ROWS << wide), n_sm, span, TREE_TC_SP,
+                                        (hd > 64 ? 16 : 13) << wide, wide ? 13000 : 9000, 3000);
+        if (tc.ns < best.ns) {
+            best = tc;
+            pl.tc = true;
+            pl.tile_rows = TREE_TC_ROWS << wide;
+        }
     }
+    pl.per_split = best.per;
+    pl.n_splits = best.parts;
+    pl.row_tiles = tiles(pl.tile_rows);
     auto take = [&](size_t n) { const size_t at = pl.bytes; pl.bytes += (n + 255) / 256 * 256; return at; };
-    const size_t heads = (size_t)kv->n_seqs * kv->n_kv_heads;
     if (pl.n_splits > 1) {
         pl.ml = take(heads * pl.row_tiles * pl.n_splits * pl.tile_rows * sizeof(float2));
         pl.o = take(heads * pl.row_tiles * pl.n_splits * pl.tile_rows * kv->head_dim * sizeof(float));

@@ -278,16 +278,10 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
             bool apart = false;
             if (__any_sync(0xffffffffu, hidden != 0)) {
                 // some row does not see some key: values must be finite for 0 * v to be 0
-                bool bad = false;
+                uint32_t zero = 0;
 #pragma unroll 4
-                for (uint32_t i = lane; i < 16 * 8 * blks; i += 32) {
-                    const uint4 w = lds_u128(vst + (i >> 7) * C::BOX + (i & 127) * 16);
-                    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        bad |= (ww[k] & 0x7C00u) == 0x7C00u || (ww[k] & 0x7C000000u) == 0x7C000000u;
-                }
-                apart = __any_sync(0xffffffffu, bad);
+                for (uint32_t i = lane; i < 16 * 8 * blks; i += 32) zero = finite4(lds_u128(vst + (i >> 7) * C::BOX + (i & 127) * 16), zero);
+                apart = __any_sync(0xffffffffu, zero != 0u);
             }
             if (!apart) {
                 uint32_t ph[4], pl[4];

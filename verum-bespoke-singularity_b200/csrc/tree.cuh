@@ -113,6 +113,14 @@ __device__ __forceinline__ void tree_part(const TreeParams &p, uint32_t first, u
     t1 = min(end, t0 + per);
 }
 
+// `zero` times the eight halves of v, added up: 0 while all are finite.
+__device__ __forceinline__ uint32_t finite4(const uint4 &v, uint32_t zero) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(zero) : "r"(w[k]), "r"(0u));
+    return zero & 0x7FFF7FFFu;   // -0 is 0
+}
+
 // 64 dims x n positions of one KV head of a cache, from a tensor map of the
 // layer's keys or values ([head_dim][position][kv head][seq], rows of 128
 // bytes in shared memory, their 16-byte chunks XOR-ed with the position's

@@ -65,6 +65,22 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
     // the queries start on their way before anything else is known
     TcQ<128> q;
     if (warp < TC_LOADER) tc_q_load(p, R0 + 16 * warp + (lane & 7), kvh, b, q);
+    if (warp == TC_LOADER && lane == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tp.km) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tp.vm) : "memory");
+        for (uint32_t s = 0; s < tp.ns; ++s) {
+            mbar_init(base + H_FULL + 8 * s, 1);
+            mbar_init(base + H_EMPTY + 8 * s, 1);
+        }
+        for (uint32_t w = 0; w < 2; ++w) {
+            mbar_init(base + H_S + 8 * w, 1);
+            mbar_init(base + H_O + 8 * w, 1);
+        }
+        mbar_init(base + H_END, 2);
+        *bad = 0;
+        reinterpret_cast<int *>(hs + H_ACC)[0] = reinterpret_cast<int *>(hs + H_ACC)[1] = 0;
+        mbar_fence_init();
+    }
     pdl_launch_dependents();
     uint32_t nc, nt;
     if (!tree_lengths(p, b, nc, nt) || R0 >= nt * p.G) return;
@@ -103,24 +119,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
     };
     uint32_t it = 0;
     if (warp == TC_LOADER) {
+        load(it++);   // the first keys are needed first; the rest follows behind the barrier
         if (lane == 0) {
-            for (uint32_t s = 0; s < tp.ns; ++s) {
-                mbar_init(base + H_FULL + 8 * s, 1);
-                mbar_init(base + H_EMPTY + 8 * s, 1);
-            }
             for (uint32_t w = 0; w < 2; ++w) {
-                mbar_init(base + H_S + 8 * w, 1);
                 mbar_init(base + H_P + 16 * w, w ? aw1 : aw0);       // weights of the tile's first 64 positions
                 mbar_init(base + H_P + 16 * w + 8, w ? aw1 : aw0);   // and of the others
-                mbar_init(base + H_O + 8 * w, 1);
             }
-            mbar_init(base + H_END, 2);
-            *bad = 0;
-            reinterpret_cast<int *>(hs + H_ACC)[0] = reinterpret_cast<int *>(hs + H_ACC)[1] = 0;
             mbar_fence_init();
         }
         __syncwarp();
-        load(it++);   // the first keys are needed first; the rest follows behind the barrier
     } else if (warp == TC_QK) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + H_TMEM), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -131,14 +138,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
         hi = __reduce_max_sync(0xffffffffu, hi);
         if (lane == 0) *reinterpret_cast<int32_t *>(hs + H_QMAX) = hi;
     } else {
-        // 8 rows at a time, two times 8 per warp and 128 rows
+        // 8 rows at a time, two times 8 per warp and 128 rows; places of rows
+        // that are not there keep what they hold (nobody reads their scores)
 #pragma unroll 1
         for (uint32_t g = 0; g < (two ? 4u : 2u); ++g) {
-            const uint32_t r = 16 * warp + 8 * (g & 1) + (lane & 7), x = g >> 1;
+            const uint32_t r0 = 16 * warp + 8 * (g & 1), x = g >> 1, n0 = TREE_TC_ROWS * ((g + 1) >> 1) + 16 * warp + 8 * ((g + 1) & 1);
+            if (x * TREE_TC_ROWS + r0 >= nrows) break;
             TcQ<128> next;
-            tc_q_load(p, R0 + TREE_TC_ROWS * ((g + 1) >> 1) + 16 * warp + 8 * ((g + 1) & 1) + (lane & 7), kvh, b, next);
-            const float f = tc_q_store(p, q, smem + tp.q_off + x * q_bytes, TREE_TC_ROWS * 16, q_bytes / 2, r, chunks);
-            if (lane < 8) fac_sm[x * TREE_TC_ROWS + r] = f;
+            if (n0 < nrows) tc_q_load(p, R0 + n0 + (lane & 7), kvh, b, next);
+            const float f = tc_q_store(p, q, smem + tp.q_off + x * q_bytes, TREE_TC_ROWS * 16, q_bytes / 2, r0 + (lane & 7), chunks);
+            if (lane < 8) fac_sm[x * TREE_TC_ROWS + r0 + lane] = f;
             q = next;
         }
         tc_proxy();
@@ -264,6 +273,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
             }
             tn += tstep;
             const bool whole = context && low >= 0 && (!p.window || qmax - low < (int32_t)p.window);
+            // a tile with drafted positions: this row's mask words, before the wait
+            const int m0 = (int)((int64_t)tb - nc) >> 5;   // word of the tile's first position (may be negative)
+            uint32_t mk[5] = {0u, 0u, 0u, 0u, 0u};
+            if (p.mask && on && tb + TREE_TC_SP > nc) {
+                const uint32_t *mrow = p.mask + ((uint64_t)b * p.n_tokens + tok) * p.words;
+#pragma unroll
+                for (int k = 0; k < 5; ++k) mk[k] = m0 + k >= 0 && m0 + k < (int)p.words ? mrow[m0 + k] : 0u;
+            }
             dead = dead || !all(!*bad && waits(base + H_S + 8 * w, (n >> 1) & 1u));
             if (dead) {   // a wait ran out: only the barriers are kept company
                 if (!whole && bar_or(bar, bar_n, false) && bar_or(bar, bar_n, false))
@@ -308,7 +325,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                     tc_ld8(sa + 8 * c, x);
                     if (!(c & 3)) {
                         const uint32_t inside = ones(nval - 8 * c);
-                        see = on ? tree_sees(p, b, tok, t, nc, nval - 8 * c) : inside;
+                        see = inside;
+                        const int d0 = (int)t - (int)nc;   // drafted number of bit 0
+                        if (d0 > -32 && on) {
+                            if (!p.mask) {
+                                see &= ones((int)tok - d0 + 1);
+                            } else {
+                                const int k = c >> 2;
+                                const uint32_t lo = k == 0 ? mk[0] : k == 1 ? mk[1] : k == 2 ? mk[2] : mk[3];
+                                const uint32_t hi = k == 0 ? mk[1] : k == 1 ? mk[2] : k == 2 ? mk[3] : mk[4];
+                                see &= __funnelshift_r(lo, hi, d0 & 31) | ones(-d0);
+                            }
+                        }
                         kp = (int32_t)t + lane;
                         if (!by_slot && (kpos || p.window || p.slopes) && lane < nval - 8 * c) kp = tree_kpos(p, kpos, b, t + lane, nc);
                         if (by_slot) {
@@ -354,11 +382,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                     const bool here = waits(base + H_FULL + 8 * (vx % tp.ns), (vx / tp.ns) & 1u);
                     bool odd = false;
                     if (here) {
+                        uint32_t zero = 0;
 #pragma unroll 8
                         for (uint32_t k = bar_r; k < slot / 16; k += bar_n) {
                             const uint4 v = *reinterpret_cast<const uint4 *>(smem + (vx % tp.ns) * slot + k * 16);
-                            odd |= not_finite2(v.x) | not_finite2(v.y) | not_finite2(v.z) | not_finite2(v.w);
+                            zero = finite4(v, zero);
                         }
+                        odd = zero != 0u;
                     }
                     if (bar_or(bar, bar_n, odd)) {
                         // rare: the rows that see such values add them here,
@@ -464,7 +494,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                 }
             }
         }
-        // ---------------- out: rows through shared memory ---------------------
+        // ---------------- out --------------------------------------------------
         const bool ok = all(waits(base + H_END, 0) && !*bad);
         tc_after();
         float L = l.x + l.y, M = mref, f0 = 1.f, f1 = 0.f;
@@ -483,55 +513,38 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
         if (active && ok && (two || join || w == 0)) {
             const bool many = p.n_splits > 1;
             const float il = many ? 1.f : (L == 0.f ? 0.f : 1.f / L);
-            float *part = p.part_o + (slot_id * p.n_splits + split) * TR * p.hd;
-            float *out = p.out + ((uint64_t)b * p.n_tokens * p.nqh + kvh * p.G) * p.hd;
+            float *dst = many ? p.part_o + ((slot_id * p.n_splits + split) * TR + ri) * p.hd
+                              : p.out + (((uint64_t)b * p.n_tokens + tok) * p.nqh + head) * p.hd;
             const uint32_t cpr = p.hd / 8, c0 = join && w ? cpr / 2 : 0u, c1 = join && !w ? cpr / 2 : cpr;
             const uint32_t o0 = tmem + ((32u * wq) << 16) + 256 + (join ? 0u : 128u * w);
-            const uint32_t pitch = p.hd * 4 + 16;   // a row's bytes: conflict-free for a thread per row
-            const uint32_t rows_at = stage0 + 2 * TREE_TC_ROWS * 8, row = rows_at + ri * pitch;
+            const bool wide = (reinterpret_cast<uintptr_t>(dst) & 31) == 0;
+            // straight from the rows' threads, a whole 32-byte sector each
 #pragma unroll 2
-            for (uint32_t c8 = c0; c8 < c1; c8 += 2) {   // 16 dims (the last 8 may lie behind the row: not kept)
-                uint32_t x[16], y[16];
-                tc_ld16(o0 + 8 * c8, x);
-                if (join) tc_ld16(o0 + 128 + 8 * c8, y);
+            for (uint32_t c8 = c0; c8 < c1; ++c8) {
+                uint32_t x[8], y[8];
+                tc_ld8(o0 + 8 * c8, x);
+                if (join) tc_ld8(o0 + 128 + 8 * c8, y);
                 tc_wait_ld(x);
                 if (join) tc_wait_ld(y);
-                float v[16];
+                float v[8];
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
+                for (int k = 0; k < 8; ++k) {
                     v[k] = __uint_as_float(x[k]) * f0;
                     if (join) v[k] = fmaf(__uint_as_float(y[k]), f1, v[k]);
                     v[k] = !many && L == 0.f ? 0.f : v[k] * il;
                 }
-#pragma unroll
-                for (int k = 0; k < 16; k += 4)
-                    if (c8 + k / 8 < c1)
-                        asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(row + 32 * c8 + 4 * k), "f"(v[k]), "f"(v[k + 1]), "f"(v[k + 2]), "f"(v[k + 3]) : "memory");
+                if (on && wide) {
+                    asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + 8 * c8), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+                                 "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
+                } else if (on) {
+                    *reinterpret_cast<float4 *>(dst + 8 * c8) = make_float4(v[0], v[1], v[2], v[3]);
+                    *reinterpret_cast<float4 *>(dst + 8 * c8 + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                }
+                __syncwarp();
             }
             if (on && (two || w == 0)) {
                 if (many) ml[ri] = make_float2(M, L);
                 else if (p.lse) p.lse[(uint64_t)(b * p.nkh + kvh) * (p.n_tokens * p.G) + rr] = L == 0.f ? -INFINITY : M + log2f(L);
-            }
-            __syncwarp();
-            // the warp's rows leave in whole sectors: lane = 16-byte piece, several
-            // rows at once where they are short, 8 loads before their stores
-            const uint32_t q4 = 2 * (c1 - c0), r0 = ri - lane, live = min(32u, nrows - r0);
-            if (q4) {   // at most 32
-                const uint32_t rpp = 32 / q4, sub = lane / q4, d = 8 * c0 + 4 * (lane - sub * q4);
-                const uint8_t *from = smem + 2 * TREE_TC_ROWS * 8 + d * 4;
-#pragma unroll 1
-                for (uint32_t x = sub; x < live; x += 8 * rpp) {
-                    uint4 v[8];
-#pragma unroll
-                    for (uint32_t u = 0; u < 8; ++u)
-                        if (x + u * rpp < live) v[u] = *reinterpret_cast<const uint4 *>(from + (r0 + x + u * rpp) * pitch);
-#pragma unroll
-                    for (uint32_t u = 0; u < 8; ++u) {
-                        const uint32_t rw = r0 + x + u * rpp, gr = R0 + rw, tk = tree_token(p, gr);
-                        float *to = many ? part + (uint64_t)rw * p.hd : out + ((uint64_t)tk * p.nqh + (gr - tk * p.G)) * p.hd;
-                        if (sub < rpp && x + u * rpp < live) *reinterpret_cast<uint4 *>(to + d) = v[u];
-                    }
-                }
             }
         }
         if (*bad && threadIdx.x == 0) dev_flag_error(p.err, DERR_TIMEOUT_FULL);

@@ -226,10 +226,11 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[h][e] *= fac[h];
-                    if (p.cap > 0.f) x[h][e] = tree_cap(x[h][e], cap2);
-                }
+                for (int e = 0; e < 4; ++e) x[h][e] *= fac[h];
+            if (p.cap > 0.f) {
+                tree_cap_all(x[0], cap2);
+                tree_cap_all(x[1], cap2);
+            }
             uint32_t hidden = 0;   // bit 4 h + e: row h does not see key e
             // every row sees every position: by the lowest key position
             const bool context = tb + 16 <= min(nc, t1);

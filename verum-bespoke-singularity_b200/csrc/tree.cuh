@@ -56,6 +56,31 @@ __device__ __forceinline__ float tree_cap(float y, float cap2) {
     return y != y ? y : copysignf(cap2 * __fdividef(num, den), y);
 }
 
+// The same for several scores of a warp: while all are below 0.55 (scores well
+// under the cap) by tanh's series up to y^15, without a division or an
+// exponential; its next term is 4e-8 of the value there.
+template <int N> __device__ __forceinline__ void tree_cap_all(float (&y)[N], float cap2) {
+    float top = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) top = fmaxf(top, fabsf(y[e]));
+    if (__all_sync(0xffffffffu, top < 0.55f)) {   // (a NaN stays one either way)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float z = y[e] * y[e];
+            float t = fmaf(z, -1.4558344e-3f, 3.5921281e-3f);   // -929569 / 638512875, 21844 / 6081075
+            t = fmaf(z, t, -8.8632355e-3f);                     // -1382 / 155925
+            t = fmaf(z, t, 2.1869489e-2f);                      // 62 / 2835
+            t = fmaf(z, t, -5.3968254e-2f);                     // -17 / 315
+            t = fmaf(z, t, 1.3333333e-1f);                      // 2 / 15
+            t = fmaf(z, t, -3.3333333e-1f);
+            y[e] = cap2 * fmaf(y[e] * z, t, y[e]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) y[e] = tree_cap(y[e], cap2);
+    }
+}
+
 // Lengths of sequence b; false (flagged once) when they do not fit the cache
 // or the call's limit: the sequence is left alone.
 __device__ __forceinline__ bool tree_lengths(const TreeParams &p, uint32_t b, uint32_t &nc, uint32_t &nt) {

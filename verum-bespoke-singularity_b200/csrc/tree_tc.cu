@@ -108,8 +108,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
     auto all = [&](bool x) { return __all_sync(0xffffffffu, x); };
 
     // ---------------- loader: items K0 V0 K1 V1 ... ------------------------
-    auto load = [&](uint32_t it) {
-        const uint32_t s = it % tp.ns, tb = t0 + it / 2 * TREE_TC_SP;
+    // (stages and phases are counted along: a division would cost an issuer more than a wait)
+    auto load = [&](uint32_t it, uint32_t s) {
+        const uint32_t tb = t0 + it / 2 * TREE_TC_SP;
         if (lane == 0) {
             mbar_arrive_expect_tx(base + H_FULL + 8 * s, slot);
             for (uint32_t k = 0; k < tp.blks; ++k)
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
     };
     uint32_t it = 0;
     if (warp == TC_LOADER) {
-        load(it++);   // the first keys are needed first; the rest follows behind the barrier
+        load(it++, 0);   // the first keys are needed first; the rest follows behind the barrier
         if (lane == 0) {
             for (uint32_t w = 0; w < 2; ++w) {
                 mbar_init(base + H_P + 16 * w, w ? aw1 : aw0);       // weights of the tile's first 64 positions
@@ -158,9 +159,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
     const uint32_t tmem = *reinterpret_cast<uint32_t *>(hs + H_TMEM);
 
     if (warp == TC_LOADER) {
-        for (; it < 2 * nch; ++it) {
-            if (!all(!*bad && (it < tp.ns || waits(base + H_EMPTY + 8 * (it % tp.ns), (it / tp.ns - 1) & 1u)))) break;
-            load(it);
+        for (uint32_t s = 1, ph = 1; it < 2 * nch; ++it) {   // ph: parity of the last time round
+            if (!all(!*bad && (it < tp.ns || waits(base + H_EMPTY + 8 * s, ph)))) break;
+            load(it, s);
+            if (++s == tp.ns) { s = 0; ph ^= 1u; }
         }
         // after a failed wait copies may still be landing: the newest of
         // every slot is waited for before the CTA ends
@@ -176,10 +178,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
         constexpr uint32_t QCH = TREE_TC_ROWS * 16u;   // bytes per chunk of the queries
         const uint64_t dq0 = tc_desc(stage0 + tp.q_off, QCH, 128u), dk = tc_desc_sw(stage0, 16u, 1024u);
         const uint32_t qlo = q_bytes / 32, lead = tc_elect();   // the low halves' offset, in descriptor units
-        for (uint32_t n = 0; n < steps; ++n) {
-            const uint32_t w = n & 1, x = two ? n & ~1u : 2 * n, s = x % tp.ns;
+        for (uint32_t n = 0, s = 0, ph = 0; n < steps; ++n) {
+            const uint32_t w = n & 1;
             // keys here, and this stream's last weights used up
-            if (!all(!*bad && waits(base + H_FULL + 8 * s, (x / tp.ns) & 1u) && (n < 2 || waits(base + H_O + 8 * w, (n / 2 - 1) & 1u)))) break;
+            if (!all(!*bad && waits(base + H_FULL + 8 * s, ph) && (n < 2 || waits(base + H_O + 8 * w, (n / 2 - 1) & 1u)))) break;
             tc_after();
             const uint64_t d = dk + s * (slot / 16), dq = dq0 + (two && w ? q_bytes / 16 : 0u);
 #pragma unroll
@@ -194,6 +196,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                 if (!two || w) tc_commit(base + H_EMPTY + 8 * s);
             }
             __syncwarp();
+            if (!two || w) {   // on to the next tile's keys, two stages further
+                s += 2;
+                if (s >= tp.ns) { s -= tp.ns; ph ^= 1u; }
+            }
         }
         if (lead) tc_commit(base + H_END);   // with the other issuer's: every product has completed
         __syncwarp();
@@ -203,9 +209,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
         const uint64_t dv = tc_desc_sw(stage0, TC_BLK, 1024u);
         const uint32_t lead = tc_elect();
         bool ok = true;
-        for (uint32_t n = 0; ok && n < steps; ++n) {
-            const uint32_t w = n & 1, i = two ? n >> 1 : n, x = 2 * i + 1, s = x % tp.ns;
-            if (!all(!*bad && waits(base + H_FULL + 8 * s, (x / tp.ns) & 1u) && waits(base + H_P + 16 * w, (n >> 1) & 1u))) break;
+        for (uint32_t n = 0, s = 1, ph = 0; ok && n < steps; ++n) {
+            const uint32_t w = n & 1, i = two ? n >> 1 : n;
+            if (!all(!*bad && waits(base + H_FULL + 8 * s, ph) && waits(base + H_P + 16 * w, (n >> 1) & 1u))) break;
             tc_after();
             const uint64_t d = dv + s * (slot / 16);
             const uint32_t o = tmem + 256 + 128 * w, pa = tmem + 128 * w;
@@ -226,6 +232,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                 if (!two || w) tc_commit(base + H_EMPTY + 8 * s);
             }
             __syncwarp();
+            if (!two || w) {
+                s += 2;
+                if (s >= tp.ns) { s -= tp.ns; ph ^= 1u; }
+            }
         }
         if (lead) tc_commit(base + H_END);
         __syncwarp();
@@ -288,10 +298,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                 continue;
             }
             tc_after();
-            // plain: the scores as the product left them, times the row's
-            // factor, plus (linear) slope * (slot - query position)
-            const bool linear = p.slopes && !kpos, plain = whole && (!p.slopes || linear) && !(p.cap > 0.f);
-            const float lin0 = (float)((int32_t)tb - qp);
+            // plain: the scores as the product left them, times the row's factor;
+            // simple: capped, or with slope * (slot - query position) added
+            const bool linear = p.slopes && !kpos, simple = whole && (!p.slopes || linear);
+            const bool plain = simple && !p.slopes && !(p.cap > 0.f);
+            const float cap2 = p.cap * TREE_LOG2E;
             float mx = -INFINITY;
             if (plain) {
                 uint32_t s[2][32];
@@ -300,21 +311,37 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     if (c < 3) tc_ld32(sa + 32 * (c + 1), s[(c + 1) & 1]);
-                    if (linear) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            s[c & 1][e] = __float_as_uint(fmaf(slope, lin0 + (float)(32 * c + e), __uint_as_float(s[c & 1][e]) * fac));
-                    }
                     mx = fmaxf(mx, max32(s[c & 1]));
                     if (c < 3) tc_wait_ld(s[(c + 1) & 1]);
                 }
-                if (!linear) mx *= fac;
+                mx *= fac;
+            } else if (simple) {
+#pragma unroll 1
+                for (int c = 0; c < 8; ++c) {
+                    uint32_t s[16];
+                    tc_ld16(sa + 16 * c, s);
+                    tc_wait_ld(s);
+                    float x[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[e] = __uint_as_float(s[e]) * fac;
+                    if (p.cap > 0.f) tree_cap_all(x, cap2);
+                    if (linear) {
+                        const float d = (float)((int32_t)tb + 16 * c - qp);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) x[e] = fmaf(slope, d + (float)e, x[e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) mx = max3(mx, x[e], x[e + 1]);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[e] = __float_as_uint(x[e]);
+                    tc_st16(sa + 16 * c, s);
+                }
+                tc_wait_st();
             } else {
                 // scores as the formula has them, back into tensor memory, 8 at
                 // a time (short code: it runs for few tiles, out of cold
                 // instruction caches)
                 const bool by_slot = !kpos && tb + TREE_TC_SP <= nc;   // the tile's positions are its slots
-                const float cap2 = p.cap * TREE_LOG2E;
                 bool hidden = (nval & 15) != 0;                        // stale rows behind the end in the last product
                 uint32_t see = 0;     // bit e: this row sees the e-th next position
                 int32_t kp = 0;       // key position of slot (32's first + lane), handed round where rows need them
@@ -352,23 +379,22 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                         hidden |= on && see != inside;
                     }
                     tc_wait_ld(x);
+                    float v[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * fac);
-                    if (p.cap > 0.f) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) x[e] = __float_as_uint(tree_cap(__uint_as_float(x[e]), cap2));
-                    }
+                    for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(x[e]) * fac;
+                    if (p.cap > 0.f) tree_cap_all(v, cap2);
                     if (p.slopes) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             const int32_t k = by_slot ? (int32_t)t + e : __shfl_sync(0xffffffffu, kp, 8 * (c & 3) + e);
-                            x[e] = __float_as_uint(fmaf(slope, (float)(k - qp), __uint_as_float(x[e])));
+                            v[e] = fmaf(slope, (float)(k - qp), v[e]);
                         }
                     }
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        if (!((see >> e) & 1u)) x[e] = 0xFF800000u;
-                        mx = fmaxf(mx, __uint_as_float(x[e]));
+                        if (!((see >> e) & 1u)) v[e] = -INFINITY;
+                        mx = fmaxf(mx, v[e]);
+                        x[e] = __float_as_uint(v[e]);
                     }
                     see >>= 8;
                     __syncwarp();
@@ -457,7 +483,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                     }
                 }
             }
-            const float f1 = plain && !linear ? fac : 1.f, b1 = mref == -INFINITY ? 0.f : mref;
+            const float f1 = plain ? fac : 1.f, b1 = mref == -INFINITY ? 0.f : mref;
             const float2 f = make_float2(f1, f1), bs = make_float2(-b1, -b1);
             uint32_t s[2][16];
             tc_ld16(sa, s[0]);
@@ -470,11 +496,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                 for (int u = 0; u < 2; ++u) {
                     if (c < 3 || !u) tc_ld16(sa + 32 * c + 16 * (u + 1), s[u ^ 1]);
                     uint32_t hw[8], lw[8];
-                    if (plain && linear) {
-                        const float d = lin0 + (float)(32 * c + 16 * u);
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) s[u][e] = __float_as_uint(fmaf(slope, d + (float)e, __uint_as_float(s[u][e]) * fac));
-                    }
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
                         const float2 x = fma2(make_float2(__uint_as_float(s[u][e]), __uint_as_float(s[u][e + 1])), f, bs);

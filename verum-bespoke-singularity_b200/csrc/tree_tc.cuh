@@ -87,6 +87,11 @@ __device__ __forceinline__ void tc_ld8(uint32_t a, uint32_t (&v)[8]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(a));
 }
+__device__ __forceinline__ void tc_st16(uint32_t a, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(a),
+                 "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+                 "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+}
 __device__ __forceinline__ void tc_st8(uint32_t a, const uint32_t (&v)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(a), "r"(v[0]), "r"(v[1]),
                  "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
@@ -197,20 +202,6 @@ __device__ __forceinline__ float tc_q_store(const TreeParams &p, const TcQ<D> &q
         *reinterpret_cast<uint4 *>(d + lo_off) = make_uint4(l[0], l[1], l[2], l[3]);
     }
     return fabsf(p.scale) * __uint_as_float((uint32_t)(127 - e) << 23) * (p.cap > 0.f ? 1.f / p.cap : TREE_LOG2E);
-}
-
-// Bit e: this row's token sees position t + e (e < 32) as far as the mask and
-// the number `n` of positions left go; nc: the context's length.
-__device__ __forceinline__ uint32_t tree_sees(const TreeParams &p, uint32_t b, uint32_t tok, uint32_t t, uint32_t nc, int n) {
-    const int d0 = (int)t - (int)nc;   // drafted number of bit 0
-    uint32_t see = ones(n);
-    if (d0 <= -32) return see;
-    if (!p.mask) return see & ones((int)tok - d0 + 1);
-    const uint32_t *mrow = p.mask + ((uint64_t)b * p.n_tokens + tok) * p.words;
-    auto word = [&](int k) -> uint32_t { return k >= 0 && k < (int)p.words ? mrow[k] : 0u; };
-    const int sft = d0 & 31, k0 = (d0 - sft) / 32;   // floor
-    const uint32_t m = sft ? (word(k0) >> sft) | (word(k0 + 1) << (32 - sft)) : word(k0);
-    return see & (m | ones(-d0));
 }
 
 }  // namespace vbs

@@ -25,7 +25,7 @@ namespace {
 
 constexpr int WT_SOFT = 256, WT_THREADS = WT_SOFT + 64;
 constexpr int WT_LOADER = WT_SOFT / 32, WT_ISSUER = WT_LOADER + 1;
-constexpr uint32_t WT_BLK = TREE_TC_SP * 128u, WT_TILES = 32;
+constexpr uint32_t WT_BLK = TREE_TC_SP * 128u, WT_TILES = 64;
 
 // words of the state behind the queries (bytes)
 constexpr uint32_t W_FULL = 0, W_EMPTY = 64, W_S = 128, W_F = 144, W_END = 160, W_TMEM = 168, W_BAD = 172, W_QMAX = 176;
@@ -71,9 +71,10 @@ __global__ void __launch_bounds__(WT_THREADS, 1) tree_weights_kernel(const __gri
     };
     auto all = [&](bool x) { return __all_sync(0xffffffffu, x); };
 
-    // item it: tile it % ntl for row tile it / ntl
-    auto load = [&](uint32_t it) {
-        const uint32_t s = it % wp.ns, tb = t0 + it % ntl * TREE_TC_SP;
+    // item: tile i in stage s, once per row tile (stages, phases and tiles are
+    // counted along: a division would cost an issuer more than a wait)
+    auto load = [&](uint32_t i, uint32_t s) {
+        const uint32_t tb = t0 + i * TREE_TC_SP;
         if (lane == 0) {
             mbar_arrive_expect_tx(base + W_FULL + 8 * s, slot);
             for (uint32_t k = 0; k < wp.blks; ++k)
@@ -97,7 +98,8 @@ __global__ void __launch_bounds__(WT_THREADS, 1) tree_weights_kernel(const __gri
             mbar_fence_init();
         }
         __syncwarp();
-        load(it++);
+        load(0, 0);
+        it = 1;
     } else if (warp == WT_ISSUER) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + W_TMEM), "r"(256u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -116,9 +118,11 @@ __global__ void __launch_bounds__(WT_THREADS, 1) tree_weights_kernel(const __gri
     const int32_t qmax = *reinterpret_cast<const int32_t *>(hs + W_QMAX);
 
     if (warp == WT_LOADER) {
-        for (; it < rts * ntl; ++it) {
-            if (!all(!*bad && (it < wp.ns || waits(base + W_EMPTY + 8 * (it % wp.ns), (it / wp.ns - 1) & 1u)))) break;
-            load(it);
+        for (uint32_t i = 1, s = 1, ph = 1; it < rts * ntl; ++it) {   // ph: parity of the last time round
+            if (i == ntl) i = 0;
+            if (s == wp.ns) { s = 0; ph ^= 1u; }
+            if (!all(!*bad && (it < wp.ns || waits(base + W_EMPTY + 8 * s, ph)))) break;
+            load(i++, s++);
         }
         if (*bad && lane == 0)   // copies may still be landing
             for (uint32_t k = it > wp.ns ? it - wp.ns : 0; k < it; ++k)
@@ -129,6 +133,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) tree_weights_kernel(const __gri
         const uint32_t lead = warp == WT_ISSUER ? tc_elect() : 0u;
         const float cap2 = p.cap * TREE_LOG2E;
         bool ok = true;
+        uint32_t s = 0, ph = 0, use[2] = {0, 0};   // issuer: stage and parity; uses of the accumulators
         for (uint32_t rt = 0; rt < rts; ++rt) {
             const uint32_t rows = min(wp.rows, R - rt * wp.rows), N = (rows + 15) / 16 * 16;
             if (warp < WT_LOADER) {
@@ -156,14 +161,15 @@ __global__ void __launch_bounds__(WT_THREADS, 1) tree_weights_kernel(const __gri
                 const uint32_t id = (1u << 4) | ((N >> 3) << 17) | ((TREE_TC_SP >> 4) << 24), qp = wp.rows * 16;
                 const uint64_t dk = tc_desc_sw(stage0, 16u, 1024u), dq = tc_desc(stage0 + wp.q_off, qp, 128u);
                 for (uint32_t i = 0; ok && i < ntl; ++i) {
-                    const uint32_t n = rt * ntl + i, s = n % wp.ns, sw = i & 1;
-                    const uint32_t use = rt * ((ntl + 1 - sw) / 2) + i / 2;   // of the stream's accumulator
-                    ok = all(!*bad && waits(base + W_FULL + 8 * s, (n / wp.ns) & 1u) && (!use || waits(base + W_F + 8 * sw, (use - 1) & 1u)));
+                    const uint32_t sw = i & 1;
+                    ok = all(!*bad && waits(base + W_FULL + 8 * s, ph) && (!use[sw] || waits(base + W_F + 8 * sw, (use[sw] - 1) & 1u)));
+                    ++use[sw];
                     if (!ok) break;
                     tc_after();
                     const uint64_t d = dk + s * (slot / 16);
-#pragma unroll 4
-                    for (uint32_t k = 0; k < hdp / 16; ++k) {
+#pragma unroll
+                    for (uint32_t k = 0; k < D / 16; ++k) {
+                        if (k >= hdp / 16) break;
                         const uint64_t da = d + (k >> 2) * (WT_BLK / 16) + (k & 3) * 2, db = dq + 2 * k * (qp / 16);
                         tc_mma_ss(tmem + 128 * sw, da, db + q_lo / 16, id, k ? 1u : 0u, lead);
                         tc_mma_ss(tmem + 128 * sw, da, db, id, 1u, lead);
@@ -173,19 +179,36 @@ __global__ void __launch_bounds__(WT_THREADS, 1) tree_weights_kernel(const __gri
                         tc_commit(base + W_EMPTY + 8 * s);
                     }
                     __syncwarp();
+                    if (++s == wp.ns) { s = 0; ph ^= 1u; }
                 }
             } else {
                 for (uint32_t i = w; ok && i < ntl; i += 2) {
-                    const uint32_t use = rt * ((ntl + 1 - w) / 2) + i / 2;
-                    ok = all(!*bad && waits(base + W_S + 8 * w, use & 1u));
-                    if (!ok) break;
-                    tc_after();
                     const uint32_t tb = t0 + i * TREE_TC_SP, t = tb + r, sa = tmem + ((32u * wq) << 16) + 128 * w;
                     const bool in = t < t1;
                     const int32_t kp = in ? tree_kpos(p, kpos, b, t, nc) : -1;
                     const bool seen = in && (!kpos || kp >= 0);            // by some row
                     const bool drafts = tb + TREE_TC_SP > nc;              // the mask decides
                     const bool edge = p.window && (kpos || drafts || qmax - (int32_t)tb >= (int32_t)p.window);
+                    // rows whose mask shows a drafted position, a bit each (before the wait)
+                    uint32_t rows_see[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
+                    if (drafts && in && t >= nc) {
+                        const uint32_t j = t - nc, g0 = rt * wp.rows;
+                        rows_see[0] = rows_see[1] = rows_see[2] = rows_see[3] = 0u;
+                        const uint32_t tok0 = tree_token(p, g0), tok1 = tree_token(p, g0 + rows - 1);
+#pragma unroll 4
+                        for (uint32_t k = tok0; k <= tok1; ++k) {
+                            const bool see = p.mask ? (p.mask[((uint64_t)b * p.n_tokens + k) * p.words + (j >> 5)] >> (j & 31)) & 1u : j <= k;
+                            // the token's rows of this tile
+                            const int lo = max(0, (int)(k * p.G) - (int)g0), hi = min((int)rows, (int)((k + 1) * p.G) - (int)g0);
+                            if (see)
+#pragma unroll
+                                for (int x = 0; x < 4; ++x) rows_see[x] |= ones(hi - 32 * x) & ~ones(lo - 32 * x);
+                        }
+                    }
+                    ok = all(!*bad && waits(base + W_S + 8 * w, use[0] & 1u));
+                    ++use[0];
+                    if (!ok) break;
+                    tc_after();
                     float sum = 0.f;
                     if (!drafts && !edge && !p.slopes && !(p.cap > 0.f)) {
 #pragma unroll 1
@@ -204,17 +227,19 @@ __global__ void __launch_bounds__(WT_THREADS, 1) tree_weights_kernel(const __gri
                         for (uint32_t c = 0; c < N; c += 8) {
                             uint32_t x[8];
                             tc_ld8(sa + c, x);
+                            const uint32_t bits = (c < 64 ? (c < 32 ? rows_see[0] : rows_see[1]) : (c < 96 ? rows_see[2] : rows_see[3])) >> (c & 31);
                             tc_wait_ld(x);
+                            float y[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(x[e]) * row_fl[c + e].x;
+                            if (p.cap > 0.f) tree_cap_all(y, cap2);
 #pragma unroll
                             for (int e = 0; e < 8; ++e) {
                                 const float2 fl = row_fl[c + e];
                                 const int2 ps = row_ps[c + e];
-                                float v = __uint_as_float(x[e]) * fl.x;
-                                if (p.cap > 0.f) v = tree_cap(v, cap2);
+                                float v = y[e];
                                 if (p.slopes) v = fmaf(__int_as_float(ps.y), (float)(kp - ps.x), v);
-                                bool see = c + e < rows && (!p.window || ps.x - kp < (int32_t)p.window);
-                                if (drafts && see)
-                                    see = t < nc || (tree_sees(p, b, tree_token(p, rt * wp.rows + c + e), t, nc, 1) & 1u);
+                                const bool see = c + e < rows && ((bits >> e) & 1u) && (!p.window || ps.x - kp < (int32_t)p.window);
                                 sum += see ? ex2(v - fl.y) : 0.f;
                             }
                         }
@@ -272,8 +297,8 @@ cudaError_t tree_weights_launch(const TreeParams &t, const CUtensorMap &km, uint
     // one CTA per SM: as many tiles each as that takes, at most WT_TILES
     const uint32_t tiles = (t.ctx_limit + TREE_TC_SP - 1) / TREE_TC_SP;
     const uint64_t units = (uint64_t)t.nkh * n_seqs;
-    const uint32_t parts = (uint32_t)std::max<uint64_t>(1, n_sm / units);
-    p.per = std::min(WT_TILES, (tiles + parts - 1) / parts);
+    const uint32_t parts = std::max((uint32_t)std::max<uint64_t>(1, n_sm / units), (tiles + WT_TILES - 1) / WT_TILES);
+    p.per = (tiles + parts - 1) / parts;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;

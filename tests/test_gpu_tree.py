@@ -372,3 +372,22 @@ def test_a_late_maximum_moves_the_reference(case):
         c.q[..., 0] = 1.0 / c.scale
         c.k[0, 0, :, 0] = ramp.astype(np.float16)
         c.check()
+
+
+@pytest.mark.parametrize("tokens,nqh,nkh,hd,seqs,n_ctx", [(16, 8, 2, 128, 3, 9000), (64, 8, 1, 64, 4, 5000), (1, 2, 2, 128, 2, 9000),
+                                                          (3, 4, 1, 256, 2, 6000), (40, 32, 8, 96, 8, 2600)])
+def test_long_sums_do_not_drift(case, tokens, nqh, nkh, hd, seqs, n_ctx):
+    """Thousands of accumulations: the tensor cores cut their accumulators
+    towards zero, by up to a unit of the last place (2^-23 of the value) each.
+    An accumulator takes 16 of them (8 of 16 positions, two halves) while it
+    grows evenly: 16 * 2^-24 = 9.5e-7 of the result, whatever the context's
+    length; left to run over 9000 positions it would reach 35 times that. As
+    much again for the scores' accumulators (8 of high halves) and for the
+    products' and exponentials' 2^-22."""
+    c = case(seqs=seqs, tokens=tokens, nqh=nqh, nkh=nkh, hd=hd, n_ctx=(n_ctx,), seed=hd + tokens)
+    c.q[..., 0] = 0.0
+    c.v[..., :] += np.float16(2.0)          # values of one sign: a cut shows as a bias
+    got, (want, _) = c.run(), c.want()
+    bias = ((got - want) / want).mean()
+    assert abs(bias) < 2 * 16 * 2.0 ** -24 + 2.0 ** -21
+    np.testing.assert_allclose(got, want, rtol=0, atol=8 * TOL)

@@ -26,6 +26,11 @@
 //  * The softmax reference stays 6 below the running maximum (log2 units), so
 //    weights are 2^6 at the first and at most 2^14 before a rescale: small
 //    weights keep their low half above fp16's smallest numbers.
+//  * The tensor cores cut their accumulators instead of rounding them: every
+//    accumulation loses half a unit of the last place towards zero, 480 of them
+//    8.5e-6 of the result. Each block's sum therefore starts at zero and is
+//    added to the running one in fp32, and the low halves' part of a score,
+//    small as it is, has an accumulator of its own.
 //  * A block where some row does not see some key takes the masked path, which
 //    also looks for infinities and NaN among its values: 0 * inf would carry
 //    them into rows that do not see them, so such a block adds its values
@@ -195,7 +200,7 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
         if (!__all_sync(0xffffffffu, !*bad && waits(full0 + 8 * (c % C::NST), (c / C::NST) & 1u))) break;
         {
             const uint32_t kst = st + 16 * (j & 3) * 128, vst = kst + C::HALF, sw = lane & 7;
-            float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, sl[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
             for (int kk = 0; kk < HD / 16; kk += 2) {
                 if (kk >= (int)kks) break;
@@ -215,14 +220,16 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
                 for (int j = 0; j < 2; ++j) {
                     uint32_t b0, b1, b2, b3;
                     ldsm_x4(kst + (kk >> 2) * C::BOX + (8 * j + (lane & 7)) * 128 + ((((2 * kk) & 7) + (lane >> 3)) ^ sw) * 16, b0, b1, b2, b3);
-                    mma_f16_acc(s[j], al[0], b0, b1);
+                    mma_f16_acc(sl[j], al[0], b0, b1);
                     mma_f16_acc(s[j], ah[0], b0, b1);
-                    mma_f16_acc(s[j], al[1], b2, b3);
+                    mma_f16_acc(sl[j], al[1], b2, b3);
                     mma_f16_acc(s[j], ah[1], b2, b3);
                 }
             }
             // x[h][e]: row h, keys tb + {qd, qd+1, 8+qd, 9+qd}
-            float x[2][4] = {{s[0][0], s[0][1], s[1][0], s[1][1]}, {s[0][2], s[0][3], s[1][2], s[1][3]}};
+            const float x00 = s[0][0] + sl[0][0], x01 = s[0][1] + sl[0][1], x02 = s[1][0] + sl[1][0], x03 = s[1][1] + sl[1][1];
+            const float x10 = s[0][2] + sl[0][2], x11 = s[0][3] + sl[0][3], x12 = s[1][2] + sl[1][2], x13 = s[1][3] + sl[1][3];
+            float x[2][4] = {{x00, x01, x02, x03}, {x10, x11, x12, x13}};
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -301,10 +308,13 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
                     uint32_t b0, b1, b2, b3;
                     ldsm_x4_trans(vst + (n >> 3) * C::BOX + ((lane & 7) + 8 * ((lane >> 3) & 1)) * 128 + (((n & 7) + (lane >> 4)) ^ sw) * 16, b0,
                                   b1, b2, b3);
-                    mma_f16_acc(o[n], pl, b0, b1);
-                    mma_f16_acc(o[n], ph, b0, b1);
-                    mma_f16_acc(o[n + 1], pl, b2, b3);
-                    mma_f16_acc(o[n + 1], ph, b2, b3);
+                    float u0[4] = {0.f, 0.f, 0.f, 0.f}, u1[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma_f16_acc(u0, pl, b0, b1);
+                    mma_f16_acc(u0, ph, b0, b1);
+                    mma_f16_acc(u1, pl, b2, b3);
+                    mma_f16_acc(u1, ph, b2, b3);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { o[n][e] += u0[e]; o[n + 1][e] += u1[e]; }
                 }
             } else {
 #pragma unroll 1
@@ -584,7 +594,7 @@ static TreePlan tree_plan(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t, int n_s
     pl.tile_rows = hd > 128 && pl.rows > 16 ? 32 : 16;
     TreeParts best = hd > 128 ? tree_parts(heads * tiles(pl.tile_rows), n_sm, span, 64, 25, 4000, 2000)
                               : tree_parts(heads * tiles(16), 2ull * n_sm, span, 64, hd > 64 ? 40 : 20, 2500, 2000);
-    if (hd <= 128) {
+    if (hd <= 128 && pl.rows > 16) {   // (16 rows are one CTA's of the mma kernel: 73.7 us for 16 x 4096 positions x 8 heads, the other 88.4)
         const uint32_t wide = pl.rows > TREE_TC_ROWS;
         const TreeParts tc = tree_parts(heads * tiles(TREE_TC_ROWS << wide), n_sm, span, TREE_TC_SP,
                                         (hd > 64 ? 16 : 13) << wide, wide ? 13000 : 9000, 3000);

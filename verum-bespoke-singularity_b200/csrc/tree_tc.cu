@@ -22,8 +22,13 @@
 //    maximum, and again, 16 columns at a time, for the weights, which go back
 //    over them as fp16 halves (columns 32 c .. + 15 the high, + 16 .. + 31
 //    the low halves of positions 32 c ..) and are announced 64 positions at a
-//    time. The accumulator is rescaled in place when the maximum moves by
-//    more than TREE_LAZY.
+//    time. The sums are rescaled when the maximum moves by more than TREE_LAZY.
+//  * The tensor cores cut accumulators instead of rounding them, towards zero:
+//    left in tensor memory over 30 tiles a result lost 8.5e-6 (zero-mean
+//    values; 1.5e-5 and more with values of one sign). So an accumulator lives
+//    for one tile, the rows' threads add it to their fp32 sums in registers
+//    (setmaxnreg gives them 232), and a score's low halves go first, while its
+//    accumulator is small.
 // All waits are bounded; after one ran out the CTA flags the device error
 // word, waits for its copies and products, frees its tensor memory and ends.
 #include "tree_tc.cuh"
@@ -34,8 +39,11 @@ namespace vbs {
 
 namespace {
 
-constexpr int TC_SOFT = 256, TC_THREADS = TC_SOFT + 96;   // softmax warps, the loader, the issuers of Q K^T and of P V
+constexpr int TC_SOFT = 256, TC_THREADS = TC_SOFT + 128;   // softmax warps; the loader, the issuers of Q K^T and of P V, one idle
 constexpr int TC_LOADER = TC_SOFT / 32, TC_QK = TC_LOADER + 1, TC_PV = TC_LOADER + 2;
+// registers: 384 x 168 at the launch = 256 x 232 + 128 x 40 (64,512 each)
+constexpr int TC_REGS_SOFT = 232, TC_REGS_OTHER = 40;
+static_assert(TC_SOFT * TC_REGS_SOFT + (TC_THREADS - TC_SOFT) * TC_REGS_OTHER <= TC_THREADS * 168, "more than launched waits forever");
 constexpr uint32_t TC_BLK = TREE_TC_SP * 128u;   // one box: 128 positions x 64 dims
 
 // words of the state behind the queries (bytes); barriers first
@@ -106,7 +114,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
         return false;
     };
     auto all = [&](bool x) { return __all_sync(0xffffffffu, x); };
-
     // ---------------- loader: items K0 V0 K1 V1 ... ------------------------
     // (stages and phases are counted along: a division would cost an issuer more than a wait)
     auto load = [&](uint32_t it, uint32_t s) {
@@ -138,7 +145,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
             for (uint32_t r = lane; r < nrows; r += 32) hi = max(hi, tree_qpos(p, b, tree_token(p, R0 + r), nc));
         hi = __reduce_max_sync(0xffffffffu, hi);
         if (lane == 0) *reinterpret_cast<int32_t *>(hs + H_QMAX) = hi;
-    } else {
+    } else if (warp < TC_LOADER) {
         // 8 rows at a time, two times 8 per warp and 128 rows; places of rows
         // that are not there keep what they hold (nobody reads their scores)
 #pragma unroll 1
@@ -157,7 +164,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
     __syncthreads();
     tc_after();
     const uint32_t tmem = *reinterpret_cast<uint32_t *>(hs + H_TMEM);
-
+    // the warpgroup of the loader and the issuers gives its registers away
+    if (warp >= TC_LOADER) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TC_REGS_OTHER));
     if (warp == TC_LOADER) {
         for (uint32_t s = 1, ph = 1; it < 2 * nch; ++it) {   // ph: parity of the last time round
             if (!all(!*bad && (it < tp.ns || waits(base + H_EMPTY + 8 * s, ph)))) break;
@@ -187,9 +196,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
 #pragma unroll
             for (uint32_t k = 0; k < 8; ++k) {
                 if (k >= hdp / 16) break;
-                const uint64_t db = d + (k >> 2) * (TC_BLK / 16) + (k & 3) * 2;
-                tc_mma_ss(tmem + 128 * w, dq + qlo + 2 * k * (QCH / 16), db, idq, k ? 1u : 0u, lead);
-                tc_mma_ss(tmem + 128 * w, dq + 2 * k * (QCH / 16), db, idq, 1u, lead);
+                tc_mma_ss(tmem + 128 * w, dq + qlo + 2 * k * (QCH / 16), d + (k >> 2) * (TC_BLK / 16) + (k & 3) * 2, idq, k ? 1u : 0u, lead);
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) {
+                if (k >= hdp / 16) break;
+                tc_mma_ss(tmem + 128 * w, dq + 2 * k * (QCH / 16), d + (k >> 2) * (TC_BLK / 16) + (k & 3) * 2, idq, 1u, lead);
             }
             if (lead) {
                 tc_commit(base + H_S + 8 * w);
@@ -215,7 +227,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
             tc_after();
             const uint64_t d = dv + s * (slot / 16);
             const uint32_t o = tmem + 256 + 128 * w, pa = tmem + 128 * w;
-            const uint32_t acc0 = n >= 2 ? 1u : reinterpret_cast<volatile uint32_t *>(hs + H_ACC)[w];
+            // every tile its own accumulator, unless the softmax put something there itself
+            const uint32_t acc0 = reinterpret_cast<volatile uint32_t *>(hs + H_ACC)[w];
             const uint32_t ks = (min(TREE_TC_SP, t1 - t0 - i * TREE_TC_SP) + 15) / 16;
 #pragma unroll
             for (uint32_t k = 0; k < TREE_TC_SP / 16; ++k) {
@@ -239,7 +252,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
         }
         if (lead) tc_commit(base + H_END);
         __syncwarp();
+    }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TC_REGS_SOFT));
         // ---------------- softmax: stream w, row = thread --------------------
         const uint32_t w = warp >> 2, wq = warp & 3, r = 32 * wq + lane;
         const uint32_t ri = two && w ? TREE_TC_ROWS + r : r;   // row of the tile
@@ -252,6 +267,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
         const float slope = p.slopes ? p.slopes[head] * TREE_LOG2E : 0.f;
         const int32_t *kpos = p.k_pos ? p.k_pos + (uint64_t)(p.k_pos_per_head ? b * p.nkh + kvh : b) * p.max_ctx : nullptr;
         float mref = -INFINITY;
+        float o[128];   // the row's sums
+#pragma unroll
+        for (int k = 0; k < 128; ++k) o[k] = 0.f;
+        auto gather = [&]() {   // the tile's accumulator into the sums
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (32 * c >= (int)hdp) break;
+                uint32_t x[32];
+                tc_ld32(oa + 32 * c, x);
+                tc_wait_ld(x);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[32 * c + k] += __uint_as_float(x[k]);
+            }
+        };
         float2 l = make_float2(0.f, 0.f);
         bool dead = false;
         // the threads that look at one tile's values together: a stream, or
@@ -298,6 +327,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                 continue;
             }
             tc_after();
+            // the last tile's accumulator (its product is done: this step's
+            // scores were computed behind it)
+            if (n >= 2) gather();
+            if (r == 0) reinterpret_cast<volatile uint32_t *>(hs + H_ACC)[w] = 0;
             // plain: the scores as the product left them, times the row's factor;
             // simple: capped, or with slope * (slot - query position) added
             const bool linear = p.slopes && !kpos, simple = whole && (!p.slopes || linear);
@@ -417,14 +450,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                         odd = zero != 0u;
                     }
                     if (bar_or(bar, bar_n, odd)) {
-                        // rare: the rows that see such values add them here,
-                        // then they become zeros for the product
+                        // rare: the rows that see such values put their part into
+                        // the accumulator, then they become zeros for the product
                         const float nm = mx > mref + TREE_LAZY ? mx - TREE_BELOW : mref;
                         const float bs = nm == -INFINITY ? 0.f : nm;
                         for (uint32_t c = 0; c < chunks; ++c) {
-                            uint32_t o[8];
-                            if (n >= 2) { tc_ld8(oa + 8 * c, o); tc_wait_ld(o); }
-                            else for (int k = 0; k < 8; ++k) o[k] = 0u;
+                            uint32_t y[8];
+                            for (int k = 0; k < 8; ++k) y[k] = 0u;
                             for (int j = 0; j < nval; ++j) {
                                 const uint4 v = lds_u128(va + (c >> 3) * TC_BLK + j * 128 + (((c & 7) ^ (j & 7)) << 4));   // the same for all lanes
                                 if (!(not_finite2(v.x) || not_finite2(v.y) || not_finite2(v.z) || not_finite2(v.w))) continue;
@@ -437,14 +469,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                                 for (int k = 0; k < 8; ++k) {
                                     const uint32_t h = (vv[k >> 1] >> (16 * (k & 1))) & 0xFFFFu;
                                     if ((h & 0x7C00u) == 0x7C00u && x != -INFINITY)
-                                        o[k] = __float_as_uint(__uint_as_float(o[k]) + pr * f16f(h));
+                                        y[k] = __float_as_uint(__uint_as_float(y[k]) + pr * f16f(h));
                                 }
                                 __syncwarp();
                             }
-                            tc_st8(oa + 8 * c, o);
+                            tc_st8(oa + 8 * c, y);
                         }
                         tc_wait_st();
-                        if (n < 2 && r == 0) reinterpret_cast<volatile uint32_t *>(hs + H_ACC)[w] = 1;
+                        if (r == 0) reinterpret_cast<volatile uint32_t *>(hs + H_ACC)[w] = 1;
                         bar_or(bar, bar_n, false);   // all have read them
                         for (uint32_t k = bar_r; k < slot / 16; k += bar_n) {
                             uint4 v = lds_u128(va + k * 16);
@@ -461,27 +493,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                     }
                 }
             }
-            // running reference; the accumulator follows when it moves
+            // running reference; the sums follow when it moves
             const bool moves = mx > mref + TREE_LAZY;
             if (__any_sync(0xffffffffu, moves)) {
-                float f = 1.f;
-                if (moves) {
-                    f = mref == -INFINITY ? 1.f : ex2(mref - (mx - TREE_BELOW));   // nothing seen before: nothing to scale
-                    mref = mx - TREE_BELOW;
-                    l.x *= f;
-                    l.y *= f;
-                }
-                if (n >= 2) {
-#pragma unroll 1
-                    for (uint32_t c = 0; c < chunks; ++c) {
-                        uint32_t o[8];
-                        tc_ld8(oa + 8 * c, o);
-                        tc_wait_ld(o);
+                const float f = !moves ? 1.f : ex2(mref - (mx - TREE_BELOW));   // 0 on the first tile
+                if (moves) mref = mx - TREE_BELOW;
+                l.x *= f;
+                l.y *= f;
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                        tc_st8(oa + 8 * c, o);
-                    }
-                }
+                for (int k = 0; k < 128; ++k) o[k] *= f;
             }
             const float f1 = plain ? fac : 1.f, b1 = mref == -INFINITY ? 0.f : mref;
             const float2 f = make_float2(f1, f1), bs = make_float2(-b1, -b1);
@@ -518,52 +538,58 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
         // ---------------- out --------------------------------------------------
         const bool ok = all(waits(base + H_END, 0) && !*bad);
         tc_after();
-        float L = l.x + l.y, M = mref, f0 = 1.f, f1 = 0.f;
-        const bool join = !two && nch > 1;   // the two streams had the same rows
+        if (active && ok && w < steps) gather();
+        float L = l.x + l.y, M = mref;
+        const bool join = !two && nch > 1;   // the two streams had the same rows: each ends half of the dims
+        const uint32_t half = join ? (p.hd / 8 + 1) / 2 * 8 : 0u;   // stream 0: below
         if (join) {
+            const uint32_t pitch = 128 * 4 + 16;   // a row's bytes: conflict-free for a thread per row
             float2 *ml_sm = reinterpret_cast<float2 *>(smem);   // over the stages: all products are done
+            float *rows_sm = reinterpret_cast<float *>(smem + 2 * TREE_TC_ROWS * 8 + r * pitch);
             ml_sm[w * TREE_TC_ROWS + r] = make_float2(active ? M : -INFINITY, active ? L : 0.f);
+#pragma unroll
+            for (int c = 0; c < 128; c += 8) {   // the other stream's half goes over
+                if (c >= (int)p.hd || (w == 0) == (c < (int)half)) continue;
+                *reinterpret_cast<float4 *>(rows_sm + c) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+                *reinterpret_cast<float4 *>(rows_sm + c + 4) = make_float4(o[c + 4], o[c + 5], o[c + 6], o[c + 7]);
+            }
             named_bar_sync(4, TC_SOFT);
-            const float2 a = ml_sm[r], c = ml_sm[TREE_TC_ROWS + r];
+            const float2 a = ml_sm[w * TREE_TC_ROWS + r], c = ml_sm[(w ^ 1) * TREE_TC_ROWS + r];
             M = fmaxf(a.x, c.x);
-            f0 = a.x == -INFINITY ? 0.f : ex2(a.x - M);
-            f1 = c.x == -INFINITY ? 0.f : ex2(c.x - M);
+            const float f0 = a.x == -INFINITY ? 0.f : ex2(a.x - M), f1 = c.x == -INFINITY ? 0.f : ex2(c.x - M);
             L = a.y * f0 + c.y * f1;
+#pragma unroll
+            for (int d = 0; d < 128; d += 4) {
+                if (d >= (int)p.hd || (w == 0) != (d < (int)half)) continue;
+                const float4 x = *reinterpret_cast<const float4 *>(rows_sm + d);
+                o[d] = fmaf(x.x, f1, o[d] * f0);
+                o[d + 1] = fmaf(x.y, f1, o[d + 1] * f0);
+                o[d + 2] = fmaf(x.z, f1, o[d + 2] * f0);
+                o[d + 3] = fmaf(x.w, f1, o[d + 3] * f0);
+            }
         }
-        // all dims of a row, or joined half of them
-        if (active && ok && (two || join || w == 0)) {
+        if (active && ok && on && (two || join || w == 0)) {
             const bool many = p.n_splits > 1;
             const float il = many ? 1.f : (L == 0.f ? 0.f : 1.f / L);
             float *dst = many ? p.part_o + ((slot_id * p.n_splits + split) * TR + ri) * p.hd
                               : p.out + (((uint64_t)b * p.n_tokens + tok) * p.nqh + head) * p.hd;
-            const uint32_t cpr = p.hd / 8, c0 = join && w ? cpr / 2 : 0u, c1 = join && !w ? cpr / 2 : cpr;
-            const uint32_t o0 = tmem + ((32u * wq) << 16) + 256 + (join ? 0u : 128u * w);
             const bool wide = (reinterpret_cast<uintptr_t>(dst) & 31) == 0;
             // straight from the rows' threads, a whole 32-byte sector each
-#pragma unroll 2
-            for (uint32_t c8 = c0; c8 < c1; ++c8) {
-                uint32_t x[8], y[8];
-                tc_ld8(o0 + 8 * c8, x);
-                if (join) tc_ld8(o0 + 128 + 8 * c8, y);
-                tc_wait_ld(x);
-                if (join) tc_wait_ld(y);
+#pragma unroll
+            for (int c = 0; c < 128; c += 8) {
+                if (c >= (int)p.hd || (join && (w == 0) != (c < (int)half))) continue;
                 float v[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    v[k] = __uint_as_float(x[k]) * f0;
-                    if (join) v[k] = fmaf(__uint_as_float(y[k]), f1, v[k]);
-                    v[k] = !many && L == 0.f ? 0.f : v[k] * il;
+                for (int k = 0; k < 8; ++k) v[k] = !many && L == 0.f ? 0.f : o[c + k] * il;
+                if (wide) {
+                    asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + c), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
+                                 "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
+                } else {
+                    *reinterpret_cast<float4 *>(dst + c) = make_float4(v[0], v[1], v[2], v[3]);
+                    *reinterpret_cast<float4 *>(dst + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
                 }
-                if (on && wide) {
-                    asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + 8 * c8), "f"(v[0]), "f"(v[1]), "f"(v[2]),
-                                 "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
-                } else if (on) {
-                    *reinterpret_cast<float4 *>(dst + 8 * c8) = make_float4(v[0], v[1], v[2], v[3]);
-                    *reinterpret_cast<float4 *>(dst + 8 * c8 + 4) = make_float4(v[4], v[5], v[6], v[7]);
-                }
-                __syncwarp();
             }
-            if (on && (two || w == 0)) {
+            if (two || w == 0) {
                 if (many) ml[ri] = make_float2(M, L);
                 else if (p.lse) p.lse[(uint64_t)(b * p.nkh + kvh) * (p.n_tokens * p.G) + rr] = L == 0.f ? -INFINITY : M + log2f(L);
             }

@@ -171,7 +171,12 @@ __global__ void __launch_bounds__(WT_THREADS, 1) tree_weights_kernel(const __gri
                     for (uint32_t k = 0; k < D / 16; ++k) {
                         if (k >= hdp / 16) break;
                         const uint64_t da = d + (k >> 2) * (WT_BLK / 16) + (k & 3) * 2, db = dq + 2 * k * (qp / 16);
-                        tc_mma_ss(tmem + 128 * sw, da, db + q_lo / 16, id, k ? 1u : 0u, lead);
+                        tc_mma_ss(tmem + 128 * sw, da, db + q_lo / 16, id, k ? 1u : 0u, lead);   // the small part first (tree_tc.cu)
+                    }
+#pragma unroll
+                    for (uint32_t k = 0; k < D / 16; ++k) {
+                        if (k >= hdp / 16) break;
+                        const uint64_t da = d + (k >> 2) * (WT_BLK / 16) + (k & 3) * 2, db = dq + 2 * k * (qp / 16);
                         tc_mma_ss(tmem + 128 * sw, da, db, id, 1u, lead);
                     }
                     if (lead) {

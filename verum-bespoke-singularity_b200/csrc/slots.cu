@@ -41,7 +41,7 @@ bool kv_desc_ok(const vbs_cu_kv_t *kv) {
 // (and, for few tokens, over blockIdx.y), and the loads of ROPE_U heads are
 // issued before the first is used, the first ones before the angles.
 // ---------------------------------------------------------------------------
-constexpr int ROPE_THREADS = 256, ROPE_U = 4;
+constexpr int ROPE_THREADS = 128, ROPE_U = 2;   // 4093 tokens of 64 + 16 heads of 128: 67.3 us; 256 and 4: 79.4, 128 and 4: 70.7
 
 struct RopeParams {
     vbs_cu_rope_t r;
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(SEL_THREADS) cache_select_kernel(const SelectP
 
 // ---------------------------------------------------------------------------
 // Row moves. Bound by memory: every row is read once and written once.
-// Apart: a thread moves 16-byte pieces of K and V of GA_U rows, all loads
+// Apart: a thread moves 16-byte pieces of K and V of GX_U rows, all loads
 // before the first store. In place: rows only move down, so a CTA takes its
 // list in ascending batches (all of a batch's loads, a barrier, its stores);
 // the pieces of a row are independent of one another, so slices of the row
@@ -455,6 +455,7 @@ __global__ void __launch_bounds__(SEL_THREADS) cache_select_kernel(const SelectP
 // CTA per list.
 // ---------------------------------------------------------------------------
 constexpr uint32_t GA_THREADS = 256, GA_U = 4, GA_WARP_MAX = 64;
+constexpr uint32_t GX_THREADS = 128, GX_U = 2;   // apart: 90.4 us for 32 x 8 lists of 2048 of 8192 rows of 256 bytes (256 and 4: 129, 256 and 2: 96.2)
 
 struct GatherSide {
     uint16_t *k, *v;
@@ -495,19 +496,19 @@ __device__ __forceinline__ bool gather_list(const GatherParams &p, uint32_t list
     return true;
 }
 
-__global__ void __launch_bounds__(GA_THREADS) gather_apart_kernel(const __grid_constant__ GatherParams p, uint32_t nblk) {
+__global__ void __launch_bounds__(GX_THREADS) gather_apart_kernel(const __grid_constant__ GatherParams p, uint32_t nblk) {
     // the heads of the same rows are neighbours in launch order: in the
     // engine's order their rows are neighbours in memory
     const uint32_t h = blockIdx.x % p.n_kv_heads, x = blockIdx.x / p.n_kv_heads;
-    const uint32_t list = x / nblk * p.n_kv_heads + h, rp = GA_THREADS / p.cpr;
+    const uint32_t list = x / nblk * p.n_kv_heads + h, rp = GX_THREADS / p.cpr;
     GatherList l;
     if (!gather_list(p, list, l)) return;
-    const uint32_t ch = threadIdx.x % p.cpr, r0 = x % nblk * (rp * GA_U) + threadIdx.x / p.cpr;
+    const uint32_t ch = threadIdx.x % p.cpr, r0 = x % nblk * (rp * GX_U) + threadIdx.x / p.cpr;
     if (threadIdx.x >= rp * p.cpr) return;
-    int64_t from[GA_U];
-    uint4 k[GA_U], v[GA_U];
+    int64_t from[GX_U];
+    uint4 k[GX_U], v[GX_U];
 #pragma unroll
-    for (uint32_t u = 0; u < GA_U; ++u) {
+    for (uint32_t u = 0; u < GX_U; ++u) {
         const uint32_t i = r0 + u * rp;
         from[u] = i < l.n ? l.src0 + l.idx[i] : -1;
         if (i < l.n && (from[u] < 0 || from[u] >= (int64_t)p.src.max_ctx)) {
@@ -516,14 +517,14 @@ __global__ void __launch_bounds__(GA_THREADS) gather_apart_kernel(const __grid_c
         }
     }
 #pragma unroll
-    for (uint32_t u = 0; u < GA_U; ++u) {
+    for (uint32_t u = 0; u < GX_U; ++u) {
         if (from[u] < 0) continue;
         const uint64_t o = l.so + (uint64_t)from[u] * p.src.pos_step + ch * 8;
         k[u] = *reinterpret_cast<const uint4 *>(p.src.k + o);
         v[u] = *reinterpret_cast<const uint4 *>(p.src.v + o);
     }
 #pragma unroll
-    for (uint32_t u = 0; u < GA_U; ++u) {
+    for (uint32_t u = 0; u < GX_U; ++u) {
         if (from[u] < 0) continue;
         const uint64_t to = (uint64_t)l.dst0 + r0 + u * rp;
         const uint64_t o = l.dof + to * p.dst.pos_step + ch * 8;
@@ -847,14 +848,14 @@ int vbs_cu_cache_gather(const vbs_cu_kv_t *src, const vbs_cu_kv_t *dst, const vb
         p.slice = std::max(std::min(4u, p.cpr), (p.cpr + want - 1) / want);
         gather_inplace_kernel<<<dim3((unsigned)lists, (p.cpr + p.slice - 1) / p.slice), GA_THREADS, 0, st>>>(p);
     } else {
-        const uint32_t rows = GA_THREADS / p.cpr * GA_U;
+        const uint32_t rows = GX_THREADS / p.cpr * GX_U;
         const uint64_t nblk = (std::min(g->n_max, dst->max_ctx) + rows - 1) / rows;
         if (lists * nblk > 0x7FFFFFFFull) {
             latch_error("vbs_cu_cache_gather: %llu lists of %u rows are too many for one call", (unsigned long long)lists,
                         g->n_max);
             return -1;
         }
-        gather_apart_kernel<<<(unsigned)(lists * nblk), GA_THREADS, 0, st>>>(p, (uint32_t)nblk);
+        gather_apart_kernel<<<(unsigned)(lists * nblk), GX_THREADS, 0, st>>>(p, (uint32_t)nblk);
     }
     return cuda_ok(cudaGetLastError(), "cache_gather") ? 0 : -1;
 }

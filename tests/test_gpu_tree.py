@@ -391,3 +391,135 @@ def test_long_sums_do_not_drift(case, tokens, nqh, nkh, hd, seqs, n_ctx):
     bias = ((got - want) / want).mean()
     assert abs(bias) < 2 * 16 * 2.0 ** -24 + 2.0 ** -21
     np.testing.assert_allclose(got, want, rtol=0, atol=8 * TOL)
+
+
+# ---- the tcgen05 kernel on short lengths -------------------------------------
+# The kernel is chosen by ctx_limit, not by the lengths: a large limit sends
+# more than 16 rows of a KV head (head_dim up to 128) to the tcgen05 kernel
+# whatever the sequences hold, in many parts, most of them empty; many
+# sequences send them there in few.
+FAR = dict(limit=20000, spare=0)
+
+
+@pytest.mark.parametrize("hd", [8, 24, 64, 72, 80, 128])
+@pytest.mark.parametrize("n_ctx,tokens", [(0, 9), (0, 130), (90, 33), (127, 17), (128, 64), (1000, 40)])
+def test_far_limit(case, hd, n_ctx, tokens):
+    case(tokens=tokens, nqh=4, nkh=2, hd=hd, n_ctx=(n_ctx,), tree=True, head_major=hd % 3 == 0, seed=hd + tokens, **FAR).check()
+
+
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("tokens,nqh", [(18, 2), (33, 6), (64, 4), (65, 8), (150, 2)])
+def test_far_limit_ragged(case, tokens, nqh, weights):
+    case(seqs=4, tokens=tokens, nqh=nqh, nkh=2, hd=64, n_ctx=(0, 260, 17, 128), n_tok=[tokens, 1, 0, tokens - 1], tree=True, seed=tokens,
+         limit=12000, spare=0).check(weights)
+
+
+@pytest.mark.parametrize("cap,slopes,window,qscale", [(30.0, False, 0, 4.0), (0.0, True, 0, 1.0), (5.0, True, 100, 6.0), (50.0, True, 0, 1.0)])
+@pytest.mark.parametrize("k_pos", [None, padded, evicted])
+def test_far_limit_options(case, cap, slopes, window, qscale, k_pos):
+    case(seqs=2, tokens=21, nqh=8, nkh=2, hd=128, n_ctx=(300, 600), cap=cap, slopes=slopes, window=window, qscale=qscale, tree=True,
+         pos=0 if k_pos is None else 700, k_pos=k_pos, seed=41, limit=12000, spare=0).check(weights=True)
+
+
+@pytest.mark.parametrize("window", [1, 60, 129, 700])
+@pytest.mark.parametrize("tree", [False, True])
+def test_many_sequences_window(case, window, tree):
+    """Few parts: a window's edge inside tiles, its first tile behind others."""
+    case(seqs=20, tokens=24, nqh=16, nkh=8, hd=64, n_ctx=(900, 333, 5), window=window, tree=tree, pos=0 if tree else None, seed=window).check()
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("hd,tokens", [(64, 37), (96, 37), (128, 37), (128, 100)])
+def test_far_limit_masked_places(case, bad, hd, tokens):
+    c = case(seqs=2, tokens=tokens, nqh=4, nkh=2, hd=hd, n_ctx=(400, 3), pos=0, tree=True, k_pos=lambda rng, c: padded(rng, c),
+             head_major=hd == 96, seed=5, limit=12000, spare=0)
+    c.sees[:, :, 2] = False
+    for x in (c.k, c.v):
+        for b in range(2):
+            end = c.n_ctx[b] + c.n_tok[b]
+            x[b, :, end:] = bad
+            x[b, :, c.n_ctx[b] + 2] = bad
+            x[b, :, :end][:, c.k_pos[b, :end] < 0] = bad
+    c.check(weights=True)
+    # visible to some rows of some tiles: theirs turn, the others stay
+    c = case(tokens=tokens, nqh=4, nkh=1, hd=hd, n_ctx=(300,), tree=True, seed=6, limit=30000, spare=0)
+    c.sees[0] = np.eye(tokens, dtype=bool)
+    c.sees[0, :, 0] = True
+    c.v[0, 0, 307, 3] = bad                      # one row sees it
+    c.v[0, 0, 300 + tokens - 1, hd - 1] = bad    # the last
+    got, (want, _) = c.run(), c.want()
+    turned = ~np.isfinite(want)
+    assert turned.sum() == 2 * 4 and (np.isnan(got) == np.isnan(want)).all() and (got[np.isinf(want)] == want[np.isinf(want)]).all()
+    np.testing.assert_allclose(got[~turned], want[~turned], rtol=0, atol=4 * TOL)
+
+
+def test_far_limit_rows_that_see_nothing(case):
+    c = case(tokens=30, nqh=4, nkh=2, hd=128, n_ctx=(0,), tree=True, seed=1, **FAR)
+    c.sees[0, 3] = False
+    c.sees[0, 20:] = False
+    out = c.check(weights=True)
+    assert (out[0, 3] == 0).all() and (out[0, 20:] == 0).all()
+    c = case(tokens=40, nqh=4, nkh=1, hd=128, n_ctx=(3000,), k_pos=lambda rng, c: np.full((1, c.M), -1), pos=0, seed=2, **FAR)
+    out = c.check(weights=True)
+    assert (out == 0).all()
+
+
+def test_far_limit_late_maximum_and_nan(case):
+    c = case(tokens=20, nqh=4, nkh=1, hd=64, n_ctx=(1500,), seed=34, **FAR)
+    c.q[..., 0] = 1.0 / c.scale
+    c.k[0, 0, :, 0] = np.minimum(np.arange(c.M) * (40.0 / 1500), 60).astype(np.float16)
+    c.check()
+    c = case(tokens=20, nqh=4, nkh=1, hd=64, n_ctx=(700,), seed=35, **FAR)
+    c.q[0, 5] = np.nan
+    got, (want, _) = c.run(), c.want()
+    assert np.isnan(got[0, 5]).all()
+    rest = [i for i in range(20) if i != 5]
+    np.testing.assert_allclose(got[0, rest], want[0, rest], rtol=0, atol=4 * TOL)
+
+
+@pytest.mark.parametrize("qscale", [1e-30, 1e4])
+def test_far_limit_large_and_small_queries(case, qscale):
+    c = case(tokens=10, nqh=4, nkh=2, hd=128, n_ctx=(500,), qscale=qscale, seed=9, **FAR)
+    if qscale > 1:
+        c.scale /= -qscale
+    c.check()
+
+
+def test_two_streams_at_once(vbs, gpu, clean_errors):
+    """Two calls that overlap in time, a workspace each, give what they give
+    alone; and a captured pair of calls, replayed."""
+    import torch
+    cases, alone, held = [], [], []
+    for k in range(2):
+        c = Case(vbs, seqs=4, tokens=20, nqh=8, nkh=2, hd=128, n_ctx=(3000,), seed=50 + k)
+        alone.append(c.run())
+        kc, vc, q = c.cache(c.k), c.cache(c.v), c.put(c.q)
+        n_ctx, out = c.put(c.n_ctx, np.int32), torch.zeros(c.q.shape, device="cuda")
+        kv = vbs.KvDesc(k=kc.data_ptr(), v=vc.data_ptr(), n_layers=1, max_ctx=c.M, n_kv_heads=2, head_dim=128, n_seqs=4, head_major=0,
+                        seq_stride=c.M * 2 * 128)
+        tree = vbs.TreeDesc(n_q_heads=8, n_tokens=20, scale=c.scale, ctx_limit=c.limit, n_ctx=n_ctx.data_ptr())
+        work = torch.empty(vbs.tree_workspace(kv, tree), dtype=torch.uint8, device="cuda")
+        held.append((kc, vc, q, n_ctx, out, kv, tree, work))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+
+    def both(s0, s1):
+        for (kc, vc, q, n_ctx, out, kv, tree, work), s in zip(held, (s0, s1)):
+            vbs.attention_tree(kv, 0, tree, q.data_ptr(), out.data_ptr(), work.data_ptr(), work.numel(), s.cuda_stream)
+
+    for _ in range(20):
+        both(*streams)
+    torch.cuda.synchronize()
+    for h, want in zip(held, alone):
+        assert (h[4].cpu().numpy() == want).all()
+        h[4].zero_()
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(streams[0]):
+        with torch.cuda.graph(g, stream=streams[0]):
+            both(streams[0], streams[0])
+    for _ in range(3):
+        g.replay()
+    torch.cuda.synchronize()
+    for h, want in zip(held, alone):
+        assert (h[4].cpu().numpy() == want).all()

@@ -157,6 +157,21 @@ def test_rope_bad_slots_are_reported(vbs, gpu):
         assert torch.equal(kc, want)
 
 
+def test_rope_padding_names_no_sequence(vbs):
+    """A token without a slot may carry any sequence number."""
+    import torch
+    n, hd, ctx = 4, 64, 8
+    kc, vc = (torch.full((2, 1, ctx, 1, hd), 7.0, dtype=torch.float16, device="cuda") for _ in range(2))
+    x = torch.ones((n, 1, hd), device="cuda")
+    q = torch.zeros_like(x)
+    d = [dev([-1, 5, -1, -1], np.int32), dev([-1, 1, 2, 1 << 30], np.int32), dev(np.zeros(n), np.int32)]
+    vbs.rope_store(vbs.rope_plan(hd), kv_of(vbs, kc, vc, False), 0, x.data_ptr(), q.data_ptr(), 1, x.data_ptr(), x.data_ptr(), n,
+                   d[2].data_ptr(), d[0].data_ptr(), seq=d[1].data_ptr())
+    want = torch.full_like(kc, 7.0)
+    want[1, 0, 5] = 1.0
+    assert torch.equal(kc, want) and torch.equal(vc, want) and torch.equal(q, x)
+
+
 # ---- selection -------------------------------------------------------------
 def scores_of(kind, rng, shape):
     x = np.exp(rng.standard_normal(shape) * 3).astype(np.float32)

@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_store_kernel(const __grid_c
     if (p.k) {
         slot = p.slot[tok];
         const int32_t s = p.seq ? p.seq[tok] : 0;
-        if (slot < -1 || slot >= (int32_t)p.max_ctx || s < 0 || s >= (int32_t)p.n_seqs) {
+        if (slot != -1 && (slot < 0 || slot >= (int32_t)p.max_ctx || s < 0 || s >= (int32_t)p.n_seqs)) {
             if (threadIdx.x == 0) dev_flag_error(p.err, DERR_BAD_ARG);
             slot = -1;
         }

@@ -264,7 +264,8 @@ VBS_API int vbs_cu_attention_static(const float *q, const uint16_t *kc, const ui
  * entry points take slots and positions apart. They share one description
  * of a cache. Device pointers throughout, fp32 activations, fp16 cache; the
  * work is queued on `stream` of the current device and no call allocates or
- * synchronizes, so every one can be captured into a graph. Values that are
+ * synchronizes, so every one can be captured into a graph (once the library
+ * has been called on the device: the first call sets it up). Values that are
  * read on the device (lengths, slots, lists) cannot be refused by the call:
  * a bad one sets the device error word, which the next synchronising call
  * of the library reports, and the rows it concerns are left as they were. */
@@ -272,8 +273,9 @@ VBS_API int vbs_cu_attention_static(const float *q, const uint16_t *kc, const ui
 /* One cache for n_seqs sequences. Within a sequence: [layer][position]
  * [kv head][head_dim] (the engine's order), or with head_major
  * [layer][kv head][position][head_dim]. Sequence s starts seq_stride * s
- * elements in. head_dim a multiple of 8, at most 256; k and v 16-byte
- * aligned, seq_stride a multiple of 8. */
+ * elements in; sequences do not overlap (one: seq_stride may be 0). head_dim
+ * a multiple of 8, at most 256; k and v 16-byte aligned, seq_stride a
+ * multiple of 8. */
 typedef struct {
     uint16_t *k, *v;
     uint32_t n_layers, max_ctx, n_kv_heads, head_dim, n_seqs;
@@ -337,18 +339,21 @@ VBS_API int vbs_cu_rope_store(const vbs_cu_rope_t *r, const vbs_cu_kv_t *kv, uin
  *    k_pos[s][slot] ([s][kv head][slot] with k_pos_per_head), rows of max_ctx,
  *    for every slot below n_ctx[s] + n_tok[s], a negative one marking a slot
  *    that nobody sees (padding, a hole); NULL: the slot's number for the
- *    context and q_pos for the new tokens. Without k_pos a window also
- *    saves reading what it leaves out.
+ *    context and q_pos for the new tokens. Within +-2^30. Without k_pos a
+ *    window also saves reading what it leaves out.
  *  - weights_out: [n_seqs][kv head][max_ctx], the attention weights of every
  *    slot below n_ctx + n_tok, summed over the tokens and the query heads of
  *    its KV head, added to weights_in (NULL: 0; may be weights_out itself);
  *    slots from there on are left as they were.
  * n_q_heads is a multiple of the cache's n_kv_heads, at most 256 of them per
- * KV head; n_tokens at most 4096. ctx_limit: an upper
- * bound of n_ctx + n_tok over the sequences, known on the host; it sizes the
- * split of long contexts and the workspace, n_ctx and n_tok are read on the
- * device. Sums and softmax are fp32; fp32 queries and weights enter the
- * tensor cores as two fp16 halves each (exact to about 2^-22). */
+ * KV head; n_tokens at most 4096; q and out do not overlap, 16-byte aligned.
+ * ctx_limit: an upper bound of n_ctx + n_tok over the sequences, known on the
+ * host, at most max_ctx and 2^28; it sizes the split of long contexts and the
+ * workspace, n_ctx and n_tok are read on the device (above it: reported as a
+ * bad length). softcap 0, or 1e-6 and up. Sums and softmax are fp32; fp32
+ * queries (below 2^100) and weights enter the tensor cores as two fp16 halves
+ * each (exact to about 2^-22). A value that is not finite makes what sees it
+ * not finite. */
 typedef struct {
     uint32_t n_q_heads, n_tokens;
     float scale, softcap;
@@ -390,7 +395,8 @@ VBS_API int vbs_cu_cache_select(const float *scores, uint64_t stride, uint32_t n
  * (vbs_cu_cache_select's lists) and the accepted branch of a draft tree
  * (src_base = dst_base = n_ctx, one list per sequence).
  *  - src and dst have the same layers, sequences, heads and head_dim; order
- *    and max_ctx may differ. They are the same cache, or do not overlap.
+ *    and max_ctx may differ. They are the same cache, or do not overlap from
+ *    their first element to their last.
  *  - In the same cache the lists ascend and no row moves up (src_base +
  *    idx[i] >= dst_base + i); a list that breaks this moves nothing and
  *    sets the device error word.

@@ -7,7 +7,7 @@ import math
 import numpy as np
 import pytest
 
-FAKE = 4096
+FAKE, FAR = 4096, 1 << 36
 
 
 def kv(vbs, **kw):
@@ -30,7 +30,8 @@ def refused(vbs, call):
 
 
 BAD_KV = [dict(k=None), dict(v=None), dict(n_layers=0), dict(max_ctx=0), dict(n_kv_heads=0), dict(head_dim=0), dict(head_dim=60),
-          dict(head_dim=264), dict(n_seqs=0), dict(k=FAKE + 8), dict(seq_stride=12), dict(seq_stride=0)]
+          dict(head_dim=264), dict(n_seqs=0), dict(k=FAKE + 8), dict(seq_stride=12), dict(seq_stride=0),
+          dict(seq_stride=2 * 64 * 128 - 8), dict(seq_stride=1 << 61), dict(max_ctx=0x7FFFFFFF, n_layers=1 << 31, n_seqs=1)]
 
 
 @pytest.mark.parametrize("kw", [dict(head_dim=0), dict(head_dim=60), dict(head_dim=264), dict(rot_dim=12), dict(rot_dim=72),
@@ -82,19 +83,27 @@ def tree(vbs, **kw):
 
 BAD_TREE = [dict(n_q_heads=0), dict(n_q_heads=3), dict(n_q_heads=1024), dict(n_tokens=0), dict(n_tokens=4097), dict(ctx_limit=0),
             dict(ctx_limit=65), dict(n_ctx=None), dict(scale=math.nan), dict(softcap=-1.0), dict(softcap=math.nan),
-            dict(window=1 << 31), dict(weights_in=FAKE)]
+            dict(window=1 << 31), dict(weights_in=FAKE), dict(scale=math.inf), dict(softcap=math.inf), dict(softcap=1e-30)]
 
 
 def test_attention_tree_refuses(vbs):
     for bad in BAD_TREE:
         refused(vbs, lambda: vbs.tree_workspace(kv(vbs), tree(vbs, **bad)))
-        refused(vbs, lambda: vbs.attention_tree(kv(vbs), 0, tree(vbs, **bad), FAKE, FAKE, FAKE, 1 << 30))
+        refused(vbs, lambda: vbs.attention_tree(kv(vbs), 0, tree(vbs, **bad), FAKE, FAR, FAKE, 1 << 30))
     for bad in BAD_KV:
         refused(vbs, lambda: vbs.tree_workspace(kv(vbs, **bad), tree(vbs)))
-        refused(vbs, lambda: vbs.attention_tree(kv(vbs, **bad), 0, tree(vbs), FAKE, FAKE, FAKE, 1 << 30))
-    for args in ((2, FAKE, FAKE, FAKE), (0, None, FAKE, FAKE), (0, FAKE, None, FAKE), (0, FAKE, FAKE, None),
-                 (0, FAKE + 4, FAKE, FAKE), (0, FAKE, FAKE + 4, FAKE), (0, FAKE, FAKE, FAKE + 4)):
+        refused(vbs, lambda: vbs.attention_tree(kv(vbs, **bad), 0, tree(vbs), FAKE, FAR, FAKE, 1 << 30))
+    for args in ((2, FAKE, FAR, FAKE), (0, None, FAR, FAKE), (0, FAKE, None, FAKE), (0, FAKE, FAR, None),
+                 (0, FAKE + 4, FAR, FAKE), (0, FAKE, FAR + 4, FAKE), (0, FAKE, FAR, FAKE + 4), (0, FAKE, FAKE, FAKE),
+                 (0, FAKE, FAKE + 2 * 3 * 4 * 64 * 4 - 16, FAKE)):
         refused(vbs, lambda: vbs.attention_tree(kv(vbs), args[0], tree(vbs), *args[1:], 1 << 30))
+
+
+def test_attention_tree_counts_its_limits(vbs):
+    wide = kv(vbs, max_ctx=1 << 29, seq_stride=1 << 38)
+    refused(vbs, lambda: vbs.tree_workspace(wide, tree(vbs, ctx_limit=(1 << 28) + 1)))
+    many = kv(vbs, n_kv_heads=8192, n_seqs=1)
+    refused(vbs, lambda: vbs.tree_workspace(many, tree(vbs, n_q_heads=8192 * 64, n_tokens=4096)))
 
 
 def test_cache_select_refuses(vbs):
@@ -134,4 +143,4 @@ def test_without_a_gpu_the_calls_say_so(vbs):
     if torch.cuda.is_available():
         pytest.skip("a GPU is present")
     with pytest.raises(vbs.VbsError, match="no usable device"):
-        vbs.attention_tree(kv(vbs), 0, tree(vbs), FAKE, FAKE, FAKE, 1 << 30)
+        vbs.attention_tree(kv(vbs), 0, tree(vbs), FAKE, FAR, FAKE, 1 << 30)

@@ -24,7 +24,10 @@ bool kv_desc_ok(const vbs_cu_kv_t *kv) {
     if (kv->max_ctx > 0x7FFFFFFFu || !kv->head_dim || kv->head_dim % 8 || kv->head_dim > 256) return false;
     if ((reinterpret_cast<uintptr_t>(kv->k) | reinterpret_cast<uintptr_t>(kv->v)) & 15) return false;
     if (kv->n_kv_heads > 65535u || kv->n_seqs > 65535u) return false;
-    return kv->seq_stride % 8 == 0 && (kv->n_seqs == 1 || kv->seq_stride);
+    // the sequences lie apart, and their elements' offsets have room to be added up
+    const unsigned __int128 one = (unsigned __int128)kv->max_ctx * kv->n_kv_heads * kv->head_dim * kv->n_layers;
+    const unsigned __int128 all = (unsigned __int128)kv->seq_stride * (kv->n_seqs - 1) + one;
+    return kv->seq_stride % 8 == 0 && (kv->n_seqs == 1 || kv->seq_stride >= one) && all < ((unsigned __int128)1 << 60);
 }
 
 // ---------------------------------------------------------------------------
@@ -662,7 +665,7 @@ static uint64_t kv_extent(const vbs_cu_kv_t *kv) {
            (uint64_t)kv->n_layers * kv->max_ctx * kv->n_kv_heads * kv->head_dim;
 }
 
-static bool overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
+bool overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
     const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
     return a && b && x < y + nb && y < x + na;
 }

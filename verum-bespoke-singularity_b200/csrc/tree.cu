@@ -39,6 +39,7 @@
 #include "tree.cuh"
 
 #include <algorithm>
+#include <cmath>
 
 namespace vbs {
 
@@ -619,10 +620,12 @@ static TreePlan tree_plan(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t, int n_s
 
 static bool tree_desc_ok(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t) {
     if (!kv_desc_ok(kv) || !t || !t->n_q_heads || t->n_q_heads % kv->n_kv_heads || !t->n_tokens || !t->ctx_limit ||
-        t->ctx_limit > kv->max_ctx || !t->n_ctx)
+        t->ctx_limit > kv->max_ctx || t->ctx_limit > 1u << 28 || !t->n_ctx)
         return false;
     if (t->n_tokens > 4096u || t->n_q_heads / kv->n_kv_heads > 256u) return false;
-    if (!(t->scale == t->scale) || !(t->softcap >= 0.f) || t->window > 0x7FFFFFFFu) return false;
+    if (!std::isfinite(t->scale) || !(t->softcap >= 0.f) || !std::isfinite(t->softcap) || t->window > 0x7FFFFFFFu) return false;
+    if (t->softcap > 0.f && t->softcap < 1e-6f) return false;   // its reciprocal scales the scores
+    if ((uint64_t)t->n_tokens * t->n_q_heads > 0x7FFFFFFFu) return false;   // rows of a sequence: CTAs are counted in 32 bits
     return !(t->weights_in && !t->weights_out);
 }
 
@@ -705,7 +708,8 @@ size_t vbs_cu_tree_workspace(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t) {
 
 int vbs_cu_attention_tree(const vbs_cu_kv_t *kv, uint32_t layer, const vbs_cu_tree_t *t, const float *q, float *out, void *work,
                           size_t work_bytes, void *stream) {
-    if (!tree_desc_ok(kv, t) || layer >= kv->n_layers || !q || !out || !work ||
+    const uint64_t bytes = tree_desc_ok(kv, t) ? (uint64_t)kv->n_seqs * t->n_tokens * t->n_q_heads * kv->head_dim * 4 : 0;
+    if (!bytes || layer >= kv->n_layers || !q || !out || !work || overlap(q, bytes, out, bytes) ||
         ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(work)) & 15)) {
         latch_error("vbs_cu_attention_tree: invalid arguments");
         return -1;

@@ -11,6 +11,7 @@
 namespace vbs {
 
 bool kv_desc_ok(const vbs_cu_kv_t *kv);
+bool overlap(const void *a, uint64_t na, const void *b, uint64_t nb);   // bytes from a, from b
 
 struct TreeParams {
     const float *q;

@@ -52,15 +52,15 @@ __global__ void __launch_bounds__(WT_THREADS, 1) tree_weights_kernel(const __gri
     int2 *row_ps = reinterpret_cast<int2 *>(hs + W_ROW + 128 * 8);             // query position, slope (bits)
     float *sums = reinterpret_cast<float *>(hs + W_SUM);
     uint32_t nc, nt;
-    if (!tree_lengths(p, b, nc, nt)) return;
+    if (!tree_lengths(p, b, nc, nt)) return pdl_wait();   // (nobody ends before the attention has)
     const uint32_t end = nc + nt, R = nt * p.G;
     const uint32_t t0 = blockIdx.y * wp.per * TREE_TC_SP, t1 = min(end, t0 + wp.per * TREE_TC_SP);
-    if (t0 >= t1) return;
+    if (t0 >= t1) return pdl_wait();
     const uint64_t out_at = (uint64_t)(b * p.nkh + kvh) * p.max_ctx;
     const uint32_t first = tree_first(p, b, nc, nt, reinterpret_cast<int32_t *>(hs + W_ROW));
     if (t1 <= first || !R) {   // in nobody's window, or nobody there
         for (uint32_t t = t0 + threadIdx.x; t < t1; t += WT_THREADS) p.weights_out[out_at + t] = p.weights_in ? p.weights_in[out_at + t] : 0.f;
-        return;
+        return pdl_wait();
     }
     const uint32_t ntl = (t1 - t0 + TREE_TC_SP - 1) / TREE_TC_SP, rts = (R + wp.rows - 1) / wp.rows;
     const int32_t *kpos = p.k_pos ? p.k_pos + (uint64_t)(p.k_pos_per_head ? b * p.nkh + kvh : b) * p.max_ctx : nullptr;

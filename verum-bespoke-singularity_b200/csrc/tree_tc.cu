@@ -271,14 +271,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
 #pragma unroll
         for (int k = 0; k < 128; ++k) o[k] = 0.f;
         auto gather = [&]() {   // the tile's accumulator into the sums
+            uint32_t x[2][16];
+            tc_ld16(oa, x[0]);
+            tc_wait_ld(x[0]);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                if (32 * c >= (int)hdp) break;
-                uint32_t x[32];
-                tc_ld32(oa + 32 * c, x);
-                tc_wait_ld(x);
+            for (int c = 0; c < 8; ++c) {
+                if (16 * c >= (int)hdp) break;
+                if (c < 7) tc_ld16(oa + 16 * (c + 1), x[(c + 1) & 1]);   // (behind hdp: columns of its own that nobody uses)
 #pragma unroll
-                for (int k = 0; k < 32; ++k) o[32 * c + k] += __uint_as_float(x[k]);
+                for (int k = 0; k < 16; ++k) o[16 * c + k] += __uint_as_float(x[c & 1][k]);
+                if (c < 7) tc_wait_ld(x[(c + 1) & 1]);
             }
         };
         float2 l = make_float2(0.f, 0.f);
@@ -320,6 +322,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
 #pragma unroll
                 for (int k = 0; k < 5; ++k) mk[k] = m0 + k >= 0 && m0 + k < (int)p.words ? mrow[m0 + k] : 0u;
             }
+            // the last tile's accumulator, beside the product of this tile's scores
+            if (n >= 2) {
+                dead = dead || !all(!*bad && waits(base + H_O + 8 * w, ((n >> 1) - 1) & 1u));
+                if (!dead) {
+                    tc_after();
+                    gather();
+                }
+            }
             dead = dead || !all(!*bad && waits(base + H_S + 8 * w, (n >> 1) & 1u));
             if (dead) {   // a wait ran out: only the barriers are kept company
                 if (!whole && bar_or(bar, bar_n, false) && bar_or(bar, bar_n, false))
@@ -327,9 +337,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                 continue;
             }
             tc_after();
-            // the last tile's accumulator (its product is done: this step's
-            // scores were computed behind it)
-            if (n >= 2) gather();
             if (r == 0) reinterpret_cast<volatile uint32_t *>(hs + H_ACC)[w] = 0;
             // plain: the scores as the product left them, times the row's factor;
             // simple: capped, or with slope * (slot - query position) added

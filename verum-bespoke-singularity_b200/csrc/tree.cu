@@ -569,11 +569,13 @@ struct TreePlan {
 struct TreeParts { uint64_t ns; uint32_t per, parts; };
 static TreeParts tree_parts(uint64_t ctas, uint64_t slots, uint32_t span, uint32_t unit, uint32_t pos_ns, uint32_t cta_ns, uint32_t join_ns) {
     TreeParts best = {~0ull, 0, 0};
-    for (uint32_t s = 1; s <= std::min(TREE_MAX_PARTS, (span + unit - 1) / unit); ++s) {
-        const uint32_t per = ((span + s - 1) / s + unit - 1) / unit * unit, parts = (span + per - 1) / per;
-        const uint64_t ns = (ctas * parts + slots - 1) / slots * ((uint64_t)per * pos_ns + cta_ns) + (parts > 1 ? join_ns : 0);
-        if (ns < best.ns) best = {ns, per, parts};
-        if (ctas * s > 16 * slots) break;
+    const uint32_t units = (span + unit - 1) / unit;
+    for (uint32_t s = 1; s <= std::min(TREE_MAX_PARTS, units);) {
+        const uint32_t per = (units + s - 1) / s, parts = (units + per - 1) / per;
+        const uint64_t ns = (ctas * parts + slots - 1) / slots * ((uint64_t)per * unit * pos_ns + cta_ns) + (parts > 1 ? join_ns : 0);
+        if (ns < best.ns) best = {ns, per * unit, parts};
+        if (per == 1 || ctas * s > 16 * slots) break;
+        s = (units + per - 2) / (per - 1);   // the next number that makes a part shorter
     }
     return best;
 }

@@ -271,16 +271,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
 #pragma unroll
         for (int k = 0; k < 128; ++k) o[k] = 0.f;
         auto gather = [&]() {   // the tile's accumulator into the sums
-            uint32_t x[2][16];
-            tc_ld16(oa, x[0]);
-            tc_wait_ld(x[0]);
+            // 64 columns a time: a load answers after some 250 cycles while products run
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                if (16 * c >= (int)hdp) break;
-                if (c < 7) tc_ld16(oa + 16 * (c + 1), x[(c + 1) & 1]);   // (behind hdp: columns of its own that nobody uses)
+            for (int c = 0; c < 2; ++c) {
+                if (64 * c >= (int)hdp) break;
+                uint32_t x[2][32];
+                tc_ld32(oa + 64 * c, x[0]);
+                tc_ld32(oa + 64 * c + 32, x[1]);   // (behind hdp: columns of its own that nobody uses)
+                tc_wait_ld(x[0]);
+                tc_wait_ld(x[1]);
 #pragma unroll
-                for (int k = 0; k < 16; ++k) o[16 * c + k] += __uint_as_float(x[c & 1][k]);
-                if (c < 7) tc_wait_ld(x[(c + 1) & 1]);
+                for (int k = 0; k < 32; ++k) { o[64 * c + k] += __uint_as_float(x[0][k]); o[64 * c + 32 + k] += __uint_as_float(x[1][k]); }
             }
         };
         float2 l = make_float2(0.f, 0.f);
@@ -512,25 +513,25 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
             }
             const float f1 = plain ? fac : 1.f, b1 = mref == -INFINITY ? 0.f : mref;
             const float2 f = make_float2(f1, f1), bs = make_float2(-b1, -b1);
-            uint32_t s[2][16];
-            tc_ld16(sa, s[0]);
+            uint32_t s[2][32];
+            tc_ld32(sa, s[0]);
             tc_wait_ld(s[0]);
-            // 16 positions at a time, the next 16 on their way (they are read
+            // 32 positions at a time, the next 32 on their way (they are read
             // before these halves go over them); behind the end: zeros
-#pragma unroll 1
+#pragma unroll
             for (int c = 0; c < 4; ++c) {
+                if (c < 3) tc_ld32(sa + 32 * (c + 1), s[(c + 1) & 1]);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    if (c < 3 || !u) tc_ld16(sa + 32 * c + 16 * (u + 1), s[u ^ 1]);
                     uint32_t hw[8], lw[8];
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
-                        const float2 x = fma2(make_float2(__uint_as_float(s[u][e]), __uint_as_float(s[u][e + 1])), f, bs);
+                        const float2 x = fma2(make_float2(__uint_as_float(s[c & 1][16 * u + e]), __uint_as_float(s[c & 1][16 * u + e + 1])), f, bs);
                         const float2 pr = make_float2(ex2(x.x), ex2(x.y));
                         l = add2(l, pr);
                         halves(pr, hw[e >> 1], lw[e >> 1]);
                     }
-                    if (c < 3 || !u) tc_wait_ld(s[u ^ 1]);
+                    if (c < 3 && u) tc_wait_ld(s[(c + 1) & 1]);
                     tc_st8(sa + 32 * c + 8 * u, hw);
                     tc_st8(sa + 32 * c + 8 * u + 16, lw);
                 }

@@ -154,13 +154,23 @@ __device__ __forceinline__ void tc_q_load(const TreeParams &p, uint32_t row, uin
     const int lane = threadIdx.x & 31;
     const bool on = row < p.n_tokens * p.G;   // rows behind n_tok are read too: no need to wait for the lengths
     const uint32_t rr = on ? row : 0u, tok = tree_token(p, rr);
+    // whole 32-byte sectors where they are aligned: half a sector a lane
+    // fetches each twice, the L1 left beside the stages is too small for it
+    const bool wide = (reinterpret_cast<uintptr_t>(p.q) & 31) == 0;
     const float *src = p.q + (((uint64_t)b * p.n_tokens + tok) * p.nqh + kvh * p.G + (rr - tok * p.G)) * p.hd;
 #pragma unroll
     for (uint32_t j = 0; j < D / 32; ++j) {
         const uint32_t c = 4 * j + (lane >> 3);
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-            q.x[j][u] = on && c < p.hd / 8 ? *reinterpret_cast<const float4 *>(src + 8 * c + 4 * u) : make_float4(0.f, 0.f, 0.f, 0.f);
+        q.x[j][0] = q.x[j][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (!on || c >= p.hd / 8) continue;
+        if (wide) {
+            asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                         : "=f"(q.x[j][0].x), "=f"(q.x[j][0].y), "=f"(q.x[j][0].z), "=f"(q.x[j][0].w), "=f"(q.x[j][1].x), "=f"(q.x[j][1].y),
+                           "=f"(q.x[j][1].z), "=f"(q.x[j][1].w) : "l"(src + 8 * c));
+        } else {
+            q.x[j][0] = *reinterpret_cast<const float4 *>(src + 8 * c);
+            q.x[j][1] = *reinterpret_cast<const float4 *>(src + 8 * c + 4);
+        }
     }
 }
 

@@ -70,6 +70,7 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
     __shared__ __align__(8) uint64_t bars[2 * C::NST];   // full, empty
     __shared__ uint32_t used[C::NST], issued[C::NST];   // blocks of the stage that are through; 1 + the stage's last tile
     __shared__ int sh_bad;
+    __shared__ __align__(8) float2 sh_ml[C::ROWS];       // the part's, where parts are joined in a cluster
     volatile int *bad = &sh_bad;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int wr = warp % WR, wp = warp / WR;
@@ -84,8 +85,15 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
     tree_part(p, first, end, split, t0, t1);
     const uint64_t slot = (uint64_t)(b * p.nkh + kvh) * p.row_tiles + tile;
     float2 *ml = p.part_ml + (slot * p.n_splits + split) * C::ROWS;
+    auto joins = [&]() {   // in the cluster: the sums of the warps' join are in the first warp's place
+        cluster_meet();
+        tree_join(p, smem_u32(sh_ml), smem_u32(smem), C::OLD * 4, min((uint32_t)C::ROWS, nrows - R0), R0, kvh, b, split, threadIdx.x,
+                  C::THREADS);
+        cluster_meet();
+    };
     if (t0 >= t1 && p.n_splits > 1) {   // no positions: an empty part
-        for (int r = threadIdx.x; r < C::ROWS; r += C::THREADS) ml[r] = make_float2(-INFINITY, 0.f);
+        for (int r = threadIdx.x; r < C::ROWS; r += C::THREADS) (p.joined ? sh_ml : ml)[r] = make_float2(-INFINITY, 0.f);
+        if (p.joined) joins();
         return;
     }
     const uint32_t nch = (t1 - t0 + C::SP - 1) / C::SP, blks = (p.hd + 63) / 64;
@@ -386,6 +394,10 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
             for (int s = 0; s < C::NST; ++s)   // copies may still be landing
                 if (issued[s]) mbar_wait_bounded(full0 + 8 * s, ((issued[s] - 1) / C::NST) & 1u, kWaitNs);
         }
+        if (p.joined) {   // the others wait for this part
+            for (int r = threadIdx.x; r < C::ROWS; r += C::THREADS) sh_ml[r] = make_float2(-INFINITY, 0.f);
+            joins();
+        }
         return;
     }
     const uint32_t live = min((uint32_t)C::ROWS, nrows - R0), q4 = p.hd / 4;
@@ -405,7 +417,10 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
             L += x[HD + 1] * f;
             a.x = fmaf(v.x, f, a.x); a.y = fmaf(v.y, f, a.y); a.z = fmaf(v.z, f, a.z); a.w = fmaf(v.w, f, a.w);
         }
-        if (p.n_splits > 1) {
+        if (p.joined) {
+            if (d == 0) sh_ml[r] = make_float2(M, L);
+            *reinterpret_cast<float4 *>(sh + r * C::OLD + d) = a;   // (read by this thread alone)
+        } else if (p.n_splits > 1) {
             if (d == 0) ml[r] = make_float2(M, L);
             *reinterpret_cast<float4 *>(po + (uint64_t)r * p.hd + d) = a;
         } else {
@@ -418,6 +433,7 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
                 p.lse[(uint64_t)(b * p.nkh + kvh) * (p.n_tokens * G) + rr] = L == 0.f ? -INFINITY : M + log2f(L);
         }
     }
+    if (p.joined) joins();
 }
 
 // ---------------------------------------------------------------------------
@@ -557,23 +573,33 @@ __global__ void __launch_bounds__(TREE_MW * 32) tree_merge_kernel(const __grid_c
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
+constexpr uint32_t TREE_JOIN_NS = 800;
+// Clusters that run at once, by kernel (head_dim up to 64, 128, 256 with 16
+// rows, 256 with 32, tcgen05) and size; set by tree_configure.
+static int tree_fit[5][TREE_CLUSTER + 1];
+
 struct TreePlan {
     uint32_t rows, tile_rows, row_tiles, n_splits, per_split;
-    bool tc;                            // tree_tc_kernel
+    bool tc, joined;                    // tree_tc_kernel; parts joined in clusters
     size_t ml, o, lse, bytes;   // offsets into the workspace, total
 };
 
 // The parts of one kernel's plan: the number that ends first, counting whole
 // waves of CTAs on `slots`, a position's and a CTA's time, and the join's.
-// Only a plan: the kernels divide what the lengths on the device leave.
-struct TreeParts { uint64_t ns; uint32_t per, parts; };
-static TreeParts tree_parts(uint64_t ctas, uint64_t slots, uint32_t span, uint32_t unit, uint32_t pos_ns, uint32_t cta_ns, uint32_t join_ns) {
-    TreeParts best = {~0ull, 0, 0};
+// Only a plan: the kernels divide what the lengths on the device leave. Up to
+// 8 parts can be a cluster that joins them itself, where all clusters run at
+// once (`clusters`[parts] of them; waiting ones cost far more than a join).
+struct TreeParts { uint64_t ns; uint32_t per, parts; bool joined; };
+static TreeParts tree_parts(uint64_t ctas, uint64_t slots, uint32_t span, uint32_t unit, uint32_t pos_ns, uint32_t cta_ns, uint32_t join_ns,
+                            const int *clusters) {
+    TreeParts best = {~0ull, 0, 0, false};
     const uint32_t units = (span + unit - 1) / unit;
     for (uint32_t s = 1; s <= std::min(TREE_MAX_PARTS, units);) {
         const uint32_t per = (units + s - 1) / s, parts = (units + per - 1) / per;
-        const uint64_t ns = (ctas * parts + slots - 1) / slots * ((uint64_t)per * unit * pos_ns + cta_ns) + (parts > 1 ? join_ns : 0);
-        if (ns < best.ns) best = {ns, per * unit, parts};
+        const uint64_t one = (uint64_t)per * unit * pos_ns + cta_ns;
+        const bool joined = parts > 1 && parts <= TREE_CLUSTER && ctas <= (uint64_t)clusters[parts];
+        const uint64_t ns = joined ? one + TREE_JOIN_NS : (ctas * parts + slots - 1) / slots * one + (parts > 1 ? join_ns : 0);
+        if (ns < best.ns) best = {ns, per * unit, parts, joined};
         if (per == 1 || ctas * s > 16 * slots) break;
         s = (units + per - 2) / (per - 1);   // the next number that makes a part shorter
     }
@@ -595,12 +621,12 @@ static TreePlan tree_plan(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t, int n_s
     // mma 40 (head_dim 128, two CTAs per SM), 20 (64), 25 (256, one per SM);
     // tc 16 and 33 (128: 128 rows, 256 rows), 13 and 25 (64).
     pl.tile_rows = hd > 128 && pl.rows > 16 ? 32 : 16;
-    TreeParts best = hd > 128 ? tree_parts(heads * tiles(pl.tile_rows), n_sm, span, 64, 25, 4000, 2000)
-                              : tree_parts(heads * tiles(16), 2ull * n_sm, span, 64, hd > 64 ? 40 : 20, 2500, 2000);
+    TreeParts best = hd > 128 ? tree_parts(heads * tiles(pl.tile_rows), n_sm, span, 64, 25, 4000, 2000, tree_fit[pl.tile_rows > 16 ? 3 : 2])
+                              : tree_parts(heads * tiles(16), 2ull * n_sm, span, 64, hd > 64 ? 40 : 20, 2500, 2000, tree_fit[hd > 64 ? 1 : 0]);
     if (hd <= 128 && pl.rows > 16) {   // (16 rows are one CTA's of the mma kernel: 73.7 us for 16 x 4096 positions x 8 heads, the other 88.4)
         const uint32_t wide = pl.rows > TREE_TC_ROWS;
         const TreeParts tc = tree_parts(heads * tiles(TREE_TC_ROWS << wide), n_sm, span, TREE_TC_SP,
-                                        (hd > 64 ? 16 : 13) << wide, wide ? 13000 : 9000, 3000);
+                                        (hd > 64 ? 16 : 13) << wide, wide ? 13000 : 9000, 3000, tree_fit[4]);
         if (tc.ns < best.ns) {
             best = tc;
             pl.tc = true;
@@ -609,9 +635,10 @@ static TreePlan tree_plan(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t, int n_s
     }
     pl.per_split = best.per;
     pl.n_splits = best.parts;
+    pl.joined = best.joined;
     pl.row_tiles = tiles(pl.tile_rows);
     auto take = [&](size_t n) { const size_t at = pl.bytes; pl.bytes += (n + 255) / 256 * 256; return at; };
-    if (pl.n_splits > 1) {
+    if (pl.n_splits > 1 && !pl.joined) {
         pl.ml = take(heads * pl.row_tiles * pl.n_splits * pl.tile_rows * sizeof(float2));
         pl.o = take(heads * pl.row_tiles * pl.n_splits * pl.tile_rows * kv->head_dim * sizeof(float));
     }
@@ -671,19 +698,19 @@ static cudaError_t tree_merge_launch(const TreeParams &p, uint32_t rows, uint32_
 template <int HD, int WR, int WP>
 static cudaError_t tree_go(const TreeParams &p, const CUtensorMap &km, const CUtensorMap &vm, dim3 grid, cudaStream_t st) {
     using C = TreeCfg<HD, WR, WP>;
-    tree_mma_kernel<HD, WR, WP><<<grid, C::THREADS, C::SMEM, st>>>(p, km, vm);
-    return cudaGetLastError();
+    return tree_launch(tree_mma_kernel<HD, WR, WP>, grid, C::THREADS, C::SMEM, p.joined, st, p, km, vm);
 }
-template <int HD, int WR, int WP> static cudaError_t tree_cfg() {
-    return cudaFuncSetAttribute(tree_mma_kernel<HD, WR, WP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                TreeCfg<HD, WR, WP>::SMEM);
+template <int HD, int WR, int WP> static cudaError_t tree_cfg(int *clusters) {
+    using C = TreeCfg<HD, WR, WP>;
+    const cudaError_t e = cudaFuncSetAttribute(tree_mma_kernel<HD, WR, WP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    return e == cudaSuccess ? tree_clusters(tree_mma_kernel<HD, WR, WP>, C::THREADS, C::SMEM, clusters) : e;
 }
 cudaError_t tree_configure() {
-    cudaError_t e = tree_cfg<64, 1, 4>();
-    if (e == cudaSuccess) e = tree_cfg<128, 1, 4>();
-    if (e == cudaSuccess) e = tree_cfg<256, 1, 8>();
-    if (e == cudaSuccess) e = tree_cfg<256, 2, 4>();
-    if (e == cudaSuccess) e = tree_tc_configure();
+    cudaError_t e = tree_cfg<64, 1, 4>(tree_fit[0]);
+    if (e == cudaSuccess) e = tree_cfg<128, 1, 4>(tree_fit[1]);
+    if (e == cudaSuccess) e = tree_cfg<256, 1, 8>(tree_fit[2]);
+    if (e == cudaSuccess) e = tree_cfg<256, 2, 4>(tree_fit[3]);
+    if (e == cudaSuccess) e = tree_tc_configure(tree_fit[4]);
     if (e == cudaSuccess) e = tree_weights_configure();
     // the join takes the attention kernels' split of shared memory and L1:
     // changing it costs an SM several microseconds between kernels
@@ -734,7 +761,7 @@ int vbs_cu_attention_tree(const vbs_cu_kv_t *kv, uint32_t layer, const vbs_cu_tr
     p.head_step = kv->head_major ? (uint64_t)kv->max_ctx * kv->head_dim : kv->head_dim;
     p.max_ctx = kv->max_ctx; p.nkh = kv->n_kv_heads; p.nqh = t->n_q_heads; p.G = t->n_q_heads / kv->n_kv_heads;
     p.hd = kv->head_dim; p.n_tokens = t->n_tokens; p.words = (t->n_tokens + 31) / 32; p.window = t->window;
-    p.ctx_limit = t->ctx_limit; p.row_tiles = pl.row_tiles; p.n_splits = pl.n_splits; p.per_split = pl.per_split;
+    p.joined = pl.joined; p.ctx_limit = t->ctx_limit; p.row_tiles = pl.row_tiles; p.n_splits = pl.n_splits; p.per_split = pl.per_split;
     p.scale = t->scale; p.cap = t->softcap; p.slopes = t->slopes; p.n_ctx = t->n_ctx; p.n_tok = t->n_tok;
     p.mask = t->mask; p.q_pos = t->q_pos; p.k_pos = t->k_pos; p.k_pos_per_head = t->k_pos_per_head;
     p.weights_in = t->weights_in; p.weights_out = t->weights_out;
@@ -745,7 +772,8 @@ int vbs_cu_attention_tree(const vbs_cu_kv_t *kv, uint32_t layer, const vbs_cu_tr
     p.g_magic = (uint32_t)((0x100000000ull + p.G - 1) / p.G);
     p.err = d->err;
     const dim3 grid(kv->n_kv_heads * pl.row_tiles, pl.n_splits, kv->n_seqs);
-    note_launches(1u + (pl.n_splits > 1) + (t->weights_out != nullptr));
+    const bool merge = pl.n_splits > 1 && !pl.joined;
+    note_launches(1u + merge + (t->weights_out != nullptr));
     CUtensorMap km, vm, wm;
     cudaError_t e = tree_map(&km, p.kc, kv, pl.tc ? TREE_TC_SP : 64);
     if (e == cudaSuccess) e = tree_map(&vm, p.vc, kv, pl.tc ? TREE_TC_SP : 64);
@@ -756,7 +784,7 @@ int vbs_cu_attention_tree(const vbs_cu_kv_t *kv, uint32_t layer, const vbs_cu_tr
             : kv->head_dim <= 128     ? tree_go<128, 1, 4>(p, km, vm, grid, st)
             : pl.tile_rows == 16      ? tree_go<256, 1, 8>(p, km, vm, grid, st)
                                       : tree_go<256, 2, 4>(p, km, vm, grid, st);
-    if (e == cudaSuccess && pl.n_splits > 1)
+    if (e == cudaSuccess && merge)
         e = tree_merge_launch(p, pl.rows, kv->n_seqs, pl.tile_rows, d->n_sm, st);
     if (e == cudaSuccess && t->weights_out) e = tree_weights_launch(p, wm, kv->n_seqs, d->n_sm, st);
     return cuda_ok(e, "attention_tree") ? 0 : -1;

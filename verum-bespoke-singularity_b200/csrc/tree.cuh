@@ -32,6 +32,7 @@ struct TreeParams {
     float2 *part_ml;              // [slot][split][tile rows]
     float *part_o;                // [slot][split][tile rows][hd], slot = (seq * nkh + kv head) * row_tiles + tile
     float *lse;                   // [seq * nkh + kv head][rows], log2 units, with weights
+    uint32_t joined;              // the parts are one cluster and joined in it: no workspace, no second kernel
     uint32_t g_magic;             // ceil(2^32 / G): row / G without a division
     uint32_t *err;
 };
@@ -159,11 +160,102 @@ __device__ __forceinline__ void tree_tma(uint32_t dst, const CUtensorMap *map, u
         ::"r"(dst), "l"(map), "r"(dim), "r"(pos), "r"(head), "r"(seq), "r"(bar) : "memory");
 }
 
+// ---- parts joined in a cluster (CTA rank = part) ---------------------------
+__device__ __forceinline__ void cluster_meet() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float2 cluster_f2(uint32_t a, uint32_t rank) {
+    float2 v;
+    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %2, %3;\n\tld.shared::cluster.v2.f32 {%0, %1}, [r];\n\t}"
+                 : "=f"(v.x), "=f"(v.y) : "r"(a), "r"(rank) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 cluster_f4(uint32_t a, uint32_t rank) {
+    float4 v;
+    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [r];\n\t}"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a), "r"(rank) : "memory");
+    return v;
+}
+
+// Every CTA of the cluster has its part's (m, l) per row at `ml` and sums at
+// `o` (rows `pitch` bytes apart) of its shared memory, the same places in all;
+// the CTAs share the rows' pieces of 16 bytes. Threads tid < n of each call
+// it, between the two cluster_meet() that all threads of all CTAs make.
+constexpr uint32_t TREE_CLUSTER = 8;
+__device__ __forceinline__ void tree_join(const TreeParams &p, uint32_t ml, uint32_t o, uint32_t pitch, uint32_t live, uint32_t R0,
+                                          uint32_t kvh, uint32_t b, uint32_t rank, uint32_t tid, uint32_t n) {
+    const uint32_t q4 = p.hd / 4, C = p.n_splits;
+    for (uint32_t i = rank * n + tid; i < live * q4; i += C * n) {
+        const uint32_t r = i / q4, d = i - r * q4;
+        float2 x[TREE_CLUSTER];
+        float4 v[TREE_CLUSTER];
+#pragma unroll
+        for (uint32_t c = 0; c < TREE_CLUSTER; ++c) {
+            x[c] = make_float2(-INFINITY, 0.f);
+            if (c < C) {
+                x[c] = cluster_f2(ml + 8 * r, c);
+                v[c] = cluster_f4(o + r * pitch + 16 * d, c);
+            }
+        }
+        float M = -INFINITY, L = 0.f;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (uint32_t c = 0; c < TREE_CLUSTER; ++c) M = fmaxf(M, x[c].x);
+#pragma unroll
+        for (uint32_t c = 0; c < TREE_CLUSTER; ++c) {
+            if (x[c].y == 0.f) continue;   // an empty part has no sums; a NaN goes through
+            const float f = ex2(x[c].x - M);
+            L += x[c].y * f;
+            a.x = fmaf(v[c].x, f, a.x); a.y = fmaf(v[c].y, f, a.y); a.z = fmaf(v[c].z, f, a.z); a.w = fmaf(v[c].w, f, a.w);
+        }
+        const float il = L == 0.f ? 0.f : 1.f / L;
+        const uint32_t rr = R0 + r, tok = tree_token(p, rr);
+        reinterpret_cast<float4 *>(p.out + (((uint64_t)b * p.n_tokens + tok) * p.nqh + kvh * p.G + (rr - tok * p.G)) * p.hd)[d] =
+            make_float4(a.x * il, a.y * il, a.z * il, a.w * il);
+        if (p.lse && d == 0) p.lse[(uint64_t)(b * p.nkh + kvh) * (p.n_tokens * p.G) + rr] = L == 0.f ? -INFINITY : M + log2f(L);
+    }
+}
+
 // tree_tc.cu: row tiles of TREE_TC_ROWS, head_dim up to 128.
 constexpr uint32_t TREE_TC_ROWS = 128, TREE_TC_SP = 128;
-cudaError_t tree_tc_configure();
+cudaError_t tree_tc_configure(int *clusters);   // clusters[c]: how many of c CTAs run at once
 cudaError_t tree_tc_launch(const TreeParams &p, const CUtensorMap &km, const CUtensorMap &vm, uint32_t n_seqs,
                            uint32_t dual, cudaStream_t st);
+
+// Kernel launch whose parts (grid.y) are a cluster, or not.
+template <class K, class... A>
+inline cudaError_t tree_launch(K kernel, dim3 grid, uint32_t threads, size_t smem, bool joined, cudaStream_t st, const A &...args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = attr[0].val.clusterDim.z = 1;
+    attr[0].val.clusterDim.y = grid.y;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = joined ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+template <class K> inline cudaError_t tree_clusters(K kernel, uint32_t threads, size_t smem, int *clusters) {
+    for (uint32_t c = 2; c <= TREE_CLUSTER; ++c) {
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = attr[0].val.clusterDim.z = 1;
+        attr[0].val.clusterDim.y = c;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(1, c, 1);
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        const cudaError_t e = cudaOccupancyMaxActiveClusters(&clusters[c], kernel, &cfg);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
 
 // tree_wt.cu: the weights per slot, after the attention wrote lse.
 cudaError_t tree_weights_configure();

@@ -44,6 +44,7 @@ constexpr int TC_LOADER = TC_SOFT / 32, TC_QK = TC_LOADER + 1, TC_PV = TC_LOADER
 // registers: 384 x 168 at the launch = 256 x 232 + 128 x 40 (64,512 each)
 constexpr int TC_REGS_SOFT = 232, TC_REGS_OTHER = 40;
 static_assert(TC_SOFT * TC_REGS_SOFT + (TC_THREADS - TC_SOFT) * TC_REGS_OTHER <= TC_THREADS * 168, "more than launched waits forever");
+constexpr uint32_t TC_PITCH = 128 * 4 + 16;   // bytes of a row of sums in shared memory: conflict-free for a thread per row
 constexpr uint32_t TC_BLK = TREE_TC_SP * 128u;   // one box: 128 positions x 64 dims
 
 // words of the state behind the queries (bytes); barriers first
@@ -98,15 +99,25 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
     tree_part(p, first, end, split, t0, t1);
     const uint64_t slot_id = (uint64_t)(b * p.nkh + kvh) * p.row_tiles + tile;
     float2 *ml = p.part_ml + (slot_id * p.n_splits + split) * TR;
+    const uint32_t two = tp.dual && nrows > TREE_TC_ROWS;
+    // parts joined in a cluster: (m, l) and sums of the rows here, behind what
+    // the streams' own join uses (all products are done by then)
+    const uint32_t jm = two ? 0u : 2 * TREE_TC_ROWS * 8 + TREE_TC_ROWS * TC_PITCH, jo = jm + 2 * TREE_TC_ROWS * 8, jp = p.hd * 4 + 16;
+    float2 *const jml = reinterpret_cast<float2 *>(smem + jm);
     if (t0 >= t1 && p.n_splits > 1) {
-        for (uint32_t r = threadIdx.x; r < TR; r += TC_THREADS) ml[r] = make_float2(-INFINITY, 0.f);
+        for (uint32_t r = threadIdx.x; r < TR; r += TC_THREADS) (p.joined ? jml : ml)[r] = make_float2(-INFINITY, 0.f);
+        if (p.joined) {
+            cluster_meet();
+            if (threadIdx.x < TC_SOFT) tree_join(p, stage0 + jm, stage0 + jo, jp, nrows, R0, kvh, b, split, threadIdx.x, TC_SOFT);
+            cluster_meet();
+        }
         return;
     }
     // step n: position tile n (dual: n / 2) for stream n % 2, the stream's
     // (n / 2)th; the streams share the rows and alternate tiles, or (dual)
     // have 128 rows each and share the tiles
     const uint32_t nch = (t1 - t0 + TREE_TC_SP - 1) / TREE_TC_SP;
-    const uint32_t two = tp.dual && nrows > TREE_TC_ROWS, steps = two ? 2 * nch : nch;
+    const uint32_t steps = two ? 2 * nch : nch;
     const uint32_t aw0 = (min(nrows, TREE_TC_ROWS) + 31) / 32, aw1 = two ? (nrows - TREE_TC_ROWS + 31) / 32 : aw0;   // 32s of rows
     auto waits = [&](uint32_t bar, uint32_t parity) -> bool {
         if (mbar_wait_bounded(bar, parity, kWaitNs)) return true;
@@ -551,9 +562,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
         const bool join = !two && nch > 1;   // the two streams had the same rows: each ends half of the dims
         const uint32_t half = join ? (p.hd / 8 + 1) / 2 * 8 : 0u;   // stream 0: below
         if (join) {
-            const uint32_t pitch = 128 * 4 + 16;   // a row's bytes: conflict-free for a thread per row
             float2 *ml_sm = reinterpret_cast<float2 *>(smem);   // over the stages: all products are done
-            float *rows_sm = reinterpret_cast<float *>(smem + 2 * TREE_TC_ROWS * 8 + r * pitch);
+            float *rows_sm = reinterpret_cast<float *>(smem + 2 * TREE_TC_ROWS * 8 + r * TC_PITCH);
             ml_sm[w * TREE_TC_ROWS + r] = make_float2(active ? M : -INFINITY, active ? L : 0.f);
 #pragma unroll
             for (int c = 0; c < 128; c += 8) {   // the other stream's half goes over
@@ -579,9 +589,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
         if (active && ok && on && (two || join || w == 0)) {
             const bool many = p.n_splits > 1;
             const float il = many ? 1.f : (L == 0.f ? 0.f : 1.f / L);
-            float *dst = many ? p.part_o + ((slot_id * p.n_splits + split) * TR + ri) * p.hd
-                              : p.out + (((uint64_t)b * p.n_tokens + tok) * p.nqh + head) * p.hd;
-            const bool wide = (reinterpret_cast<uintptr_t>(dst) & 31) == 0;
+            float *dst = p.joined ? reinterpret_cast<float *>(smem + jo + ri * jp)
+                         : many   ? p.part_o + ((slot_id * p.n_splits + split) * TR + ri) * p.hd
+                                  : p.out + (((uint64_t)b * p.n_tokens + tok) * p.nqh + head) * p.hd;
+            const bool wide = !p.joined && (reinterpret_cast<uintptr_t>(dst) & 31) == 0;
             // straight from the rows' threads, a whole 32-byte sector each
 #pragma unroll
             for (int c = 0; c < 128; c += 8) {
@@ -598,11 +609,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                 }
             }
             if (two || w == 0) {
-                if (many) ml[ri] = make_float2(M, L);
+                if (many) (p.joined ? jml : ml)[ri] = make_float2(M, L);
                 else if (p.lse) p.lse[(uint64_t)(b * p.nkh + kvh) * (p.n_tokens * p.G) + rr] = L == 0.f ? -INFINITY : M + log2f(L);
             }
         }
         if (*bad && threadIdx.x == 0) dev_flag_error(p.err, DERR_TIMEOUT_FULL);
+        if (p.joined) {
+            cluster_meet();
+            tree_join(p, stage0 + jm, stage0 + jo, jp, nrows, R0, kvh, b, split, threadIdx.x, TC_SOFT);
+            cluster_meet();
+        }
+    }
+    if (warp >= TC_LOADER && p.joined) {
+        cluster_meet();
+        cluster_meet();
     }
     tc_before();
     __syncthreads();
@@ -616,8 +636,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
 
 }  // namespace
 
-cudaError_t tree_tc_configure() {
-    return cudaFuncSetAttribute(tree_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
+cudaError_t tree_tc_configure(int *clusters) {
+    const cudaError_t e = cudaFuncSetAttribute(tree_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
+    return e == cudaSuccess ? tree_clusters(tree_tc_kernel, TC_THREADS, 232448, clusters) : e;
 }
 
 cudaError_t tree_tc_launch(const TreeParams &t, const CUtensorMap &km, const CUtensorMap &vm, uint32_t n_seqs, uint32_t dual,
@@ -636,8 +657,7 @@ cudaError_t tree_tc_launch(const TreeParams &t, const CUtensorMap &km, const CUt
     p.q_off = p.ns * p.blks * TC_BLK;
     p.h_off = p.q_off + q_bytes;
     const dim3 grid(t.nkh * t.row_tiles, t.n_splits, n_seqs);
-    tree_tc_kernel<<<grid, TC_THREADS, p.h_off + H_BYTES, st>>>(p);
-    return cudaGetLastError();
+    return tree_launch(tree_tc_kernel, grid, TC_THREADS, p.h_off + H_BYTES, t.joined, st, p);
 }
 
 }  // namespace vbs

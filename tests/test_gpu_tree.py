@@ -523,3 +523,79 @@ def test_two_streams_at_once(vbs, gpu, clean_errors):
     torch.cuda.synchronize()
     for h, want in zip(held, alone):
         assert (h[4].cpu().numpy() == want).all()
+
+
+# ---- many KV heads: 256 rows a CTA; in one part, in parts of a cluster, in
+# parts that a second kernel joins
+MANY = [(10, 100), (5, 700), (5, 1500), (10, 3000)]
+
+
+def many(case, seqs, limit, tokens=33, **kw):
+    lengths = (limit - tokens, 0, limit // 2, 5, (limit - tokens) // 128 * 128)
+    return case(seqs=seqs, tokens=tokens, nqh=32, nkh=8, n_ctx=lengths, n_tok=[(tokens, tokens, 20, 1, 32)[b % 5] for b in range(seqs)],
+                limit=limit, spare=0, **kw)
+
+
+@pytest.mark.parametrize("hd", [64, 72, 128])
+@pytest.mark.parametrize("seqs,limit", MANY)
+def test_many_heads(case, hd, seqs, limit):
+    many(case, seqs, limit, hd=hd, tree=True, head_major=hd == 72, seed=hd).check(weights=limit < 1000)
+
+
+@pytest.mark.parametrize("cap,slopes,window,qscale", [(30.0, False, 0, 4.0), (0.0, True, 0, 1.0), (5.0, True, 100, 6.0)])
+@pytest.mark.parametrize("k_pos", [None, padded, evicted])
+def test_many_heads_options(case, cap, slopes, window, qscale, k_pos):
+    many(case, 5, 700, hd=128, tree=True, cap=cap, slopes=slopes, window=window, qscale=qscale, pos=0 if k_pos is None else 700, k_pos=k_pos,
+         seed=43).check(weights=True)
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("seqs,limit", MANY[:2])
+def test_many_heads_masked_places(case, bad, seqs, limit):
+    c = many(case, seqs, limit, hd=128, pos=0, tree=True, k_pos=lambda rng, c: padded(rng, c), seed=5)
+    c.sees[:, :, 2] = False
+    for x in (c.k, c.v):
+        for b in range(seqs):
+            end = c.n_ctx[b] + c.n_tok[b]
+            x[b, :, end:] = bad
+            if c.n_tok[b] > 2:
+                x[b, :, c.n_ctx[b] + 2] = bad
+            x[b, :, :end][:, c.k_pos[b, :end] < 0] = bad
+    c.check()
+
+
+@pytest.mark.parametrize("seqs,tokens,nkh,limit", [(5, 9, 8, 100), (10, 2, 8, 100), (1, 5, 2, 700), (1, 2, 2, 1500), (10, 4, 8, 2000)])
+def test_wide_heads(case, seqs, tokens, nkh, limit):
+    case(seqs=seqs, tokens=tokens, nqh=4 * nkh, nkh=nkh, hd=256, n_ctx=(limit - tokens, 0, 33), limit=limit, spare=0, tree=True,
+         seed=tokens).check(weights=limit < 1000)
+
+
+@pytest.mark.parametrize("hd,tokens,limit", [(64, 3, 500), (128, 33, 700), (256, 3, 500)])
+def test_parts_of_a_cluster_in_a_graph(vbs, gpu, clean_errors, hd, tokens, limit):
+    """Parts that join themselves, captured and replayed over new lengths."""
+    import torch
+    c = Case(vbs, seqs=2, tokens=tokens, nqh=8, nkh=2, hd=hd, n_ctx=(limit - tokens, 17), limit=limit, spare=0, seed=hd)
+    first = c.run()
+    k, v, q = c.cache(c.k), c.cache(c.v), c.put(c.q)
+    out = torch.zeros(c.q.shape, device="cuda")
+    n_ctx = c.put(c.n_ctx, np.int32)
+    c.kv.k, c.kv.v, c.tree.n_ctx, c.tree.n_tok = k.data_ptr(), v.data_ptr(), n_ctx.data_ptr(), None
+    nbytes = vbs.tree_workspace(c.kv, c.tree)
+    work = torch.full((nbytes,), 255, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(2):
+            vbs.attention_tree(c.kv, 0, c.tree, q.data_ptr(), out.data_ptr(), work.data_ptr(), nbytes,
+                               torch.cuda.current_stream().cuda_stream)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert np.array_equal(out.cpu().numpy(), first)
+    for lengths in ((0, limit - tokens), (129, 64)):
+        c.n_ctx = np.asarray(lengths)
+        n_ctx.copy_(c.put(c.n_ctx, np.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        np.testing.assert_allclose(out.cpu().numpy(), c.want()[0], rtol=0, atol=4 * TOL)
+    gpu.synchronize_device(gpu.get_device(0))
+    assert vbs.last_error() == "ok"

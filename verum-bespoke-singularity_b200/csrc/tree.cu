@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(TREE_MW * 32) tree_merge_kernel(const __grid_c
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-constexpr uint32_t TREE_JOIN_NS = 800;
+constexpr uint32_t TREE_JOIN_NS = 800, TREE_MERGE_NS = 3000, TREE_MERGE_RATE = 4000;   // in a cluster; by a second kernel, and bytes per ns of the parts' sums
 // Clusters that run at once, by kernel (head_dim up to 64, 128, 256 with 16
 // rows, 256 with 32, tcgen05) and size; set by tree_configure.
 static int tree_fit[5][TREE_CLUSTER + 1];
@@ -590,15 +590,17 @@ struct TreePlan {
 // 8 parts can be a cluster that joins them itself, where all clusters run at
 // once (`clusters`[parts] of them; waiting ones cost far more than a join).
 struct TreeParts { uint64_t ns; uint32_t per, parts; bool joined; };
-static TreeParts tree_parts(uint64_t ctas, uint64_t slots, uint32_t span, uint32_t unit, uint32_t pos_ns, uint32_t cta_ns, uint32_t join_ns,
+static TreeParts tree_parts(uint64_t ctas, uint64_t slots, uint32_t span, uint32_t unit, uint32_t pos_ns, uint32_t cta_ns, uint32_t row_bytes,
                             const int *clusters) {
     TreeParts best = {~0ull, 0, 0, false};
     const uint32_t units = (span + unit - 1) / unit;
     for (uint32_t s = 1; s <= std::min(TREE_MAX_PARTS, units);) {
         const uint32_t per = (units + s - 1) / s, parts = (units + per - 1) / per;
-        const uint64_t one = (uint64_t)per * unit * pos_ns + cta_ns;
+        const uint64_t one = (uint64_t)per * unit * pos_ns / 10 + cta_ns;
         const bool joined = parts > 1 && parts <= TREE_CLUSTER && ctas <= (uint64_t)clusters[parts];
-        const uint64_t ns = joined ? one + TREE_JOIN_NS : (ctas * parts + slots - 1) / slots * one + (parts > 1 ? join_ns : 0);
+        uint64_t ns = (ctas * parts + slots - 1) / slots * one;
+        if (joined) ns = one + TREE_JOIN_NS;
+        else if (parts > 1) ns += TREE_MERGE_NS + ctas * parts * row_bytes / TREE_MERGE_RATE;
         if (ns < best.ns) best = {ns, per * unit, parts, joined};
         if (per == 1 || ctas * s > 16 * slots) break;
         s = (units + per - 2) / (per - 1);   // the next number that makes a part shorter
@@ -615,23 +617,26 @@ static TreePlan tree_plan(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t, int n_s
     const uint64_t heads = (uint64_t)kv->n_kv_heads * kv->n_seqs;
     auto tiles = [&](uint32_t rows) { return (pl.rows + rows - 1) / rows; };
     // tree_mma_kernel: 16 rows a CTA (32 above head_dim 128, where a CTA has an
-    // SM to itself); tree_tc_kernel: 128 rows, 256 if there are more. The tc
-    // kernel's time for a position is the same for 1 row and for 128 but its
-    // start is the longer. Measured on full SMs, ns per position and CTA:
-    // mma 40 (head_dim 128, two CTAs per SM), 20 (64), 25 (256, one per SM);
-    // tc 16 and 33 (128: 128 rows, 256 rows), 13 and 25 (64).
-    pl.tile_rows = hd > 128 && pl.rows > 16 ? 32 : 16;
-    TreeParts best = hd > 128 ? tree_parts(heads * tiles(pl.tile_rows), n_sm, span, 64, 25, 4000, 2000, tree_fit[pl.tile_rows > 16 ? 3 : 2])
-                              : tree_parts(heads * tiles(16), 2ull * n_sm, span, 64, hd > 64 ? 40 : 20, 2500, 2000, tree_fit[hd > 64 ? 1 : 0]);
-    if (hd <= 128 && pl.rows > 16) {   // (16 rows are one CTA's of the mma kernel: 73.7 us for 16 x 4096 positions x 8 heads, the other 88.4)
-        const uint32_t wide = pl.rows > TREE_TC_ROWS;
-        const TreeParts tc = tree_parts(heads * tiles(TREE_TC_ROWS << wide), n_sm, span, TREE_TC_SP,
-                                        (hd > 64 ? 16 : 13) << wide, wide ? 13000 : 9000, 3000, tree_fit[4]);
-        if (tc.ns < best.ns) {
-            best = tc;
-            pl.tc = true;
-            pl.tile_rows = TREE_TC_ROWS << wide;
-        }
+    // SM to itself); tree_tc_kernel: 128 rows, or 256 of more, which halves
+    // what K and V cost but doubles a CTA. Measured on full SMs, ns per
+    // position and CTA: 30 (head_dim 128), 22 (64) with two CTAs per SM, 22 and 44
+    // (256; 16 and 32 rows); 15 and 28.5 (128; 128 and 256 rows), 10 and 19.5 (64).
+    TreeParts best = {~0ull, 0, 0, false};
+    auto plan = [&](bool tc, uint32_t rows, uint32_t per_sm, uint32_t unit, uint32_t pos_ns, uint32_t cta_ns, const int *clusters) {
+        const TreeParts one = tree_parts(heads * tiles(rows), (uint64_t)per_sm * n_sm, span, unit, pos_ns, cta_ns, rows * hd * 4, clusters);
+        if (one.ns >= best.ns) return;
+        best = one;
+        pl.tc = tc;
+        pl.tile_rows = rows;
+    };
+    if (hd > 128) {
+        if (pl.rows <= 16) plan(false, 16, 1, 64, 220, 6000, tree_fit[2]);
+        else plan(false, 32, 1, 64, 440, 6000, tree_fit[3]);
+    } else {
+        const bool big = hd > 64;
+        plan(false, 16, 2, 64, big ? 300 : 220, 4000, tree_fit[big ? 1 : 0]);
+        if (pl.rows > 16) plan(true, TREE_TC_ROWS, 1, TREE_TC_SP, big ? 150 : 100, 9000, tree_fit[4]);   // (16 rows are one CTA's of the other kernel)
+        if (pl.rows > TREE_TC_ROWS) plan(true, 2 * TREE_TC_ROWS, 1, TREE_TC_SP, big ? 285 : 195, 12000, tree_fit[4]);
     }
     pl.per_split = best.per;
     pl.n_splits = best.parts;

@@ -320,6 +320,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                 low = min(min(kn[0], kn[1]), min(kn[2], kn[3]));
                 low = __reduce_min_sync(0xffffffffu, low);
             }
+            // the tile's key positions where they are not its slots, lane: 32 k + lane
+            const bool by_slot = !kpos && tb + TREE_TC_SP <= nc;
+            int32_t kc[4] = {kn[0], kn[1], kn[2], kn[3]};
+            if (!context && (kpos || p.window || p.slopes)) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) kc[k] = 32 * k + lane < nval ? tree_kpos(p, kpos, b, tb + 32 * k + lane, nc) : 0;
+            }
             if (kpos && tn + TREE_TC_SP <= nc) {   // the next tile's, ahead
 #pragma unroll
                 for (int k = 0; k < 4; ++k) kn[k] = kpos[tn + 32 * k + lane];
@@ -350,10 +357,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
             }
             tc_after();
             if (r == 0) reinterpret_cast<volatile uint32_t *>(hs + H_ACC)[w] = 0;
-            // plain: the scores as the product left them, times the row's factor;
-            // simple: capped, or with slope * (slot - query position) added
-            const bool linear = p.slopes && !kpos, simple = whole && (!p.slopes || linear);
-            const bool plain = simple && !p.slopes && !(p.cap > 0.f);
+            // plain: the scores as the product left them, times the row's factor
+            const bool turned = p.slopes || p.cap > 0.f, plain = whole && !turned;
             const float cap2 = p.cap * TREE_LOG2E;
             float mx = -INFINITY;
             if (plain) {
@@ -367,7 +372,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                     if (c < 3) tc_wait_ld(s[(c + 1) & 1]);
                 }
                 mx *= fac;
-            } else if (simple) {
+            } else if (turned) {
+                // capped, with slope * (key position - query position) added,
+                // back into tensor memory
+                const bool linear = p.slopes && by_slot;
 #pragma unroll 1
                 for (int c = 0; c < 8; ++c) {
                     uint32_t s[16];
@@ -381,79 +389,66 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                         const float d = (float)((int32_t)tb + 16 * c - qp);
 #pragma unroll
                         for (int e = 0; e < 16; ++e) x[e] = fmaf(slope, d + (float)e, x[e]);
+                    } else if (p.slopes) {
+                        const int32_t kp = c < 4 ? (c < 2 ? kc[0] : kc[1]) : (c < 6 ? kc[2] : kc[3]);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            x[e] = fmaf(slope, (float)(__shfl_sync(0xffffffffu, kp, 16 * (c & 1) + e) - qp), x[e]);
                     }
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) mx = max3(mx, x[e], x[e + 1]);
 #pragma unroll
                     for (int e = 0; e < 16; ++e) s[e] = __float_as_uint(x[e]);
+                    __syncwarp();
                     tc_st16(sa + 16 * c, s);
                 }
                 tc_wait_st();
-            } else {
-                // scores as the formula has them, back into tensor memory, 8 at
-                // a time (short code: it runs for few tiles, out of cold
-                // instruction caches)
-                const bool by_slot = !kpos && tb + TREE_TC_SP <= nc;   // the tile's positions are its slots
-                bool hidden = (nval & 15) != 0;                        // stale rows behind the end in the last product
-                uint32_t see = 0;     // bit e: this row sees the e-th next position
-                int32_t kp = 0;       // key position of slot (32's first + lane), handed round where rows need them
+            }
+            if (!whole) {
+                // what the row does not see becomes -inf, 32 positions at a time
+                bool hidden = (nval & 15) != 0;   // stale rows behind the end in the last product
+                const float fm = turned ? 1.f : fac;
+                mx = -INFINITY;
 #pragma unroll 1
-                for (int c = 0; c < 16; ++c) {
-                    const uint32_t t = tb + 8 * c;
-                    uint32_t x[8];
-                    tc_ld8(sa + 8 * c, x);
-                    if (!(c & 3)) {
-                        const uint32_t inside = ones(nval - 8 * c);
-                        see = inside;
-                        const int d0 = (int)t - (int)nc;   // drafted number of bit 0
-                        if (d0 > -32 && on) {
-                            if (!p.mask) {
-                                see &= ones((int)tok - d0 + 1);
-                            } else {
-                                const int k = c >> 2;
-                                const uint32_t lo = k == 0 ? mk[0] : k == 1 ? mk[1] : k == 2 ? mk[2] : mk[3];
-                                const uint32_t hi = k == 0 ? mk[1] : k == 1 ? mk[2] : k == 2 ? mk[3] : mk[4];
-                                see &= __funnelshift_r(lo, hi, d0 & 31) | ones(-d0);
-                            }
-                        }
-                        kp = (int32_t)t + lane;
-                        if (!by_slot && (kpos || p.window || p.slopes) && lane < nval - 8 * c) kp = tree_kpos(p, kpos, b, t + lane, nc);
-                        if (by_slot) {
-                            if (p.window) see &= ~ones(qp - (int32_t)p.window + 1 - (int32_t)t);
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t x[32];
+                    tc_ld32(sa + 32 * c, x);
+                    const int32_t t = (int32_t)(tb + 32 * c), d0 = t - (int)nc;   // drafted number of bit 0
+                    const uint32_t inside = ones(nval - 32 * c);
+                    uint32_t see = inside;   // bit e: this row sees position t + e
+                    if (d0 > -32 && on) {
+                        if (!p.mask) {
+                            see &= ones((int)tok - d0 + 1);
                         } else {
-                            if (kpos) see &= __ballot_sync(0xffffffffu, kp >= 0);
-                            if (p.window) {
+                            const uint32_t lo = c == 0 ? mk[0] : c == 1 ? mk[1] : c == 2 ? mk[2] : mk[3];
+                            const uint32_t hi = c == 0 ? mk[1] : c == 1 ? mk[2] : c == 2 ? mk[3] : mk[4];
+                            see &= __funnelshift_r(lo, hi, d0 & 31) | ones(-d0);
+                        }
+                    }
+                    if (by_slot) {
+                        if (p.window) see &= ~ones(qp - (int32_t)p.window + 1 - t);
+                    } else {
+                        const int32_t kp = c == 0 ? kc[0] : c == 1 ? kc[1] : c == 2 ? kc[2] : kc[3];
+                        if (kpos) see &= __ballot_sync(0xffffffffu, kp >= 0);
+                        if (p.window) {
 #pragma unroll 4
-                                for (int e = 0; e < 32; ++e)
-                                    if (qp - __shfl_sync(0xffffffffu, kp, e) >= (int32_t)p.window) see &= ~(1u << e);
-                            }
-                        }
-                        hidden |= on && see != inside;
-                    }
-                    tc_wait_ld(x);
-                    float v[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(x[e]) * fac;
-                    if (p.cap > 0.f) tree_cap_all(v, cap2);
-                    if (p.slopes) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const int32_t k = by_slot ? (int32_t)t + e : __shfl_sync(0xffffffffu, kp, 8 * (c & 3) + e);
-                            v[e] = fmaf(slope, (float)(k - qp), v[e]);
+                            for (int e = 0; e < 32; ++e)
+                                if (qp - __shfl_sync(0xffffffffu, kp, e) >= (int32_t)p.window) see &= ~(1u << e);
                         }
                     }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        if (!((see >> e) & 1u)) v[e] = -INFINITY;
-                        mx = fmaxf(mx, v[e]);
-                        x[e] = __float_as_uint(v[e]);
-                    }
-                    see >>= 8;
+                    hidden |= on && see != inside;
                     __syncwarp();
-                    tc_st8(sa + 8 * c, x);
+                    tc_wait_ld(x);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const float v = (see >> e) & 1u ? __uint_as_float(x[e]) * fm : -INFINITY;
+                        mx = fmaxf(mx, v);
+                        x[e] = __float_as_uint(v);
+                    }
+                    tc_st32(sa + 32 * c, x);
                 }
                 tc_wait_st();
-                if (!whole && bar_or(bar, bar_n, hidden)) {
+                if (bar_or(bar, bar_n, hidden)) {
                     // values that some row does not see must be finite, or
                     // 0 * v would reach it
                     const uint32_t vx = 2 * i + 1, va = stage0 + (vx % tp.ns) * slot;

@@ -599,3 +599,14 @@ def test_parts_of_a_cluster_in_a_graph(vbs, gpu, clean_errors, hd, tokens, limit
         np.testing.assert_allclose(out.cpu().numpy(), c.want()[0], rtol=0, atol=4 * TOL)
     gpu.synchronize_device(gpu.get_device(0))
     assert vbs.last_error() == "ok"
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("tokens,hd,n_ctx", [(7, 64, 500), (33, 128, 700), (33, 256, 300), (5, 128, 2000)])
+def test_queries_behind_the_last_token(case, bad, tokens, hd, n_ctx):
+    """A padded batch: what the queries of tokens that are not there hold
+    reaches neither the rows nor the weights."""
+    c = case(seqs=3, tokens=tokens, nqh=8, nkh=2, hd=hd, n_ctx=(n_ctx, 130, 64), n_tok=[1, tokens - 2, 0], seed=tokens)
+    for b in range(3):
+        c.q[b, c.n_tok[b]:] = bad
+    c.check(weights=True)

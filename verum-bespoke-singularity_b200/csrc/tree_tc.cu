@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
 
     // the queries start on their way before anything else is known
     TcQ<128> q;
-    if (warp < TC_LOADER) tc_q_load(p, R0 + 16 * warp + (lane & 7), kvh, b, q);
+    if (warp < TC_LOADER) tc_q_load(p, R0 + 16 * warp + (lane & 7), p.n_tokens * p.G, kvh, b, q);   // (rows behind n_tok too: their scores are nobody's)
     if (warp == TC_LOADER && lane == 0) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tp.km) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tp.vm) : "memory");
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
             const uint32_t r0 = 16 * warp + 8 * (g & 1), x = g >> 1, n0 = TREE_TC_ROWS * ((g + 1) >> 1) + 16 * warp + 8 * ((g + 1) & 1);
             if (x * TREE_TC_ROWS + r0 >= nrows) break;
             TcQ<128> next;
-            if (n0 < nrows) tc_q_load(p, R0 + n0 + (lane & 7), kvh, b, next);
+            if (n0 < nrows) tc_q_load(p, R0 + n0 + (lane & 7), p.n_tokens * p.G, kvh, b, next);
             const float f = tc_q_store(p, q, smem + tp.q_off + x * q_bytes, TREE_TC_ROWS * 16, q_bytes / 2, r0 + (lane & 7), chunks);
             if (lane < 8) fac_sm[x * TREE_TC_ROWS + r0 + lane] = f;
             q = next;

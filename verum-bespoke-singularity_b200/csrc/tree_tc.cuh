@@ -150,9 +150,9 @@ __device__ __forceinline__ void halves(float2 p, uint32_t &hi, uint32_t &lo) {
 template <int D> struct TcQ { float4 x[D / 32][2]; };   // up to D dims
 
 template <int D>
-__device__ __forceinline__ void tc_q_load(const TreeParams &p, uint32_t row, uint32_t kvh, uint32_t b, TcQ<D> &q) {
+__device__ __forceinline__ void tc_q_load(const TreeParams &p, uint32_t row, uint32_t limit, uint32_t kvh, uint32_t b, TcQ<D> &q) {
     const int lane = threadIdx.x & 31;
-    const bool on = row < p.n_tokens * p.G;   // rows behind n_tok are read too: no need to wait for the lengths
+    const bool on = row < limit;
     const uint32_t rr = on ? row : 0u, tok = tree_token(p, rr);
     // whole 32-byte sectors where they are aligned: half a sector a lane
     // fetches each twice, the L1 left beside the stages is too small for it

@@ -13,8 +13,8 @@
 // CTA = (KV head, up to WT_TILES tiles of 128 positions, sequence); K tiles
 // by TMA into a ring; queries in row tiles of 128 (64 above head_dim 128)
 // as the second operand, both halves into one accumulator; tiles alternate
-// between two streams of 4 warps with an accumulator each, so exponentials
-// run beside the next product. Waits are bounded as in tree_tc.cu.
+// between two streams of 4 warps with two accumulators each, so exponentials
+// run beside the next products. Waits are bounded as in tree_tc.cu.
 #include "tree_tc.cuh"
 
 #include <algorithm>
@@ -28,7 +28,7 @@ constexpr int WT_LOADER = WT_SOFT / 32, WT_ISSUER = WT_LOADER + 1;
 constexpr uint32_t WT_BLK = TREE_TC_SP * 128u, WT_TILES = 64;
 
 // words of the state behind the queries (bytes)
-constexpr uint32_t W_FULL = 0, W_EMPTY = 64, W_S = 128, W_F = 144, W_END = 160, W_TMEM = 168, W_BAD = 172, W_QMAX = 176;
+constexpr uint32_t W_FULL = 0, W_EMPTY = 64, W_S = 128, W_F = 160, W_END = 192, W_TMEM = 200, W_BAD = 204, W_QMAX = 208;
 constexpr uint32_t W_ROW = 256;                          // per row: factor and lse (8 bytes), query position and slope (8 bytes)
 constexpr uint32_t W_POS = W_ROW + 128 * 16, W_SUM = W_POS, W_BYTES = W_SUM + WT_TILES * TREE_TC_SP * 4;
 
@@ -89,9 +89,9 @@ __global__ void __launch_bounds__(WT_THREADS, 1) tree_weights_kernel(const __gri
                 mbar_init(base + W_FULL + 8 * s, 1);
                 mbar_init(base + W_EMPTY + 8 * s, 1);
             }
-            for (uint32_t w = 0; w < 2; ++w) {
-                mbar_init(base + W_S + 8 * w, 1);
-                mbar_init(base + W_F + 8 * w, 4);
+            for (uint32_t a = 0; a < 4; ++a) {
+                mbar_init(base + W_S + 8 * a, 1);
+                mbar_init(base + W_F + 8 * a, 4);
             }
             mbar_init(base + W_END, 1);
             *bad = 0;
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) tree_weights_kernel(const __gri
         load(0, 0);
         it = 1;
     } else if (warp == WT_ISSUER) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + W_TMEM), "r"(256u) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + W_TMEM), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         int32_t hi = (int32_t)0x80000000;   // highest query position, for the tiles inside everybody's window
         if (p.window)
@@ -109,6 +109,23 @@ __global__ void __launch_bounds__(WT_THREADS, 1) tree_weights_kernel(const __gri
         hi = __reduce_max_sync(0xffffffffu, hi);
         if (lane == 0) *reinterpret_cast<int32_t *>(hs + W_QMAX) = hi;
     }
+    // a row tile's queries; the first one's do not wait for the attention
+    float qf[2] = {0.f, 0.f};
+    auto queries = [&](uint32_t rt) {
+        TcQ<D> q[D > 128 ? 1 : 2];
+        const uint32_t row = 8 * warp + (lane & 7);
+#pragma unroll
+        for (int g = 0; g < (D > 128 ? 1 : 2); ++g) tc_q_load(p, rt * wp.rows + row + 64 * g, R, kvh, b, q[g]);
+#pragma unroll 1
+        for (int g = 0; g < (D > 128 ? 1 : 2); ++g) {
+            const float f = tc_q_store(p, q[0], smem + wp.q_off, wp.rows * 16, q_lo, row + 64 * g, chunks);
+            if (g) qf[1] = f;
+            else qf[0] = f;
+            if constexpr (D <= 128) q[0] = q[1];
+        }
+        tc_proxy();
+    };
+    if (warp < WT_LOADER) queries(0);
     for (uint32_t i = threadIdx.x; i < ntl * TREE_TC_SP; i += WT_THREADS) sums[i] = 0.f;
     tc_before();
     __syncthreads();
@@ -133,37 +150,41 @@ __global__ void __launch_bounds__(WT_THREADS, 1) tree_weights_kernel(const __gri
         const uint32_t lead = warp == WT_ISSUER ? tc_elect() : 0u;
         const float cap2 = p.cap * TREE_LOG2E;
         bool ok = true;
-        uint32_t s = 0, ph = 0, use[2] = {0, 0};   // issuer: stage and parity; uses of the accumulators
+        uint32_t s = 0, ph = 0;             // issuer: stage and parity
+        uint32_t free = 15u, full = 0u;     // parities of the four accumulators' barriers (the first wait for `free` passes)
         for (uint32_t rt = 0; rt < rts; ++rt) {
-            const uint32_t rows = min(wp.rows, R - rt * wp.rows), N = (rows + 15) / 16 * 16;
+            const uint32_t rows = min(wp.rows, R - rt * wp.rows), N = (rows + 31) / 32 * 32;
             if (warp < WT_LOADER) {
-                // the row tile's queries and numbers
-#pragma unroll 1
-                for (uint32_t g = warp; g < wp.rows / 8; g += WT_SOFT / 32) {
-                    const uint32_t row = 8 * g + (lane & 7), gr = rt * wp.rows + row;
-                    TcQ<D> q;
-                    tc_q_load(p, gr, kvh, b, q);
-                    const float f = tc_q_store(p, q, smem + wp.q_off, wp.rows * 16, q_lo, row, chunks);
+                // the row tile's queries and numbers: all loads first
+                constexpr int NG = D > 128 ? 1 : 2;   // 8s of rows per warp
+                if (rt) queries(rt);
+                float z[NG], sl[NG];
+                int32_t qp[NG];
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const uint32_t row = 8 * (warp + 8 * g) + (lane & 7), rr = row < rows ? rt * wp.rows + row : 0u, tok = tree_token(p, rr);
+                    z[g] = row < rows ? __ldcg(p.lse + (uint64_t)(b * p.nkh + kvh) * (p.n_tokens * p.G) + rr) : -INFINITY;
+                    qp[g] = tree_qpos(p, b, tok, nc);
+                    sl[g] = p.slopes ? p.slopes[kvh * p.G + (rr - tok * p.G)] * TREE_LOG2E : 0.f;
+                }
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const uint32_t row = 8 * (warp + 8 * g) + (lane & 7);
                     if (lane < 8) {
-                        const bool on = row < rows;
-                        const uint32_t rr = on ? gr : 0u, tok = tree_token(p, rr);
-                        const float z = on ? __ldcg(p.lse + (uint64_t)(b * p.nkh + kvh) * (p.n_tokens * p.G) + rr) : -INFINITY;
                         // a row that is not there or sees nothing: weight 2^(0 - inf) = 0
-                        row_fl[row] = z == -INFINITY ? make_float2(0.f, INFINITY) : make_float2(f, z);
-                        row_ps[row] = make_int2(tree_qpos(p, b, tok, nc),
-                                                p.slopes ? __float_as_int(p.slopes[kvh * p.G + (rr - tok * p.G)] * TREE_LOG2E) : 0);
+                        row_fl[row] = z[g] == -INFINITY ? make_float2(0.f, INFINITY) : make_float2(qf[g], z[g]);
+                        row_ps[row] = make_int2(qp[g], __float_as_int(sl[g]));
                     }
                 }
-                tc_proxy();
             }
             named_bar_sync(1, WT_SOFT + 32);   // queries in place
             if (warp == WT_ISSUER) {
                 const uint32_t id = (1u << 4) | ((N >> 3) << 17) | ((TREE_TC_SP >> 4) << 24), qp = wp.rows * 16;
                 const uint64_t dk = tc_desc_sw(stage0, 16u, 1024u), dq = tc_desc(stage0 + wp.q_off, qp, 128u);
                 for (uint32_t i = 0; ok && i < ntl; ++i) {
-                    const uint32_t sw = i & 1;
-                    ok = all(!*bad && waits(base + W_FULL + 8 * s, ph) && (!use[sw] || waits(base + W_F + 8 * sw, (use[sw] - 1) & 1u)));
-                    ++use[sw];
+                    const uint32_t sw = i & 3;
+                    ok = all(!*bad && waits(base + W_FULL + 8 * s, ph) && waits(base + W_F + 8 * sw, (free >> sw) & 1u));
+                    free ^= 1u << sw;
                     if (!ok) break;
                     tc_after();
                     const uint64_t d = dk + s * (slot / 16);
@@ -188,7 +209,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) tree_weights_kernel(const __gri
                 }
             } else {
                 for (uint32_t i = w; ok && i < ntl; i += 2) {
-                    const uint32_t tb = t0 + i * TREE_TC_SP, t = tb + r, sa = tmem + ((32u * wq) << 16) + 128 * w;
+                    const uint32_t tb = t0 + i * TREE_TC_SP, t = tb + r, sw = i & 3, sa = tmem + ((32u * wq) << 16) + 128 * sw;
                     const bool in = t < t1;
                     const int32_t kp = in ? tree_kpos(p, kpos, b, t, nc) : -1;
                     const bool seen = in && (!kpos || kp >= 0);            // by some row
@@ -210,36 +231,39 @@ __global__ void __launch_bounds__(WT_THREADS, 1) tree_weights_kernel(const __gri
                                 for (int x = 0; x < 4; ++x) rows_see[x] |= ones(hi - 32 * x) & ~ones(lo - 32 * x);
                         }
                     }
-                    ok = all(!*bad && waits(base + W_S + 8 * w, use[0] & 1u));
-                    ++use[0];
+                    ok = all(!*bad && waits(base + W_S + 8 * sw, (full >> sw) & 1u));
+                    full ^= 1u << sw;
                     if (!ok) break;
                     tc_after();
                     float sum = 0.f;
                     if (!drafts && !edge && !p.slopes && !(p.cap > 0.f)) {
+                        uint32_t x[2][32];
+                        tc_ld32(sa, x[0]);
+                        tc_wait_ld(x[0]);
+#pragma unroll
+                        for (uint32_t c = 0; c < 128; c += 32) {   // the next 32 on their way
+                            if (c >= N) break;
+                            if (c + 32 < N) tc_ld32(sa + c + 32, x[(c / 32 + 1) & 1]);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) {
+                                const float2 fl = row_fl[c + e];
+                                sum += ex2(fmaf(__uint_as_float(x[(c / 32) & 1][e]), fl.x, -fl.y));
+                            }
+                            if (c + 32 < N) tc_wait_ld(x[(c / 32 + 1) & 1]);
+                        }
+                    } else {
 #pragma unroll 1
                         for (uint32_t c = 0; c < N; c += 16) {
                             uint32_t x[16];
                             tc_ld16(sa + c, x);
-                            tc_wait_ld(x);
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                const float2 fl = row_fl[c + e];
-                                sum += ex2(fmaf(__uint_as_float(x[e]), fl.x, -fl.y));
-                            }
-                        }
-                    } else {
-#pragma unroll 1
-                        for (uint32_t c = 0; c < N; c += 8) {
-                            uint32_t x[8];
-                            tc_ld8(sa + c, x);
                             const uint32_t bits = (c < 64 ? (c < 32 ? rows_see[0] : rows_see[1]) : (c < 96 ? rows_see[2] : rows_see[3])) >> (c & 31);
                             tc_wait_ld(x);
-                            float y[8];
+                            float y[16];
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(x[e]) * row_fl[c + e].x;
+                            for (int e = 0; e < 16; ++e) y[e] = __uint_as_float(x[e]) * row_fl[c + e].x;
                             if (p.cap > 0.f) tree_cap_all(y, cap2);
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) {
+                            for (int e = 0; e < 16; ++e) {
                                 const float2 fl = row_fl[c + e];
                                 const int2 ps = row_ps[c + e];
                                 float v = y[e];
@@ -252,7 +276,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) tree_weights_kernel(const __gri
                     if (seen) sums[i * TREE_TC_SP + r] += sum;
                     tc_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(base + W_F + 8 * w);
+                    if (lane == 0) mbar_arrive(base + W_F + 8 * sw);
                 }
             }
             named_bar_sync(1, WT_SOFT + 32);   // the row tile is through (its products were waited for by those who read them)
@@ -276,7 +300,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) tree_weights_kernel(const __gri
         }
         __syncwarp();
         tc_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
 }
 

@@ -208,10 +208,13 @@ __global__ void __launch_bounds__(WT_THREADS, 1) tree_weights_kernel(const __gri
                     if (++s == wp.ns) { s = 0; ph ^= 1u; }
                 }
             } else {
+                auto kp_at = [&](uint32_t t) { return t < t1 ? tree_kpos(p, kpos, b, t, nc) : -1; };
+                int32_t kn = kp_at(t0 + w * TREE_TC_SP + r);   // the next tile's, ahead
                 for (uint32_t i = w; ok && i < ntl; i += 2) {
                     const uint32_t tb = t0 + i * TREE_TC_SP, t = tb + r, sw = i & 3, sa = tmem + ((32u * wq) << 16) + 128 * sw;
                     const bool in = t < t1;
-                    const int32_t kp = in ? tree_kpos(p, kpos, b, t, nc) : -1;
+                    const int32_t kp = kn;
+                    kn = kp_at(t + 2 * TREE_TC_SP);
                     const bool seen = in && (!kpos || kp >= 0);            // by some row
                     const bool drafts = tb + TREE_TC_SP > nc;              // the mask decides
                     const bool edge = p.window && (kpos || drafts || qmax - (int32_t)tb >= (int32_t)p.window);
@@ -240,16 +243,20 @@ __global__ void __launch_bounds__(WT_THREADS, 1) tree_weights_kernel(const __gri
                         uint32_t x[2][32];
                         tc_ld32(sa, x[0]);
                         tc_wait_ld(x[0]);
+                        // the next 32 on their way (behind N: columns that nobody reads); short code, it starts cold
+#pragma unroll 1
+                        for (uint32_t c = 0; c < N; c += 64) {
 #pragma unroll
-                        for (uint32_t c = 0; c < 128; c += 32) {   // the next 32 on their way
-                            if (c >= N) break;
-                            if (c + 32 < N) tc_ld32(sa + c + 32, x[(c / 32 + 1) & 1]);
+                            for (int u = 0; u < 2; ++u) {
+                                if (c + 32 * u >= N) break;
+                                tc_ld32(sa + ((c + 32 * u + 32) & 127), x[u ^ 1]);
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) {
-                                const float2 fl = row_fl[c + e];
-                                sum += ex2(fmaf(__uint_as_float(x[(c / 32) & 1][e]), fl.x, -fl.y));
+                                for (int e = 0; e < 32; ++e) {
+                                    const float2 fl = row_fl[c + 32 * u + e];
+                                    sum += ex2(fmaf(__uint_as_float(x[u][e]), fl.x, -fl.y));
+                                }
+                                tc_wait_ld(x[u ^ 1]);
                             }
-                            if (c + 32 < N) tc_wait_ld(x[(c / 32 + 1) & 1]);
                         }
                     } else {
 #pragma unroll 1

@@ -226,6 +226,18 @@ def test_select_long(vbs, n, keep, lists):
         assert (idx[0, 0, h] == ref.select(x[0, 0, h], n, keep, 4, min(keep - 4, 64))).all()
 
 
+@pytest.mark.parametrize("n", [260, 2600])
+@pytest.mark.parametrize("share", range(1, 26, 2))
+def test_select_border(vbs, n, share):
+    """The border falls into every kind of value, its ends and neighbours."""
+    kinds = np.asarray([np.nan, np.inf, -np.inf, 1e-44, -1e-44, 0.0, -0.0, 3.4e38, -3.4e38, 1.0, -1.0, 1.1754944e-38, -1.1754944e-38], dtype=np.float32)
+    x = kinds[np.random.default_rng(share).integers(0, 13, (1, 1, 2, n))]
+    keep = n * share // 26
+    idx, _ = run_select(vbs, x, [n], keep, 3, 2)
+    for h in range(2):
+        assert (idx[0, 0, h] == ref.select(x[0, 0, h], n, keep, 3, 2)).all()
+
+
 def test_select_short_and_empty(vbs):
     x = scores_of("plain", np.random.default_rng(0), (1, 3, 2, 300))
     idx, count = run_select(vbs, x, [0, 5, 20], 20, 3, 3)

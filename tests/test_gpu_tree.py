@@ -610,3 +610,23 @@ def test_queries_behind_the_last_token(case, bad, tokens, hd, n_ctx):
     for b in range(3):
         c.q[b, c.n_tok[b]:] = bad
     c.check(weights=True)
+
+
+@pytest.mark.parametrize("tokens,nqh,nkh", [(2, 4, 2), (5, 2, 1), (16, 1, 1)])
+@pytest.mark.parametrize("slow", ["first", "every", "none"])
+def test_wide_heads_uneven_blocks(case, tokens, nqh, nkh, slow):
+    """Heads of 256, many stages a part, some blocks much slower than others
+    (holes with values that are not finite): no warp runs ahead of a stage."""
+    def holes(rng, c):
+        kp = np.tile(np.arange(c.M), (c.S, 1))
+        if slow == "first":
+            kp[:, 3] = -1
+        elif slow == "every":
+            kp[:, 5::128] = -1
+        return kp
+
+    c = case(seqs=80, tokens=tokens, nqh=nqh, nkh=nkh, hd=256, n_ctx=(1500 - tokens, 700, 1301), limit=1500, spare=0, pos=0, k_pos=holes, seed=tokens)
+    c.v[np.broadcast_to((c.k_pos < 0)[:, None, :], c.v.shape[:3])] = np.inf
+    first = c.check()
+    for _ in range(20):
+        assert np.array_equal(c.run(), first, equal_nan=True)

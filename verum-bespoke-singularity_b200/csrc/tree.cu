@@ -16,8 +16,8 @@
 // tree_mma_kernel (few rows, or head_dim above 128): stages of 64 positions of
 // K and V come by TMA (128-byte swizzle: ldmatrix without bank conflicts), the
 // warps take blocks of 16 positions in turn and wait for stages, never for one
-// another; the last warp through a stage fills it again: mma.sync m16n8k16 with
-// fp32 accumulators, online softmax with a lazy rescale, joined at the end. fp32
+// another; the warp that ends a stage's last block fills it again: mma.sync
+// m16n8k16 with fp32 accumulators, online softmax with a lazy rescale, joined at the end. fp32
 // queries and weights are two fp16 halves each (x = hi + lo to 2^-22); both
 // halves run on the same B fragments into the same accumulators, 16 rows per
 // warp. Bound by memory up to some 40 rows. (More rows: tree_tc.cu.)
@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ int32_t sh_min[C::NW];
     __shared__ __align__(8) uint64_t bars[2 * C::NST];   // full, empty
-    __shared__ uint32_t used[C::NST], issued[C::NST];   // warps that are through with the stage; 1 + the stage's last tile
+    __shared__ uint32_t used[C::NST], issued[C::NST];   // blocks of the stage that are through; 1 + the stage's last tile
     __shared__ int sh_bad;
     __shared__ __align__(8) float2 sh_ml[C::ROWS];       // the part's, where parts are joined in a cluster
     volatile int *bad = &sh_bad;
@@ -107,15 +107,33 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
     // stage c's keys and values (one thread)
     auto load = [&](uint32_t c) {
         const uint32_t s = c % C::NST, st = sbase + s * C::STAGE;
-        issued[s] = c + 1;
+        asm volatile("st.release.cta.shared.u32 [%0], %1;" ::"r"(smem_u32(&issued[s])), "r"(c + 1) : "memory");
         mbar_arrive_expect_tx(full0 + 8 * s, 2 * blks * C::BOX);
         for (uint32_t k = 0; k < blks; ++k) tree_tma(st + k * C::BOX, &km, 64 * k, t0 + c * C::SP, kvh, b, full0 + 8 * s);
         for (uint32_t k = 0; k < blks; ++k) tree_tma(st + C::HALF + k * C::BOX, &vm, 64 * k, t0 + c * C::SP, kvh, b, full0 + 8 * s);
     };
+    // tile c's load has been issued: the tile before it in its stage is done with
+    auto under_way = [&](uint32_t c) -> bool {
+        const uint32_t at = smem_u32(&issued[c % C::NST]);
+        uint32_t n;
+        auto there = [&]() {
+            asm volatile("ld.acquire.cta.shared.u32 %0, [%1];" : "=r"(n) : "r"(at) : "memory");
+            return n > c;
+        };
+        if (there()) return true;
+        const uint64_t since = global_ns();
+        while (!there()) {
+            if (*bad || global_ns() - since > kWaitNs) {
+                *bad = 1;
+                return false;
+            }
+        }
+        return true;
+    };
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::NST; ++s) {
             mbar_init(full0 + 8 * s, 1);
-            mbar_init(empty0 + 8 * s, C::NW);
+            mbar_init(empty0 + 8 * s, 4 * WR);
             used[s] = issued[s] = 0;
         }
         sh_bad = 0;
@@ -202,16 +220,17 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
     auto kp_at = [&](uint32_t t) { return lane < 16 && t + lane < t1 ? tree_kpos(p, kpos, b, t + lane, nc) : 0x7FFFFFFF; };
     const bool want_pos = kpos || p.window || p.slopes;
     int32_t kn = want_pos ? kp_at(t0 + 16 * wp) : 0;
-    // Every warp waits for every stage and gives it back, with a block in it
-    // or not: a barrier's parity tells two neighbouring phases apart, so a
-    // warp must not miss one (with 8 warps and 3 stages it could)
-    for (uint32_t c = 0; c < nch; ++c) {
-        const uint32_t j = 4 * c + (wp & 3), tb = t0 + 16 * j, st = sbase + c % C::NST * C::STAGE;
-        const bool mine = c % (WP / 4) == (uint32_t)wp / 4 && tb < t1;
+    // A barrier's parity tells two neighbouring phases apart. 8 warps and 3
+    // stages: a warp visits every other tile, so a stage may be a whole tile
+    // behind the one that the warp is at; it looks first whether that is under
+    // way. (All warps through all stages instead: 131 us for the 110 of 16
+    // sequences of up to 8000 positions with a window of 4096.)
+    for (uint32_t tb = t0 + 16 * wp, j = wp; tb < t1; tb += 16 * WP, j += WP) {
+        const uint32_t c = j / 4, st = sbase + c % C::NST * C::STAGE;
         const int32_t kp = kn;
-        if (mine && want_pos) kn = kp_at(tb + 16 * WP);
-        if (!__all_sync(0xffffffffu, !*bad && waits(full0 + 8 * (c % C::NST), (c / C::NST) & 1u))) break;
-        if (mine) {
+        if (want_pos) kn = kp_at(tb + 16 * WP);
+        if (!__all_sync(0xffffffffu, !*bad && (WP == 4 || under_way(c)) && waits(full0 + 8 * (c % C::NST), (c / C::NST) & 1u))) break;
+        {
             const uint32_t kst = st + 16 * (j & 3) * 128, vst = kst + C::HALF, sw = lane & 7;
             float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, sl[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -363,11 +382,11 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
         }
         __syncwarp();
         if (lane == 0) {
-            // the stage's last warp fills it again (it waits for arrivals
+            // the stage's last block fills it again (it waits for arrivals
             // that are all made by then)
             const uint32_t s = c % C::NST;
             mbar_arrive(empty0 + 8 * s);
-            if (atomicAdd(&used[s], 1u) == C::NW - 1) {
+            if (atomicAdd(&used[s], 1u) == 4 * WR - 1) {
                 used[s] = 0;
                 if (c + C::NST < nch && waits(empty0 + 8 * s, (c / C::NST) & 1u)) load(c + C::NST);
             }

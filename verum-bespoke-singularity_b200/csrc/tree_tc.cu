@@ -8,7 +8,8 @@
 // tiles of 128. Tiles alternate between two streams, each with its own
 // scores (128 columns of tensor memory), accumulator (128 columns) and
 // softmax state, so one stream's softmax runs beside the other's products;
-// the two are joined at the end.
+// the two are joined at the end. Or 256 rows, 128 a stream, that share the
+// tiles: half the bytes of K and V, twice the time of a tile.
 //  * One thread stages K and V tiles (32 KB each at head_dim 128) into a ring
 //    with TMA, 64 dims x 128 positions a box, rows of 128 bytes with the
 //    128-byte swizzle. The image is a K-major operand for Q K^T (MN =
@@ -19,10 +20,12 @@
 //  * One thread issues tcgen05.mma: S = Qhi K^T + Qlo K^T (both operands in
 //    shared memory), O += Phi V + Plo V (P from tensor memory).
 //  * 2 x 4 softmax warps, a thread per row: the scores are read once for the
-//    maximum, and again, 16 columns at a time, for the weights, which go back
-//    over them as fp16 halves (columns 32 c .. + 15 the high, + 16 .. + 31
-//    the low halves of positions 32 c ..) and are announced 64 positions at a
-//    time. The sums are rescaled when the maximum moves by more than TREE_LAZY.
+//    maximum, and again for the weights, which go back over them as fp16
+//    halves (columns 32 c .. + 15 the high, + 16 .. + 31 the low halves of
+//    positions 32 c ..) and are announced 64 positions at a time. The sums are
+//    rescaled when the maximum moves by more than TREE_LAZY. A load from tensor
+//    memory answers after some 250 cycles while products run, so 32 or 64
+//    columns go at a time (16 each: 504 rows x 8192 positions 57.3 us, then 53.3).
 //  * The tensor cores cut accumulators instead of rounding them, towards zero:
 //    left in tensor memory over 30 tiles a result lost 8.5e-6 (zero-mean
 //    values; 1.5e-5 and more with values of one sign). So an accumulator lives

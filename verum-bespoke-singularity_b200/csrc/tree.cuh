@@ -46,37 +46,41 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// cap * tanh(x / cap) in log2 units from y = x / cap. Below 1 the Pade form
-// y (945 + 105 y^2 + y^4) / (945 + 420 y^2 + 15 y^4) of tanh, off by 6e-8 at
-// most, so that small scores keep their relative accuracy (1 - 2 / (e^2y + 1)
-// alone would be off by 2^-24 of the cap); above 1 (e^2y - 1) / (e^2y + 1).
+// cap * tanh(x / cap) in log2 units from y = x / cap. Below 0.55 tanh's series
+// up to y^15, without a division or an exponential (its next term is 4e-8 of
+// the value there): small scores keep their relative accuracy, which 1 - 2 /
+// (e^2y + 1) alone, off by 2^-24 of the cap, would not. Below 1 the Pade form
+// y (945 + 105 y^2 + y^4) / (945 + 420 y^2 + 15 y^4), off by 6e-8 at most;
+// above 1 (e^2y - 1) / (e^2y + 1).
+__device__ __forceinline__ float tree_cap_low(float y, float cap2) {
+    const float z = y * y;
+    float t = fmaf(z, -1.4558344e-3f, 3.5921281e-3f);   // -929569 / 638512875, 21844 / 6081075
+    t = fmaf(z, t, -8.8632355e-3f);                     // -1382 / 155925
+    t = fmaf(z, t, 2.1869489e-2f);                      // 62 / 2835
+    t = fmaf(z, t, -5.3968254e-2f);                     // -17 / 315
+    t = fmaf(z, t, 1.3333333e-1f);                      // 2 / 15
+    t = fmaf(z, t, -3.3333333e-1f);
+    return cap2 * fmaf(y * z, t, y);
+}
 __device__ __forceinline__ float tree_cap(float y, float cap2) {
     const float a = fminf(fabsf(y), 30.f), z = y * y, e = ex2(a * (2.f * TREE_LOG2E));
     const bool small = a < 1.f;
     const float num = small ? a * fmaf(z, z + 105.f, 945.f) : e - 1.f;
     const float den = small ? fmaf(z, fmaf(z, 15.f, 420.f), 945.f) : e + 1.f;
-    return y != y ? y : copysignf(cap2 * __fdividef(num, den), y);
+    const float low = tree_cap_low(y, cap2);
+    return y != y ? y : a < 0.55f ? low : copysignf(cap2 * __fdividef(num, den), y);
 }
 
-// The same for several scores of a warp: while all are below 0.55 (scores well
-// under the cap) by tanh's series up to y^15, without a division or an
-// exponential; its next term is 4e-8 of the value there.
+// The same for several scores of a warp, without the upper forms while all are
+// below 0.55 (scores well under the cap). A score's result is its own either
+// way: the vote also counts scores that nobody sees.
 template <int N> __device__ __forceinline__ void tree_cap_all(float (&y)[N], float cap2) {
     float top = 0.f;
 #pragma unroll
     for (int e = 0; e < N; ++e) top = fmaxf(top, fabsf(y[e]));
     if (__all_sync(0xffffffffu, top < 0.55f)) {   // (a NaN stays one either way)
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const float z = y[e] * y[e];
-            float t = fmaf(z, -1.4558344e-3f, 3.5921281e-3f);   // -929569 / 638512875, 21844 / 6081075
-            t = fmaf(z, t, -8.8632355e-3f);                     // -1382 / 155925
-            t = fmaf(z, t, 2.1869489e-2f);                      // 62 / 2835
-            t = fmaf(z, t, -5.3968254e-2f);                     // -17 / 315
-            t = fmaf(z, t, 1.3333333e-1f);                      // 2 / 15
-            t = fmaf(z, t, -3.3333333e-1f);
-            y[e] = cap2 * fmaf(y[e] * z, t, y[e]);
-        }
+        for (int e = 0; e < N; ++e) y[e] = tree_cap_low(y[e], cap2);
     } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) y[e] = tree_cap(y[e], cap2);

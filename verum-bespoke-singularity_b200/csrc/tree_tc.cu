@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
         const bool active = wq < aw, on = ri < nrows;
         const uint32_t rr = R0 + (on ? ri : 0u), tok = tree_token(p, rr), head = kvh * p.G + (rr - tok * p.G);
         const uint32_t sa = tmem + ((32u * wq) << 16) + 128 * w, oa = sa + 256;
-        const float fac = fac_sm[ri];
+        const float fac = on ? fac_sm[ri] : 0.f;
         const int32_t qp = tree_qpos(p, b, tok, nc), qmax = *reinterpret_cast<const int32_t *>(hs + H_QMAX);
         const float slope = p.slopes ? p.slopes[head] * TREE_LOG2E : 0.f;
         const int32_t *kpos = p.k_pos ? p.k_pos + (uint64_t)(p.k_pos_per_head ? b * p.nkh + kvh : b) * p.max_ctx : nullptr;
@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
             // the tile's key positions where they are not its slots, lane: 32 k + lane
             const bool by_slot = !kpos && tb + TREE_TC_SP <= nc;
             int32_t kc[4] = {kn[0], kn[1], kn[2], kn[3]};
-            if (!context && (kpos || p.window || p.slopes)) {
+            if (!by_slot && !context && (kpos || p.window || p.slopes)) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) kc[k] = 32 * k + lane < nval ? tree_kpos(p, kpos, b, tb + 32 * k + lane, nc) : 0;
             }
@@ -402,7 +402,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                     for (int e = 0; e < 16; e += 2) mx = max3(mx, x[e], x[e + 1]);
 #pragma unroll
                     for (int e = 0; e < 16; ++e) s[e] = __float_as_uint(x[e]);
-                    __syncwarp();
                     tc_st16(sa + 16 * c, s);
                 }
                 tc_wait_st();

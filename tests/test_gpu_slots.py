@@ -459,3 +459,58 @@ def test_prompt_eviction_and_drafts_together(vbs):
     want, _ = ref.attend(q.cpu().numpy().reshape(S, 1, nqh, hd), *rows, n_ctx.cpu().numpy(), [1] * S, hd ** -0.5, window=140,
                          q_pos=last[:, None], k_pos=k_pos[0].cpu().numpy())
     np.testing.assert_allclose(out.cpu().numpy(), want, rtol=0, atol=1e-4)
+
+
+def test_offsets_past_32_bits(vbs, gpu):
+    """Three sequences 2^31 + 8 elements apart, the last behind 2^32: store,
+    attention (both kernels, with weights) and moves as in caches of their own."""
+    import torch
+    S, ctx, H, hd, n, stride = 3, 320, 2, 64, 300, (1 << 31) + 8
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 20 GB")
+    big = [torch.empty(2 * stride + ctx * H * hd, dtype=torch.float16, device="cuda") for _ in range(2)]
+    view = [[b[s * stride:s * stride + ctx * H * hd].view(ctx, H, hd) for s in range(S)] for b in big]
+    for side in view:
+        for x in side:
+            x.fill_(0.5)
+    kv = vbs.KvDesc(k=big[0].data_ptr(), v=big[1].data_ptr(), n_layers=1, max_ctx=ctx, n_kv_heads=H, head_dim=hd, n_seqs=S,
+                    head_major=0, seq_stride=stride)
+    rng = np.random.default_rng(1)
+    x = dev(rng.standard_normal((2, S * n, H, hd)), np.float32)
+    zero, slot, seq = dev(np.zeros(S * n), np.int32), dev(np.tile(np.arange(n), S), np.int32), dev(np.repeat(np.arange(S), n), np.int32)
+    vbs.rope_store(vbs.rope_plan(hd), kv, 0, 0, 0, 0, x[0].data_ptr(), x[1].data_ptr(), S * n, zero.data_ptr(), slot.data_ptr(),
+                   seq=seq.data_ptr())
+    half = x.to(torch.float16).view(2, S, n, H, hd)
+    for side in range(2):
+        for s in range(S):
+            assert torch.equal(view[side][s][:n], half[side, s]) and (view[side][s][n:] == 0.5).all()
+
+    small = [torch.stack(side).contiguous() for side in view]          # the same, without gaps
+    near = vbs.KvDesc(k=small[0].data_ptr(), v=small[1].data_ptr(), n_layers=1, max_ctx=ctx, n_kv_heads=H, head_dim=hd, n_seqs=S,
+                      head_major=0, seq_stride=ctx * H * hd)
+    for T in (1, 40):
+        q = dev(rng.standard_normal((S, T, 8, hd)), np.float32)
+        n_ctx = dev([n - T, 17, n - T], np.int32)
+        got = []
+        for c in (kv, near):
+            out, w = torch.zeros_like(q), torch.zeros((S, H, ctx), device="cuda")
+            t = vbs.TreeDesc(n_q_heads=8, n_tokens=T, scale=0.125, ctx_limit=ctx, n_ctx=n_ctx.data_ptr(), weights_out=w.data_ptr())
+            work = torch.empty(vbs.tree_workspace(c, t), dtype=torch.uint8, device="cuda")
+            vbs.attention_tree(c, 0, t, q.data_ptr(), out.data_ptr(), work.data_ptr(), work.numel())
+            torch.cuda.synchronize()
+            got.append((out, w))
+        assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+    idx, count = dev(np.arange(0, n, 2), np.int32), dev([n // 2] * S, np.int32)
+    g = vbs.GatherDesc(n_max=n // 2, idx=idx.data_ptr(), count=count.data_ptr())
+    apart = [torch.zeros_like(s) for s in small]
+    to = vbs.KvDesc(k=apart[0].data_ptr(), v=apart[1].data_ptr(), n_layers=1, max_ctx=ctx, n_kv_heads=H, head_dim=hd, n_seqs=S,
+                    head_major=0, seq_stride=ctx * H * hd)
+    vbs.cache_gather(kv, to, g)
+    vbs.cache_gather(kv, kv, g)
+    torch.cuda.synchronize()
+    for side in range(2):
+        for s in range(S):
+            want = small[side][s][0:n:2]
+            assert torch.equal(apart[side][s][:n // 2], want) and torch.equal(view[side][s][:n // 2], want)
+            assert torch.equal(view[side][s][n // 2:], small[side][s][n // 2:])

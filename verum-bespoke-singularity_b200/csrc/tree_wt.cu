@@ -17,7 +17,8 @@
 // run beside the next products. Waits are bounded as in tree_tc.cu.
 // Bound by the exponentials (2048 cycles of their unit per pair of tiles) and
 // the CTA's start: 57 us with the attention for 128 rows x 4 x 4096 positions
-// of 8 KV heads of 128, some 25 of them this kernel's.
+// of 8 KV heads of 128, some 25 of them this kernel's (66 with inputs that are
+// not in L2).
 #include "tree_tc.cuh"
 
 #include <algorithm>

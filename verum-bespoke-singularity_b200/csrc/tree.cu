@@ -634,41 +634,58 @@ static TreeParts tree_parts(uint64_t ctas, uint64_t slots, uint32_t span, uint32
     return best;
 }
 
-static TreePlan tree_plan(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t, int n_sm) {
-    TreePlan pl = {};
-    const uint32_t G = t->n_q_heads / kv->n_kv_heads, hd = kv->head_dim;
-    pl.rows = t->n_tokens * G;
-    uint32_t span = t->ctx_limit;
-    if (t->window && !t->k_pos) span = (uint32_t)std::min<uint64_t>(span, (uint64_t)t->window + t->n_tokens + 63);
-    const uint64_t heads = (uint64_t)kv->n_kv_heads * kv->n_seqs;
-    auto tiles = [&](uint32_t rows) { return (pl.rows + rows - 1) / rows; };
-    // tree_mma_kernel: 16 rows a CTA (32 above head_dim 128, where a CTA has an
-    // SM to itself); tree_tc_kernel: 128 rows, or 256 of more, which halves
-    // what K and V cost but doubles a CTA. Measured on full SMs, ns per
-    // position and CTA: 30 (head_dim 128), 22 (64) with two CTAs per SM, 22 and 44
-    // (256; 16 and 32 rows); 15 and 28.5 (128; 128 and 256 rows), 10 and 19.5 (64).
-    TreeParts best = {~0ull, 0, 0, false};
-    auto plan = [&](bool tc, uint32_t rows, uint32_t per_sm, uint32_t unit, uint32_t pos_ns, uint32_t cta_ns, const int *clusters) {
-        const TreeParts one = tree_parts(heads * tiles(rows), (uint64_t)per_sm * n_sm, span, unit, pos_ns, cta_ns, rows * hd * 4, clusters);
-        if (one.ns >= best.ns) return;
-        best = one;
-        pl.tc = tc;
-        pl.tile_rows = rows;
-    };
+// The kernels that take `rows` rows of a KV head. tree_mma_kernel: 16 rows a
+// CTA (32 above head_dim 128, where a CTA has an SM to itself);
+// tree_tc_kernel: 128 rows, or 256 of more, which halves what K and V cost
+// but doubles a CTA. Measured on full SMs, ns per position and CTA: 30
+// (head_dim 128), 22 (64) with two CTAs per SM, 22 and 44 (256; 16 and 32
+// rows); 15 and 28.5 (128; 128 and 256 rows), 10 and 19.5 (64).
+struct TreeKind {
+    bool tc;
+    uint32_t rows, per_sm, unit, pos_ns, cta_ns;   // pos_ns in tenths
+    const int *clusters;
+};
+static uint32_t tree_kinds(uint32_t hd, uint32_t rows, TreeKind (&k)[3]) {
+    uint32_t n = 0;
     if (hd > 128) {
-        if (pl.rows <= 16) plan(false, 16, 1, 64, 220, 6000, tree_fit[2]);
-        else plan(false, 32, 1, 64, 440, 6000, tree_fit[3]);
+        k[n++] = rows <= 16 ? TreeKind{false, 16, 1, 64, 220, 6000, tree_fit[2]} : TreeKind{false, 32, 1, 64, 440, 6000, tree_fit[3]};
     } else {
         const bool big = hd > 64;
-        plan(false, 16, 2, 64, big ? 300 : 220, 4000, tree_fit[big ? 1 : 0]);
-        if (pl.rows > 16) plan(true, TREE_TC_ROWS, 1, TREE_TC_SP, big ? 150 : 100, 9000, tree_fit[4]);   // (16 rows are one CTA's of the other kernel)
-        if (pl.rows > TREE_TC_ROWS) plan(true, 2 * TREE_TC_ROWS, 1, TREE_TC_SP, big ? 285 : 195, 12000, tree_fit[4]);
+        k[n++] = {false, 16, 2, 64, big ? 300u : 220u, 4000, tree_fit[big ? 1 : 0]};
+        if (rows > 16) k[n++] = {true, TREE_TC_ROWS, 1, TREE_TC_SP, big ? 150u : 100u, 9000, tree_fit[4]};   // (16 rows are one CTA's of the other kernel)
+        if (rows > TREE_TC_ROWS) k[n++] = {true, 2 * TREE_TC_ROWS, 1, TREE_TC_SP, big ? 285u : 195u, 12000, tree_fit[4]};
+    }
+    return n;
+}
+
+// Positions that a plan counts with.
+static uint32_t tree_span(const vbs_cu_tree_t *t) {
+    return t->window && !t->k_pos ? (uint32_t)std::min<uint64_t>(t->ctx_limit, (uint64_t)t->window + t->n_tokens + 63) : t->ctx_limit;
+}
+static size_t tree_aligned(size_t n) { return (n + 255) / 256 * 256; }
+
+static TreePlan tree_plan(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t, int n_sm) {
+    TreePlan pl = {};
+    const uint32_t G = t->n_q_heads / kv->n_kv_heads, hd = kv->head_dim, span = tree_span(t);
+    pl.rows = t->n_tokens * G;
+    const uint64_t heads = (uint64_t)kv->n_kv_heads * kv->n_seqs;
+    TreeParts best = {~0ull, 0, 0, false};
+    TreeKind kinds[3];
+    const uint32_t n_kinds = tree_kinds(hd, pl.rows, kinds);
+    for (uint32_t i = 0; i < n_kinds; ++i) {
+        const TreeKind &k = kinds[i];
+        const uint32_t tiles = (pl.rows + k.rows - 1) / k.rows;
+        const TreeParts one = tree_parts(heads * tiles, (uint64_t)k.per_sm * n_sm, span, k.unit, k.pos_ns, k.cta_ns, k.rows * hd * 4, k.clusters);
+        if (one.ns >= best.ns) continue;
+        best = one;
+        pl.tc = k.tc;
+        pl.tile_rows = k.rows;
+        pl.row_tiles = tiles;
     }
     pl.per_split = best.per;
     pl.n_splits = best.parts;
     pl.joined = best.joined;
-    pl.row_tiles = tiles(pl.tile_rows);
-    auto take = [&](size_t n) { const size_t at = pl.bytes; pl.bytes += (n + 255) / 256 * 256; return at; };
+    auto take = [&](size_t n) { const size_t at = pl.bytes; pl.bytes += tree_aligned(n); return at; };
     if (pl.n_splits > 1 && !pl.joined) {
         pl.ml = take(heads * pl.row_tiles * pl.n_splits * pl.tile_rows * sizeof(float2));
         pl.o = take(heads * pl.row_tiles * pl.n_splits * pl.tile_rows * kv->head_dim * sizeof(float));
@@ -676,6 +693,59 @@ static TreePlan tree_plan(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t, int n_s
     if (t->weights_out) pl.lse = take(heads * pl.rows * sizeof(float));
     pl.bytes = std::max<size_t>(pl.bytes, 256);
     return pl;
+}
+
+// Bytes that every plan up to this description's ctx_limit, n_tokens and
+// window fits into. A plan's own need is no guide to another's: it falls to
+// nothing where its parts become a cluster and comes back where they do not
+// fit one, and a shorter call may take wider row tiles.
+// A plan of x positions costs no more than any kernel's plan that fills the
+// SMs once (more CTAs than that: the one without parts), slope * x + fixed;
+// it costs at least its positions' share of the SMs, its CTAs' fixed time and
+// its join. So the room between the two bounds CTAs x parts, and as a minimum
+// of lines less a line it is largest at an end or where two lines meet.
+static size_t tree_bytes(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t, int n_sm) {
+    const uint32_t hd = kv->head_dim, rows = t->n_tokens * (t->n_q_heads / kv->n_kv_heads);
+    const uint64_t heads = (uint64_t)kv->n_kv_heads * kv->n_seqs;
+    const double span = tree_span(t);
+    size_t bytes = 0;
+    for (uint32_t r = std::min(rows, 16u); heads <= 16ull * 2 * n_sm; r = std::min(rows, r + 16)) {   // (all row tiles are multiples of 16)
+        TreeKind kinds[3];
+        const uint32_t n = tree_kinds(hd, r, kinds);
+        double slope[3], fixed[3], at[5] = {0., span};
+        uint32_t n_at = 2;
+        bool any = false;
+        for (uint32_t i = 0; i < n; ++i) {
+            const TreeKind &k = kinds[i];
+            const uint64_t slots = (uint64_t)k.per_sm * n_sm, ctas = heads * ((r + k.rows - 1) / k.rows), once = slots / ctas, waves = (ctas + slots - 1) / slots;
+            const double pos = k.pos_ns / 10., unit = k.unit * pos;
+            slope[i] = once ? pos / once : waves * pos;
+            fixed[i] = once ? unit / once + unit + k.cta_ns + TREE_MERGE_NS + slots * (double)(k.rows * hd * 4) / TREE_MERGE_RATE : waves * (unit + k.cta_ns);
+            any |= ctas <= 16 * slots;   // (tree_parts ends after one part)
+            for (uint32_t j = 0; j < i; ++j) {
+                const double x = (fixed[i] - fixed[j]) / (slope[j] - slope[i]);
+                if (x > 0. && x < span) at[n_at++] = x;
+            }
+        }
+        for (uint32_t i = 0; i < n; ++i) {
+            const TreeKind &k = kinds[i];
+            const uint64_t slots = (uint64_t)k.per_sm * n_sm, ctas = heads * ((r + k.rows - 1) / k.rows);
+            if (ctas > 16 * slots) continue;
+            double room = 0.;
+            for (uint32_t a = 0; a < n_at; ++a) {
+                double least = slope[0] * at[a] + fixed[0];
+                for (uint32_t j = 1; j < n; ++j) least = std::min(least, slope[j] * at[a] + fixed[j]);
+                room = std::max(room, least - TREE_MERGE_NS - ctas * (k.pos_ns / 10.) * at[a] / slots);
+            }
+            // (tree_parts cuts off fractions of a nanosecond: one of a CTA's time, one of the join's)
+            const double most = (room + 1) / ((k.cta_ns - 1.) / slots + (double)(k.rows * hd * 4) / TREE_MERGE_RATE);
+            const uint64_t units = ((uint64_t)span + k.unit - 1) / k.unit;
+            const uint64_t all = std::min((uint64_t)most, ctas * std::min<uint64_t>(units, TREE_MAX_PARTS)) * k.rows;
+            bytes = std::max(bytes, tree_aligned(all * sizeof(float2)) + tree_aligned(all * hd * sizeof(float)));
+        }
+        if (r == rows || !any) break;
+    }
+    return std::max<size_t>(bytes + (t->weights_out ? tree_aligned(heads * rows * sizeof(float)) : 0), 256);
 }
 
 static bool tree_desc_ok(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t) {
@@ -763,7 +833,7 @@ size_t vbs_cu_tree_workspace(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t) {
     }
     DevState *d = backend_current();
     if (!d) { latch_error("vbs_cu_tree_workspace: no usable device"); return 0; }
-    return tree_plan(kv, t, d->n_sm).bytes;
+    return tree_bytes(kv, t, d->n_sm);
 }
 
 int vbs_cu_attention_tree(const vbs_cu_kv_t *kv, uint32_t layer, const vbs_cu_tree_t *t, const float *q, float *out, void *work,

@@ -352,8 +352,8 @@ VBS_API int vbs_cu_rope_store(const vbs_cu_rope_t *r, const vbs_cu_kv_t *kv, uin
  * workspace, n_ctx and n_tok are read on the device (above it: reported as a
  * bad length). softcap 0, or 1e-6 and up. Sums and softmax are fp32; fp32
  * queries (below 2^100) and weights enter the tensor cores as two fp16 halves
- * each (exact to about 2^-22). A value that is not finite makes what sees it
- * not finite. */
+ * each (exact to about 2^-22, small weights to 2^-34 of the row's largest).
+ * A value that is not finite makes what sees it not finite. */
 typedef struct {
     uint32_t n_q_heads, n_tokens;
     float scale, softcap;

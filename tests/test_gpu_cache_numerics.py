@@ -1,0 +1,71 @@
+"""vbs_cu_attention_tree where its numbers are stretched: weights far below
+a row's largest, positions far apart, keys that are infinite."""
+import numpy as np
+import pytest
+
+from test_gpu_tree import TOL, Case
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture()
+def case(vbs, gpu, clean_errors):
+    yield lambda **kw: Case(vbs, **kw)
+    gpu.synchronize_device(gpu.get_device(0))
+    assert vbs.last_error() == "ok"
+
+
+# ---- weights far below the largest -------------------------------------------
+# A weight reaches the product as two fp16 halves beside a largest weight of
+# 2^10 or more. Below, one key weighs 1 and all others 2^-31 to 2^-33: their
+# high halves are 2 to 8 of fp16's smallest steps (2^-24), rounded, their low
+# halves nothing. Rounding each by half a step at random leaves a sum of 1500
+# of them off by 0.2% (one deviation), and the spread of the weights, denser
+# towards the small ones, by a bias of 0.3%: 2% is eight deviations and the
+# bias. (Where they are lost, the whole of a part is missing.)
+PLANS = [(1, 2, 2, 64, 1, 3000), (5, 4, 2, 128, 1, 5000), (2, 32, 32, 256, 5, 1500), (5, 32, 8, 256, 20, 1500), (40, 4, 2, 128, 1, 3000),
+         (33, 32, 8, 96, 5, 1500), (17, 32, 8, 64, 20, 1500)]
+
+
+@pytest.mark.parametrize("tokens,nqh,nkh,hd,seqs,n_ctx", PLANS)
+@pytest.mark.parametrize("where", ["first", "last"])
+def test_many_small_weights_beside_a_large_one(case, tokens, nqh, nkh, hd, seqs, n_ctx, where):
+    c = case(seqs=seqs, tokens=tokens, nqh=nqh, nkh=nkh, hd=hd, n_ctx=(n_ctx,), seed=hd + tokens)
+    rng = np.random.default_rng(tokens)
+    at = 0 if where == "first" else n_ctx - 1
+    c.q[...] = 0.0
+    c.q[..., 0] = 1.0 / c.scale
+    c.q[..., 1] = 2.0 ** -7 / c.scale        # spreads the scores between fp16's steps
+    c.k[..., 0] = -np.log(2.0) * rng.uniform(31, 33, c.k.shape[:3])
+    c.k[..., 1] = rng.uniform(-1, 1, c.k.shape[:3])
+    c.k[:, :, at, :2] = 0.0
+    c.v[...] = rng.uniform(0.5, 1.5, c.v.shape)
+    c.v[:, :, at] = 0.0                      # the large weight's own part: nothing hides the others'
+    got, (want, _) = c.run(), c.want()
+    assert 0 < want.max() < 1e-5
+    np.testing.assert_allclose(got, want, rtol=0.02, atol=0)
+
+
+@pytest.mark.parametrize("tokens,nqh,nkh,hd,seqs,n_ctx", PLANS)
+@pytest.mark.parametrize("base", [0.0, 3e6])
+def test_scores_that_rise_by_the_most_a_reference_takes(case, tokens, nqh, nkh, hd, seqs, n_ctx, base):
+    """Every 128 positions weigh 2^15.94 times the ones before: the weights
+    stay below fp16's largest number, however the scores round (3e6: to
+    steps of a half). The last ones are nearly all that is left."""
+    c = case(seqs=seqs, tokens=tokens, nqh=nqh, nkh=nkh, hd=hd, n_ctx=(n_ctx,), seed=hd)
+    c.q[...] = 0.0
+    c.q[..., 0] = 100.0 / c.scale
+    c.q[..., 1] = 1.0 / c.scale
+    c.k[..., 0] = base / 100.0
+    c.k[..., 1] = (np.arange(c.M) // 128) * (15.94 * np.log(2.0))
+    c.v[...] = np.abs(c.v) + np.float16(0.5)
+    got = c.run()
+    for i in range(tokens):
+        end = n_ctx + i + 1
+        first = (end - 1) // 128 * 128
+        for h in range(nqh):
+            last = c.v[:, h // (nqh // nkh), first:end].astype(np.float64).mean(1)
+            # steps of 15.94 +- 0.1 (keys in fp16) +- 1 (products and scores of 3e6): the 128 before weigh
+            # 2^-14.8 each, their values up to 12 times the last ones'
+            share = 128.0 / (end - first) * 2.0 ** -14.8
+            np.testing.assert_allclose(got[:, i, h], last, rtol=share * 12 + 1e-5, atol=0)

@@ -26,9 +26,12 @@
 // memory up to some 40 rows. (More rows: tree_tc.cu.)
 //  * Queries are scaled per row by a power of two to 2^8..2^9, so neither half
 //    leaves fp16's range; the power goes into the score's factor (exact).
-//  * The softmax reference stays 6 below the running maximum (log2 units), so
-//    weights are 2^6 at the first and at most 2^14 before a rescale: small
-//    weights keep their low half above fp16's smallest numbers.
+//  * The softmax reference stays 10 below the running maximum (log2 units), so
+//    the largest weight is 2^10 at first and below 2^16 before a rescale. fp16's
+//    smallest step, 2^-24, is then 2^-34 of the largest weight, and what it cuts
+//    off 100,000 small weights beside a large one 3e-6 of it (half a step each).
+//    (With 6 below, what lay under 2^-31 of the largest added nothing to the
+//    result but all of itself to the sum.)
 //  * The tensor cores cut their accumulators instead of rounding them: every
 //    accumulation loses half a unit of the last place towards zero, 480 of them
 //    8.5e-6 of the result. Each block's sum therefore starts at zero and is
@@ -306,7 +309,7 @@ __global__ void __launch_bounds__(TreeCfg<HD, WR, WP>::THREADS) tree_mma_kernel(
                 float mx = fmaxf(fmaxf(x[h][0], x[h][1]), fmaxf(x[h][2], x[h][3]));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                if (mx > mref[h] + TREE_LAZY) {
+                if (mx - mref[h] > TREE_LAZY) {   // (what the weights' exponents are: large scores round)
                     const float r = ex2(mref[h] - (mx - TREE_BELOW));   // 0 on the first block
                     mref[h] = mx - TREE_BELOW;
                     l[h] *= r;

@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
             }
             tc_after();
             if (r == 0) reinterpret_cast<volatile uint32_t *>(hs + H_ACC)[w] = 0;
-            // plain: the scores as the product left them, times the row's factor
+            // plain: the scores as the product left them; the row's factor goes with the reference
             const bool turned = p.slopes || p.cap > 0.f, plain = whole && !turned;
             const float cap2 = p.cap * TREE_LOG2E;
             float mx = -INFINITY;
@@ -374,7 +374,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                     mx = fmaxf(mx, max32(s[c & 1]));
                     if (c < 3) tc_wait_ld(s[(c + 1) & 1]);
                 }
-                mx *= fac;
             } else if (turned) {
                 // capped, with slope * (key position - query position) added,
                 // back into tensor memory
@@ -468,7 +467,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                     if (bar_or(bar, bar_n, odd)) {
                         // rare: the rows that see such values put their part into
                         // the accumulator, then they become zeros for the product
-                        const float nm = mx > mref + TREE_LAZY ? mx - TREE_BELOW : mref;
+                        const float nm = mx - mref > TREE_LAZY ? mx - TREE_BELOW : mref;
                         const float bs = nm == -INFINITY ? 0.f : nm;
                         for (uint32_t c = 0; c < chunks; ++c) {
                             uint32_t y[8];
@@ -510,16 +509,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                 }
             }
             // running reference; the sums follow when it moves
-            const bool moves = mx > mref + TREE_LAZY;
+            // (the largest weight's exponent, rounded as the weights' are)
+            const float f1 = plain ? fac : 1.f;
+            const bool moves = fmaf(mx, f1, -mref) > TREE_LAZY;
             if (__any_sync(0xffffffffu, moves)) {
-                const float f = !moves ? 1.f : ex2(mref - (mx - TREE_BELOW));   // 0 on the first tile
-                if (moves) mref = mx - TREE_BELOW;
+                const float to = fmaf(mx, f1, -TREE_BELOW), f = !moves ? 1.f : ex2(mref - to);   // 0 on the first tile
+                if (moves) mref = to;
                 l.x *= f;
                 l.y *= f;
 #pragma unroll
                 for (int k = 0; k < 128; ++k) o[k] *= f;
             }
-            const float f1 = plain ? fac : 1.f, b1 = mref == -INFINITY ? 0.f : mref;
+            const float b1 = mref == -INFINITY ? 0.f : mref;
             const float2 f = make_float2(f1, f1), bs = make_float2(-b1, -b1);
             uint32_t s[2][32];
             tc_ld32(sa, s[0]);

@@ -311,12 +311,13 @@ VBS_API int vbs_cu_rope_init(vbs_cu_rope_t *r, uint32_t head_dim, uint32_t rot_d
  * sequence seq[i] (NULL: sequence 0) of `layer` as fp16, rounded as the
  * engine's CACHE primitive does. pos: [n_tokens][n_axes], any int32. q rows
  * of q_stride floats (0: n_q_heads * head_dim), k and v rows of kv_stride
- * floats (0: n_kv_heads * head_dim); q_out rows have no gaps and q_out may
- * be q when q has none either. n_q_heads 0 (q and q_out NULL) only stores;
- * k and v NULL only turns the queries (kv, slot and seq are not used and
- * may be NULL). slot -1 stores nothing for that token, whose seq is not
- * looked at. Slots of one call are distinct; given twice, the slot holds a
- * mix of the two tokens. Pointers 16-byte aligned, strides multiples of 4. */
+ * floats (0: n_kv_heads * head_dim); q_out rows have no gaps, and q_out is q
+ * (which then has none either) or overlaps no row of q, k or v. n_q_heads 0
+ * (q and q_out NULL) only stores; k and v NULL only turns the queries (kv,
+ * slot and seq are not used and may be NULL). slot -1 stores nothing for that
+ * token, whose seq is not looked at. Slots of one call are distinct; given
+ * twice, the slot holds a mix of the two tokens. Pointers 16-byte aligned,
+ * strides multiples of 4. */
 VBS_API int vbs_cu_rope_store(const vbs_cu_rope_t *r, const vbs_cu_kv_t *kv, uint32_t layer, const float *q,
                               uint64_t q_stride, float *q_out, uint32_t n_q_heads, const float *k, const float *v,
                               uint64_t kv_stride, uint32_t n_tokens, const int32_t *pos, const int32_t *seq,

@@ -683,6 +683,14 @@ bool overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
     return a && b && x < y + nb && y < x + na;
 }
 
+// Any of n rows of `row` bytes, `stride` bytes apart from a, and nb bytes from b.
+static bool rows_overlap(const void *a, uint64_t n, unsigned __int128 stride, uint64_t row, const void *b, uint64_t nb) {
+    const unsigned __int128 x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    if (!a || !b) return false;
+    const unsigned __int128 i = y < x + row ? 0 : (y - x - row) / stride + 1;   // the first row that ends behind b
+    return i < n && x + i * stride < y + nb;
+}
+
 }  // namespace vbs
 
 using namespace vbs;
@@ -757,6 +765,13 @@ int vbs_cu_rope_store(const vbs_cu_rope_t *r, const vbs_cu_kv_t *kv, uint32_t la
             ok = kv_stride >= row && kv_stride % 4 == 0 &&
                  !((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15);
         }
+    }
+    if (ok && turn) {   // queries are written while other tokens' inputs are read
+        const uint64_t qrow = (uint64_t)n_q_heads * r->head_dim * 4, krow = store ? (uint64_t)kv->n_kv_heads * r->head_dim * 4 : 0;
+        const uint64_t all = n_tokens * qrow;
+        ok = (q == q_out || !rows_overlap(q, n_tokens, (unsigned __int128)q_stride * 4, qrow, q_out, all)) &&
+             (!store || (!rows_overlap(k, n_tokens, (unsigned __int128)kv_stride * 4, krow, q_out, all) &&
+                         !rows_overlap(v, n_tokens, (unsigned __int128)kv_stride * 4, krow, q_out, all)));
     }
     if (!ok) {
         latch_error("vbs_cu_rope_store: invalid arguments");

@@ -344,7 +344,7 @@ VBS_API int vbs_cu_rope_store(const vbs_cu_rope_t *r, const vbs_cu_kv_t *kv, uin
  *    window also saves reading what it leaves out.
  *  - weights_out: [n_seqs][kv head][max_ctx], the attention weights of every
  *    slot below n_ctx + n_tok, summed over the tokens and the query heads of
- *    its KV head, added to weights_in (NULL: 0; may be weights_out itself);
+ *    its KV head, added to weights_in (NULL: 0; weights_out itself or apart);
  *    slots from there on are left as they were.
  * n_q_heads is a multiple of the cache's n_kv_heads, at most 256 of them per
  * KV head; n_tokens at most 4096; q and out do not overlap, 16-byte aligned.

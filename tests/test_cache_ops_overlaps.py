@@ -62,3 +62,20 @@ def test_rope_store_takes_what_does_not_overlap(vbs, kw):
         pytest.skip("a GPU is present: the call would run")
     got = rope(vbs, **kw)
     assert "no usable device" in got
+
+
+W = 2 * NK * 64 * 4                       # bytes of the weights: sequences, heads, max_ctx
+
+
+@pytest.mark.parametrize("shift,fine", [(0, True), (W, True), (-W, True), (16, False), (-16, False), (W - 16, False), (16 - W, False)])
+def test_attention_weights_in_over_weights_out(vbs, shift, fine):
+    """The same buffer, or none of it: each position's sum is read and written
+    by a thread of its own."""
+    import torch
+    if fine and torch.cuda.is_available():
+        pytest.skip("a GPU is present: the call would run")
+    kv = vbs.KvDesc(k=KV, v=KV + (1 << 30), n_layers=1, max_ctx=64, n_kv_heads=NK, head_dim=HD, n_seqs=2, head_major=0, seq_stride=64 * NK * HD)
+    tree = vbs.TreeDesc(n_q_heads=NQ, n_tokens=3, scale=0.125, ctx_limit=64, n_ctx=4096, weights_in=IN + shift, weights_out=IN)
+    for call in (lambda: vbs.tree_workspace(kv, tree),
+                 lambda: vbs.attention_tree(kv, 0, tree, IN + (1 << 20), IN + (2 << 20), IN + (3 << 20), 1 << 20)):
+        assert ("no usable device" if fine else "invalid arguments") in outcome(vbs, call)

@@ -759,7 +759,9 @@ static bool tree_desc_ok(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t) {
     if (!std::isfinite(t->scale) || !(t->softcap >= 0.f) || !std::isfinite(t->softcap) || t->window > 0x7FFFFFFFu) return false;
     if (t->softcap > 0.f && t->softcap < 1e-6f) return false;   // its reciprocal scales the scores
     if ((uint64_t)t->n_tokens * t->n_q_heads > 0x7FFFFFFFu) return false;   // rows of a sequence: CTAs are counted in 32 bits
-    return !(t->weights_in && !t->weights_out);
+    if (t->weights_in && !t->weights_out) return false;
+    const uint64_t w = (uint64_t)kv->n_seqs * kv->n_kv_heads * kv->max_ctx * 4;   // (below 2^63: kv_desc_ok)
+    return t->weights_in == t->weights_out || !overlap(t->weights_in, w, t->weights_out, w);   // all of it or nothing
 }
 
 // Tensor map of one layer's keys or values, boxes of 64 dims x `rows`

@@ -340,7 +340,7 @@ VBS_API int vbs_cu_rope_store(const vbs_cu_rope_t *r, const vbs_cu_kv_t *kv, uin
  *    k_pos[s][slot] ([s][kv head][slot] with k_pos_per_head), rows of max_ctx,
  *    for every slot below n_ctx[s] + n_tok[s], a negative one marking a slot
  *    that nobody sees (padding, a hole); NULL: the slot's number for the
- *    context and q_pos for the new tokens. Within +-2^30. Without k_pos a
+ *    context and q_pos for the new tokens. Less than 2^30 in size. Without k_pos a
  *    window also saves reading what it leaves out.
  *  - weights_out: [n_seqs][kv head][max_ctx], the attention weights of every
  *    slot below n_ctx + n_tok, summed over the tokens and the query heads of

@@ -69,3 +69,16 @@ def test_scores_that_rise_by_the_most_a_reference_takes(case, tokens, nqh, nkh, 
             # 2^-14.8 each, their values up to 12 times the last ones'
             share = 128.0 / (end - first) * 2.0 ** -14.8
             np.testing.assert_allclose(got[:, i, h], last, rtol=share * 12 + 1e-5, atol=0)
+
+
+# ---- positions far apart ------------------------------------------------------
+@pytest.mark.parametrize("tokens,nqh,nkh,hd,kw", [(4, 4, 2, 64, {}), (3, 2, 1, 256, {}), (20, 4, 1, 128, dict(limit=20000, spare=0)),
+                                                  (33, 32, 8, 64, dict(seqs=10))])
+@pytest.mark.parametrize("window", [2 ** 30 - 1, 2 ** 31 - 1])
+def test_windows_over_positions_at_their_limits(case, tokens, nqh, nkh, hd, kw, window):
+    """Queries at the lowest and the highest position there is: the distances
+    between them pass what a 32-bit subtraction of the window's edge holds."""
+    c = case(tokens=tokens, nqh=nqh, nkh=nkh, hd=hd, n_ctx=(300,), window=window, pos=0, tree=True, seed=hd, **kw)
+    c.q_pos[:, ::2] = -(2 ** 30 - 1)
+    c.q_pos[:, 1::2] = 2 ** 30 - 1
+    c.check(weights=True)

@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
                         }
                     }
                     if (by_slot) {
-                        if (p.window) see &= ~ones(qp - (int32_t)p.window + 1 - t);
+                        if (p.window && qp >= (int32_t)p.window) see &= ~ones(qp - (int32_t)p.window + 1 - t);   // (slots are 0 or more)
                     } else {
                         const int32_t kp = c == 0 ? kc[0] : c == 1 ? kc[1] : c == 2 ? kc[2] : kc[3];
                         if (kpos) see &= __ballot_sync(0xffffffffu, kp >= 0);

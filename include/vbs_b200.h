@@ -340,8 +340,8 @@ VBS_API int vbs_cu_rope_store(const vbs_cu_rope_t *r, const vbs_cu_kv_t *kv, uin
  *    k_pos[s][slot] ([s][kv head][slot] with k_pos_per_head), rows of max_ctx,
  *    for every slot below n_ctx[s] + n_tok[s], a negative one marking a slot
  *    that nobody sees (padding, a hole); NULL: the slot's number for the
- *    context and q_pos for the new tokens. Less than 2^30 in size. Without k_pos a
- *    window also saves reading what it leaves out.
+ *    context and q_pos for the new tokens. Less than 2^30 in size. Without
+ *    k_pos a window also saves reading what it leaves out.
  *  - weights_out: [n_seqs][kv head][max_ctx], the attention weights of every
  *    slot below n_ctx + n_tok, summed over the tokens and the query heads of
  *    its KV head, added to weights_in (NULL: 0; weights_out itself or apart);
@@ -354,7 +354,10 @@ VBS_API int vbs_cu_rope_store(const vbs_cu_rope_t *r, const vbs_cu_kv_t *kv, uin
  * bad length). softcap 0, or 1e-6 and up. Sums and softmax are fp32; fp32
  * queries (below 2^100) and weights enter the tensor cores as two fp16 halves
  * each (exact to about 2^-22, small weights to 2^-34 of the row's largest).
- * A value that is not finite makes what sees it not finite. */
+ * A NaN among the keys and a value that is not finite make the rows that see
+ * them not finite. A row that sees an infinite key is not specified: by the
+ * formula its score can be -inf (weight 0), or the cap, and the halves of the
+ * query can make a NaN of it. */
 typedef struct {
     uint32_t n_q_heads, n_tokens;
     float scale, softcap;

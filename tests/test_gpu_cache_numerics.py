@@ -82,3 +82,28 @@ def test_windows_over_positions_at_their_limits(case, tokens, nqh, nkh, hd, kw, 
     c.q_pos[:, ::2] = -(2 ** 30 - 1)
     c.q_pos[:, 1::2] = 2 ** 30 - 1
     c.check(weights=True)
+
+
+# ---- keys that are not finite ---------------------------------------------------
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("tokens,nqh,nkh,hd,kw", [(5, 4, 2, 64, {}), (4, 4, 2, 256, {}), (21, 8, 2, 128, {}),
+                                                  (21, 4, 1, 128, dict(limit=20000, spare=0)), (33, 32, 8, 96, dict(seqs=10))])
+def test_visible_keys_that_are_not_finite(case, bad, cap, tokens, nqh, nkh, hd, kw):
+    """A draft's key, one number of it or all, seen by that draft alone: the
+    other rows meet the formula as always. Its own rows
+    are NaN for a NaN; an infinite key's score depends on how the query
+    splits, so theirs may be anything."""
+    c = case(tokens=tokens, nqh=nqh, nkh=nkh, hd=hd, n_ctx=(300,), cap=cap, tree=True, seed=tokens, **kw)
+    c.sees[:] = np.eye(tokens, dtype=bool)
+    c.k[:, :, 302, 5] = bad
+    c.k[:, :, 303] = bad
+    got, (want, _) = c.run(weights=True), c.want()
+    others = [i for i in range(tokens) if i not in (2, 3)]
+    np.testing.assert_allclose(got[0][:, others], want[:, others], rtol=0, atol=4 * TOL)
+    if np.isnan(bad):
+        assert np.isnan(got[0][:, 2:4]).all()
+    # the weights of the drafts that other rows alone see
+    end = 300 + tokens
+    alone = [300 + i for i in others]
+    assert np.isfinite(got[1][:, :, alone]).all() and (got[1][:, :, end:] == 7.0).all()

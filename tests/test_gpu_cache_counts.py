@@ -4,6 +4,7 @@ and row tiles. A position too few or too many shows, however many there are."""
 import numpy as np
 import pytest
 
+import cache_ops as ref
 from test_gpu_tree import Case, evicted, many, padded
 
 pytestmark = pytest.mark.gpu
@@ -116,3 +117,31 @@ def test_weights_to_their_own_size(case, kw):
         end = int(c.n_ctx[b] + c.n_tok[b])
         np.testing.assert_allclose(got[b, :, :end], wts[b, :, :end], rtol=4e-5, atol=0)
         np.testing.assert_allclose(got[b, :, :end].sum(-1, dtype=np.float64), c.n_tok[b] * c.nqh / c.H, rtol=4e-5)
+
+
+@pytest.mark.parametrize("hd", [104, 128])
+def test_wide_row_tiles_with_few_rows_under_load(case, hd):
+    """Row tiles of 256 that hold at most 128 rows in most sequences: three
+    stages, whose loads come late beside another stream's copies. The result
+    is the same in every run."""
+    import torch
+    c = many(case, 10, 3000, hd=hd, tree=True, seed=hd)
+    c.n_tok = np.minimum(c.n_tok, [33] + [32] * 9)
+    first = c.check(weights=True)
+    k, v, q = c.cache(c.k), c.cache(c.v), c.put(c.q)
+    lists = [c.put(x, np.int32) for x in (c.n_ctx, c.n_tok)] + [c.put(ref.mask_words(c.sees).view(np.int32))]
+    kv, tree = c.kv, c.tree
+    kv.k, kv.v, tree.n_ctx, tree.n_tok, tree.mask = k.data_ptr(), v.data_ptr(), *[x.data_ptr() for x in lists]
+    tree.weights_in = tree.weights_out = None
+    nbytes = c.vbs.tree_workspace(kv, tree)
+    work = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    side, main, big = torch.cuda.Stream(), torch.cuda.Stream(), torch.empty(1 << 29, dtype=torch.uint8, device="cuda")
+    outs = [torch.full(c.q.shape, 7.0, device="cuda") for _ in range(50)]
+    torch.cuda.synchronize()
+    for out in outs:
+        with torch.cuda.stream(side):
+            big[: 1 << 28].copy_(big[1 << 28:])
+        c.vbs.attention_tree(kv, 0, tree, q.data_ptr(), out.data_ptr(), work.data_ptr(), nbytes, main.cuda_stream)
+    torch.cuda.synchronize()
+    for out in outs:
+        assert np.array_equal(out.cpu().numpy(), first)

@@ -203,8 +203,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(const __grid_con
         const uint32_t qlo = q_bytes / 32, lead = tc_elect();   // the low halves' offset, in descriptor units
         for (uint32_t n = 0, s = 0, ph = 0; n < steps; ++n) {
             const uint32_t w = n & 1;
-            // keys here, and this stream's last weights used up
-            if (!all(!*bad && waits(base + H_FULL + 8 * s, ph) && (n < 2 || waits(base + H_O + 8 * w, (n / 2 - 1) & 1u)))) break;
+            // this stream's last weights used up, and then the keys here. In
+            // this order: with an odd number of stages an issuer meets every
+            // other phase of a stage, and a parity tells neighbours apart. The
+            // phase between, values of a tile before, is over once that tile's
+            // second product is; asked earlier, three stages can still be
+            // waiting for those values, and they pass for these keys.
+            if (!all(!*bad && (n < 2 || waits(base + H_O + 8 * w, (n / 2 - 1) & 1u)) && waits(base + H_FULL + 8 * s, ph))) break;
             tc_after();
             const uint64_t d = dk + s * (slot / 16), dq = dq0 + (two && w ? q_bytes / 16 : 0u);
 #pragma unroll

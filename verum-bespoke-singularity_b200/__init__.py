@@ -312,7 +312,8 @@ def rope_store(rope, kv, layer, q, q_out, n_q_heads, k, v, n_tokens, pos, slot, 
 
 
 def tree_workspace(kv, tree) -> int:
-    """Bytes of workspace that attention_tree needs for this description."""
+    """Bytes of workspace that attention_tree needs for this description and
+    every one with a smaller ctx_limit, n_tokens or window."""
     n = int(lib().vbs_cu_tree_workspace(C.byref(kv), C.byref(tree)))
     if not n:
         raise VbsError(f"vbs_cu_tree_workspace: {last_error()}")

@@ -175,9 +175,10 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_store_kernel(const __grid_c
 //     are the counts of kept slots before them.
 // Every warp owns a run of consecutive keys and visits only those, so the
 // counts per warp are all that has to be scanned. Reading twice instead of
-// keeping the keys in shared memory leaves room for four CTAs per SM instead
-// of two: the steps are short and wait for one another, and other CTAs fill
-// the waits (1024 lists of up to 16384: 77.6 us with the keys kept). A cluster
+// keeping the keys in shared memory leaves room for three CTAs per SM (40
+// registers) instead of two: the steps are short and wait for one another, and
+// other CTAs fill the waits (1024 lists of up to 16384: 77.6 us with the keys
+// kept). Bound by instruction issue: 71% of the schedulers' cycles there. A cluster
 // of 2, 4 or 8 CTAs shares a list only where there are few long ones:
 // histograms and counts are then read from the other CTAs' shared memory.
 // ---------------------------------------------------------------------------

@@ -30,7 +30,8 @@
 //    left in tensor memory over 30 tiles a result lost 8.5e-6 (zero-mean
 //    values; 1.5e-5 and more with values of one sign). So an accumulator lives
 //    for one tile, the rows' threads add it to their fp32 sums in registers
-//    (setmaxnreg gives them 232), and a score's low halves go first, while its
+//    (setmaxnreg gives them 232, but the compiler counts with the launch's 168
+//    and spills 352 bytes), and a score's low halves go first, while its
 //    accumulator is small.
 // All waits are bounded; after one ran out the CTA flags the device error
 // word, waits for its copies and products, frees its tensor memory and ends.

@@ -377,7 +377,8 @@ typedef struct {
  * 0 with the error latched for a bad description. It serves this description
  * and every one that differs from it in a smaller ctx_limit, n_tokens or
  * window (no window being the largest) or lacks its weights_out: ask once,
- * for the longest context and the most tokens. The caller owns the
+ * for the longest context and the most tokens. (Drafts take tens of MB,
+ * chunks of thousands of tokens on long contexts hundreds.) The caller owns the
  * workspace: two calls that can overlap in time (other streams, captured
  * graphs) take one each. Nothing in it is kept between calls. */
 VBS_API size_t vbs_cu_tree_workspace(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t);

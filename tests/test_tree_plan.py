@@ -68,9 +68,11 @@ def test_drawn_descriptions(plans):
     assert switched > 30   # the sweeps do cross from one plan to another
 
 
-def test_the_query_stays_near_what_plans_need(plans):
-    """It is an upper bound, not any: a few times the largest plan of the
-    sweep, or the sums of all SMs once full of the widest row tiles."""
-    for hd, nkh, group, n in ((128, 8, 4, 16), (128, 8, 8, 63), (64, 2, 4, 7), (256, 4, 4, 9)):
-        row, = plans([(hd, nkh, 1, group, n, 0, 0, 0, 64, 32768)])
-        assert row[-1][1] <= max(4 * max(plan for plan, *_ in row), 148 * 256 * (8 + 4 * hd) + 512)
+@pytest.mark.parametrize("hd,nkh,group,tokens,limit", [(128, 8, 4, 16, 32768), (128, 8, 8, 63, 32768), (64, 2, 4, 7, 32768), (256, 4, 4, 9, 32768),
+                                                       (128, 8, 4, 512, 131072), (128, 8, 4, 2048, 131072), (256, 8, 4, 300, 131072)])
+def test_the_query_stays_near_what_plans_need(plans, hd, nkh, group, tokens, limit):
+    """It is an upper bound, not any: a few times the largest plan of all
+    shorter calls, or the sums of all SMs once full of the widest row tiles."""
+    counts = sorted(set(range(1, tokens, max(1, tokens // 100))) | {tokens})
+    rows = plans([(hd, nkh, 1, group, n, 0, 0, 0, limit // 256, limit) for n in counts])
+    assert rows[-1][-1][1] <= max(4 * max(plan for row in rows for plan, *_ in row), 148 * 256 * (8 + 4 * hd) + 512)

@@ -698,55 +698,72 @@ static TreePlan tree_plan(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t, int n_s
     return pl;
 }
 
+// The largest min over the lines (slope * x + fixed) less own * x, x up to
+// span: along the lines' lower envelope while it grows.
+struct TreeLine { double slope, fixed; };
+static double tree_room(const TreeLine *l, uint32_t n, double own, double span) {
+    uint32_t j = 0;
+    for (uint32_t i = 1; i < n; ++i)
+        if (l[i].fixed < l[j].fixed || (l[i].fixed == l[j].fixed && l[i].slope < l[j].slope)) j = i;
+    double x = 0.;
+    while (l[j].slope > own) {
+        double to = span;
+        uint32_t next = j;
+        for (uint32_t i = 0; i < n; ++i) {
+            if (l[i].slope >= l[j].slope) continue;
+            const double at = (l[i].fixed - l[j].fixed) / (l[j].slope - l[i].slope);
+            if (at < to) { to = at; next = i; }
+        }
+        x = std::max(x, to);
+        if (next == j) break;
+        j = next;
+    }
+    return l[j].fixed + (l[j].slope - own) * x;
+}
+
 // Bytes that every plan up to this description's ctx_limit, n_tokens and
 // window fits into. A plan's own need is no guide to another's: it falls to
 // nothing where its parts become a cluster and comes back where they do not
 // fit one, and a shorter call may take wider row tiles.
-// A plan of x positions costs no more than any kernel's plan that fills the
-// SMs once (more CTAs than that: the one without parts), slope * x + fixed;
-// it costs at least its positions' share of the SMs, its CTAs' fixed time and
-// its join. So the room between the two bounds CTAs x parts, and as a minimum
-// of lines less a line it is largest at an end or where two lines meet.
+// The plan of x positions costs no more than any that tree_parts looked at:
+// without parts, or with those that fill the SMs w times, w up to 16, each a
+// line in x. It costs at least its positions' share of the SMs, its CTAs'
+// fixed time and its join's. The room between bounds CTAs x parts.
 static size_t tree_bytes(const vbs_cu_kv_t *kv, const vbs_cu_tree_t *t, int n_sm) {
     const uint32_t hd = kv->head_dim, rows = t->n_tokens * (t->n_q_heads / kv->n_kv_heads);
     const uint64_t heads = (uint64_t)kv->n_kv_heads * kv->n_seqs;
-    const double span = tree_span(t);
+    const uint32_t span = tree_span(t);
     size_t bytes = 0;
-    for (uint32_t r = std::min(rows, 16u); heads <= 16ull * 2 * n_sm; r = std::min(rows, r + 16)) {   // (all row tiles are multiples of 16)
+    for (uint32_t r = std::min(rows, 16u);;) {   // (row tiles are multiples of 16; up to 16 rows may have a kernel of their own)
         TreeKind kinds[3];
+        TreeLine lines[3 * 17];
         const uint32_t n = tree_kinds(hd, r, kinds);
-        double slope[3], fixed[3], at[5] = {0., span};
-        uint32_t n_at = 2;
-        bool any = false;
+        uint32_t n_lines = 0, step = 0;
         for (uint32_t i = 0; i < n; ++i) {
             const TreeKind &k = kinds[i];
-            const uint64_t slots = (uint64_t)k.per_sm * n_sm, ctas = heads * ((r + k.rows - 1) / k.rows), once = slots / ctas, waves = (ctas + slots - 1) / slots;
+            const uint64_t slots = (uint64_t)k.per_sm * n_sm, ctas = heads * ((r + k.rows - 1) / k.rows), waves = (ctas + slots - 1) / slots;
             const double pos = k.pos_ns / 10., unit = k.unit * pos;
-            slope[i] = once ? pos / once : waves * pos;
-            fixed[i] = once ? unit / once + unit + k.cta_ns + TREE_MERGE_NS + slots * (double)(k.rows * hd * 4) / TREE_MERGE_RATE : waves * (unit + k.cta_ns);
-            any |= ctas <= 16 * slots;   // (tree_parts ends after one part)
-            for (uint32_t j = 0; j < i; ++j) {
-                const double x = (fixed[i] - fixed[j]) / (slope[j] - slope[i]);
-                if (x > 0. && x < span) at[n_at++] = x;
+            lines[n_lines++] = {waves * pos, waves * (unit + k.cta_ns)};
+            for (uint64_t w = waves; w <= 16; ++w) {
+                const double parts = (double)std::min<uint64_t>(w * slots / ctas, TREE_MAX_PARTS);
+                lines[n_lines++] = {w * pos / parts, w * (unit / parts + unit + k.cta_ns) + TREE_MERGE_NS + w * slots * (double)(k.rows * hd * 4) / TREE_MERGE_RATE};
             }
         }
         for (uint32_t i = 0; i < n; ++i) {
             const TreeKind &k = kinds[i];
             const uint64_t slots = (uint64_t)k.per_sm * n_sm, ctas = heads * ((r + k.rows - 1) / k.rows);
-            if (ctas > 16 * slots) continue;
-            double room = 0.;
-            for (uint32_t a = 0; a < n_at; ++a) {
-                double least = slope[0] * at[a] + fixed[0];
-                for (uint32_t j = 1; j < n; ++j) least = std::min(least, slope[j] * at[a] + fixed[j]);
-                room = std::max(room, least - TREE_MERGE_NS - ctas * (k.pos_ns / 10.) * at[a] / slots);
-            }
+            if (ctas > 16 * slots) continue;   // (tree_parts ends after one part)
+            if (!step) step = k.rows;          // the narrowest that still has parts
+            const double room = tree_room(lines, n_lines, ctas * (k.pos_ns / 10.) / slots, span) - TREE_MERGE_NS;
             // (tree_parts cuts off fractions of a nanosecond: one of a CTA's time, one of the join's)
-            const double most = (room + 1) / ((k.cta_ns - 1.) / slots + (double)(k.rows * hd * 4) / TREE_MERGE_RATE);
-            const uint64_t units = ((uint64_t)span + k.unit - 1) / k.unit;
-            const uint64_t all = std::min((uint64_t)most, ctas * std::min<uint64_t>(units, TREE_MAX_PARTS)) * k.rows;
+            const double most = std::max(0., room + 1) / ((k.cta_ns - 1.) / slots + (double)(k.rows * hd * 4) / TREE_MERGE_RATE);
+            // (tree_parts' last step starts at 16 times the SMs and at most doubles the parts)
+            const uint64_t parts = std::min<uint64_t>(32 * slots, ctas * std::min<uint64_t>((span + k.unit - 1) / k.unit, TREE_MAX_PARTS));
+            const size_t all = (size_t)std::min(most, (double)parts) * k.rows;
             bytes = std::max(bytes, tree_aligned(all * sizeof(float2)) + tree_aligned(all * hd * sizeof(float)));
         }
-        if (r == rows || !any) break;
+        if (r == rows || !step) break;
+        r = std::min<uint64_t>(rows, r / step * step + step);
     }
     return std::max<size_t>(bytes + (t->weights_out ? tree_aligned(heads * rows * sizeof(float)) : 0), 256);
 }
